@@ -499,6 +499,45 @@ int nrf_kilo_clip_adam(float* const* params, float* const* grads, float* const* 
                        const int32_t* live, float grad_scale, float clip_value, float lr, float beta1, float beta2, float eps,
                        int step, float reg_grad_coeff, float reg_loss_coeff, float* loss_accum, nrf_stream_t stream);
 
+/* ---- rows grouped by expert: matrix products with one weight matrix per expert -------------------------------------- */
+
+/* The general form of what nrf_kilo_forward does for its fixed tiny networks: row i of a batch goes through the weights of
+ * expert index[i].  Any number of experts up to 16384, layer sizes up to 65536, up to 2^28 rows, three types.  (The reference
+ * has no counterpart beyond BatchedKiloNeRF's bmm over padded cells, src/models/kilonerf/network.py:123-167.)  Pointers are
+ * contiguous tensors of `dtype`, aligned to one element; the plan and workspaces to 16 bytes.  Every entry point may be
+ * captured into a graph; nothing is read back. */
+enum { NRF_DTYPE_FP32 = 0, NRF_DTYPE_BF16 = 1, NRF_DTYPE_FP16 = 2 };
+enum { NRF_ACT_NONE = 0, NRF_ACT_RELU = 1 };
+
+/* The plan of a batch: index (n_rows,) int32, the expert of each row; a value outside [0, num_experts) means none.  `plan`
+ * (nrf_expert_plan_bytes) starts with int32 counts[num_experts]; from the next multiple of four words
+ * offsets[num_experts + 1], the exclusive sums of counts; from the next multiple of four words order[n_rows]: the rows of
+ * expert 0, of expert 1, ..., each expert's ascending, then the rows of no expert.  What follows is private.  The same
+ * bytes on every run.  workspace: nrf_expert_plan_workspace_bytes (0 for small batches: may be NULL).  Both size
+ * functions return -1 for sizes out of range. */
+int64_t nrf_expert_plan_bytes(int64_t n_rows, int num_experts);
+int64_t nrf_expert_plan_workspace_bytes(int64_t n_rows, int num_experts);
+int nrf_expert_plan(const int32_t* index, int64_t n_rows, int num_experts, void* plan, int64_t plan_bytes, void* workspace,
+                    int64_t workspace_bytes, nrf_stream_t stream);
+
+/* y[i] = act(weight[index[i]] x[i] + bias[index[i]]); rows of no expert give zeros.  x (n_rows, n_in), weight
+ * (num_experts, n_out, n_in), bias (num_experts, n_out) or NULL, y (n_rows, n_out), all of `dtype`; `plan` from
+ * nrf_expert_plan with these n_rows and num_experts.  Sums are fp32, y is rounded once.  NRF_DTYPE_FP32 multiplies three
+ * bf16 terms per operand (24 significand bits, the rule of nrf_mlp_forward_rays_bf16x3); there an operand that is not
+ * finite gives NaN in every output it reaches. */
+int nrf_expert_linear(const void* x, const void* weight, const void* bias, const void* plan, int64_t n_rows, int num_experts,
+                      int n_in, int n_out, int dtype, int act, void* y, nrf_stream_t stream);
+
+/* Its gradients.  With NRF_ACT_RELU, `y` holds the forward's outputs (a row's gradient passes where y > 0); with
+ * NRF_ACT_NONE it may be NULL.  grad_x (n_rows, n_in): zeros for rows of no expert.  grad_weight (num_experts, n_out, n_in)
+ * and grad_bias (num_experts, n_out): every element written, zeros for experts without rows.  Each of the three may be
+ * NULL, but grad_bias needs grad_weight.  Sums are in a fixed order: the same bits on every run. */
+int64_t nrf_expert_linear_backward_workspace_bytes(int64_t n_rows, int num_experts, int n_in, int n_out, int dtype);
+int nrf_expert_linear_backward(const void* grad_y, const void* x, const void* weight, const void* y, const void* plan,
+                               int64_t n_rows, int num_experts, int n_in, int n_out, int dtype, int act, void* grad_x,
+                               void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes,
+                               nrf_stream_t stream);
+
 /* ---- whole forward path: volume_renderer.py:143-153 (render_coarse + render_fine) --- */
 
 typedef struct nrf_render_args {

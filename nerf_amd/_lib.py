@@ -36,6 +36,8 @@ SYMBOLS = (
     "nrf_kilo_dir_table_bytes", "nrf_kilo_encode_dirs", "nrf_kilo_forward_encoded",
     "nrf_kilo_packed_bf16x3_floats", "nrf_kilo_pack_weights_bf16x3", "nrf_kilo_forward_bf16x3",
     "nrf_occ_bricks_bytes", "nrf_occ_pack_bricks", "nrf_kilo_march_count_bricks",
+    "nrf_expert_plan_bytes", "nrf_expert_plan_workspace_bytes", "nrf_expert_plan", "nrf_expert_linear",
+    "nrf_expert_linear_backward_workspace_bytes", "nrf_expert_linear_backward",
 )
 
 P = C.c_void_p
@@ -233,6 +235,16 @@ def lib() -> C.CDLL:
     L.nrf_kilo_cells_scatter.argtypes = [P, P, INT, INT, P, P]
     L.nrf_kilo_cells_gather.restype = INT
     L.nrf_kilo_cells_scatter.restype = INT
+    for name in ("nrf_expert_plan_bytes", "nrf_expert_plan_workspace_bytes"):
+        getattr(L, name).restype = I64
+        getattr(L, name).argtypes = [I64, INT]
+    L.nrf_expert_plan.argtypes = [P, I64, INT, P, I64, P, I64, P]
+    L.nrf_expert_linear.argtypes = [P, P, P, P, I64, INT, INT, INT, INT, INT, P, P]
+    L.nrf_expert_linear_backward_workspace_bytes.restype = I64
+    L.nrf_expert_linear_backward_workspace_bytes.argtypes = [I64, INT, INT, INT, INT]
+    L.nrf_expert_linear_backward.argtypes = [P, P, P, P, P, I64, INT, INT, INT, INT, INT, P, P, P, P, I64, P]
+    for name in ("nrf_expert_plan", "nrf_expert_linear", "nrf_expert_linear_backward"):
+        getattr(L, name).restype = INT
     for name in ("nrf_kilo_pack_weights_transposed", "nrf_kilo_composite_backward", "nrf_kilo_backward", "nrf_l2_reg"):
         getattr(L, name).restype = INT
     for name in ("nrf_kilo_pack_weights", "nrf_kilo_route", "nrf_kilo_forward", "nrf_kilo_march_count",

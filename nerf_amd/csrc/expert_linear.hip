@@ -1,0 +1,408 @@
+// The experts' matrix products (experts.h: rows grouped by expert) and their gradients.
+//
+//   y[i] = act(W[e_i] x[i] + b[e_i])      dz[i] = dy[i] (y[i] > 0)      dx[i] = W[e_i]^T dz[i]
+//   dW[e] = sum_{i of e} dz[i] x[i]^T     db[e] = sum_{i of e} dz[i]
+//
+// One kernel shape serves the three products: C[b][a] = sum_k B[b][k] A[a][k], A the side whose index is contiguous in the
+// output (so a lane's four accumulator rows are one vector store), both operands staged in LDS as [row][k]:
+//   forward   a = output feature (W rows)             b = batch row (x rows, gathered)       k = input
+//   dx        a = input feature (W columns)           b = batch row (dz rows, gathered)      k = output
+//   dW        a = input feature (x columns, gathered) b = output feature (dz columns)        k = the expert's batch rows
+// bf16 / fp16 operands go to the matrix cores as they are.  fp32 operands are split into three bf16 terms on their way into
+// LDS (split3.h: 24 significand bits, six products, fp32 sums): an operand that is not finite gives NaN.  Sums are fp32;
+// an output is rounded to its type once, after bias and relu.
+#include "experts.h"
+#include "split3.h"
+
+namespace {
+
+using nrf::PlanLayout;
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+enum Form { kForward, kDx, kDw };
+
+struct Bf16 {};
+struct Fp16 {};
+struct Fp32 {};
+template <class T> struct Traits;
+template <> struct Traits<Bf16> { typedef unsigned short elem; static constexpr int planes = 1; };
+template <> struct Traits<Fp16> { typedef unsigned short elem; static constexpr int planes = 1; };
+template <> struct Traits<Fp32> { typedef float elem; static constexpr int planes = 3; };
+
+// eight consecutive elements; rows may start at any multiple of the element size (the hardware takes unaligned vectors)
+typedef unsigned u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_u4 __attribute__((ext_vector_type(4), aligned(4)));
+template <class T> struct Oct;
+template <> struct Oct<Fp32> {
+    f32x4 lo, hi;
+    __device__ __forceinline__ void zero() { lo = hi = (f32x4){0.f, 0.f, 0.f, 0.f}; }
+    __device__ __forceinline__ void load(const float* p, int valid) {
+        if (valid >= 8) {
+            lo = *reinterpret_cast<const f32x4_u4*>(p), hi = *reinterpret_cast<const f32x4_u4*>(p + 4);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) lo[j] = j < valid ? p[j] : 0.f, hi[j] = 4 + j < valid ? p[4 + j] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void keep_positive(const Oct& y) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lo[j] = y.lo[j] > 0.f ? lo[j] : 0.f, hi[j] = y.hi[j] > 0.f ? hi[j] : 0.f;
+    }
+    // -> the eight elements of each bf16 term
+    __device__ __forceinline__ void terms(const SplitSel& sel, u32x4 (&out)[3]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float a = j < 2 ? lo[2 * j] : hi[2 * j - 4], b = j < 2 ? lo[2 * j + 1] : hi[2 * j - 3];
+            unsigned p0, p1, p2;
+            split_pair_dot2(sel, a, b, p0, p1, p2);
+            out[0][j] = p0, out[1][j] = p1, out[2][j] = p2;
+        }
+    }
+};
+template <class T, unsigned INF> struct Oct16 {
+    u32x4 v;
+    __device__ __forceinline__ void zero() { v = (u32x4){0, 0, 0, 0}; }
+    __device__ __forceinline__ void load(const unsigned short* p, int valid) {
+        if (valid >= 8) {
+            v = *reinterpret_cast<const u32x4_u2*>(p);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j] = (2 * j < valid ? unsigned(p[2 * j]) : 0u) | (2 * j + 1 < valid ? unsigned(p[2 * j + 1]) << 16 : 0u);
+        }
+    }
+    __device__ __forceinline__ void keep_positive(const Oct16& y) {   // positive: bits in 1 .. INF (NaN lies above)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned lo = y.v[j] & 0xffffu, hi = y.v[j] >> 16;
+            v[j] &= (lo - 1u < INF ? 0xffffu : 0u) | (hi - 1u < INF ? 0xffff0000u : 0u);
+        }
+    }
+    __device__ __forceinline__ void terms(const SplitSel&, u32x4 (&out)[1]) const { out[0] = v; }
+};
+template <> struct Oct<Bf16> : Oct16<Bf16, 0x7f80u> {};
+template <> struct Oct<Fp16> : Oct16<Fp16, 0x7c00u> {};
+
+template <class T>
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+    if constexpr (__is_same(T, Fp16))
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// the products of an operand pair's terms, small ones first
+template <class T>
+__device__ __forceinline__ f32x4 mfma_terms(const u32x4* a, const u32x4* b, f32x4 c) {
+    if constexpr (Traits<T>::planes == 3) {
+        c = mfma16<T>(a[0], b[2], c), c = mfma16<T>(a[1], b[1], c), c = mfma16<T>(a[2], b[0], c);
+        c = mfma16<T>(a[0], b[1], c), c = mfma16<T>(a[1], b[0], c);
+    }
+    return mfma16<T>(a[0], b[0], c);
+}
+
+__device__ __forceinline__ float to_float(float v, Fp32) { return v; }
+__device__ __forceinline__ float to_float(unsigned short v, Bf16) { return __uint_as_float(unsigned(v) << 16); }
+__device__ __forceinline__ float to_float(unsigned short v, Fp16) { return float(__builtin_bit_cast(_Float16, v)); }
+__device__ __forceinline__ float from_float(float v, Fp32) { return v; }
+__device__ __forceinline__ unsigned short from_float(float v, Bf16) { return __builtin_bit_cast(unsigned short, (__bf16)v); }
+__device__ __forceinline__ unsigned short from_float(float v, Fp16) { return __builtin_bit_cast(unsigned short, (_Float16)v); }
+
+// four consecutive outputs, `valid` of them inside the row
+template <class T>
+__device__ __forceinline__ void store4(typename Traits<T>::elem* p, const f32x4& v, int valid) {
+    typedef typename Traits<T>::elem elem;
+    typedef elem vec __attribute__((ext_vector_type(4), aligned(sizeof(elem))));
+    if (valid >= 4) {
+        vec o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = from_float(v[j], T{});
+        *reinterpret_cast<vec*>(p) = o;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < valid) p[j] = from_float(v[j], T{});
+    }
+}
+
+struct ExpertArgs {
+    const void *x, *w, *bias, *y, *g;     // y: the saved outputs whose sign is the relu's mask, or NULL
+    const int* plan;
+    void *out, *db;                       // the product's output; db: dW only, may be NULL
+    float* partial;                       // dW split over the rows: fp32 sums, reduced by a second kernel
+    int64_t n;
+    int E, n_in, n_out, relu, splits;
+};
+
+// The general tile: 64 x 64 outputs, k in steps of 32, four wavefronts of 32 x 32 each, the next step's loads in registers
+// while this step is multiplied.  Any size, any alignment.
+constexpr int kT = 64, kK = 32, kPitch = kK + 8;   // LDS row pitch: 80 B, so that 16 rows' 16 B reads spread over the banks
+
+template <class T, int FORM>
+__global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
+    typedef typename Traits<T>::elem elem;
+    constexpr int P = Traits<T>::planes;
+    __shared__ __align__(16) unsigned short s_a[P][kT][kPitch], s_b[P][kT][kPitch];
+    __shared__ int s_rows[kT];            // forward / dx: the tile's batch rows
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, q = lane >> 4;
+    const int wa = (wave & 1) * 32, wb = (wave >> 1) * 32;
+    const int a0 = blockIdx.y * kT;       // first A row = first output column
+    const PlanLayout L(g.n, g.E);
+    const int* order = g.plan + L.order;
+
+    int expert, b0 = 0, b_count, k_begin = 0, k_end;
+    const int n_a = FORM == kForward ? g.n_out : g.n_in;
+    if (FORM == kDw) {
+        expert = blockIdx.x / g.splits;
+        const int split = blockIdx.x % g.splits;
+        const int first = g.plan[L.offsets + expert], rows = g.plan[expert];
+        const int per = (((rows + g.splits - 1) / g.splits) + kK - 1) / kK * kK;   // whole k steps
+        k_begin = first + (split * per < rows ? split * per : rows);
+        k_end = first + (split * per + per < rows ? split * per + per : rows);
+        b0 = blockIdx.z * kT;
+        b_count = g.n_out - b0 < kT ? g.n_out - b0 : kT;
+    } else {
+        const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[1])[blockIdx.x];
+        b_count = tile.y >> 16;
+        expert = tile.y & 0xffff;
+        if (b_count == 0) return;
+        if (t < kT) s_rows[t] = t < b_count ? order[tile.x + t] : -1;
+        __syncthreads();
+        k_end = FORM == kForward ? g.n_in : g.n_out;
+    }
+    const bool none = FORM != kDw && expert == g.E;   // rows of no expert: zeros
+    const int64_t w_off = int64_t(none ? 0 : expert) * g.n_out * g.n_in;
+    const elem* w = static_cast<const elem*>(g.w) + w_off;
+    const elem* x = static_cast<const elem*>(g.x);
+    const elem* dy = static_cast<const elem*>(g.g);
+    const elem* ys = static_cast<const elem*>(g.y);
+    const SplitSel sel = SplitSel::make();
+
+    // This thread's eight elements of a step: along k for an operand whose k is contiguous, along the tile's rows otherwise.
+    const int kr = t >> 2, kc = (t & 3) * 8;          // [64 rows][4 octets of k]
+    const int ck = t >> 3, cr = (t & 7) * 8;          // [32 k][8 octets of rows]
+    constexpr bool a_cols = FORM != kForward, b_cols = FORM == kDw;
+    const int my_row = FORM == kDw ? 0 : s_rows[kr];
+
+    auto load_a = [&](Oct<T>& v, int k0) {
+        v.zero();
+        if (!a_cols) {
+            if (a0 + kr < n_a && k0 + kc < k_end) v.load(w + int64_t(a0 + kr) * g.n_in + k0 + kc, k_end - k0 - kc);
+        } else if (k0 + ck < k_end && a0 + cr < n_a) {
+            if (FORM == kDx) v.load(w + int64_t(k0 + ck) * g.n_in + a0 + cr, n_a - a0 - cr);
+            else v.load(x + int64_t(order[k0 + ck]) * g.n_in + a0 + cr, n_a - a0 - cr);
+        }
+    };
+    auto load_b = [&](Oct<T>& v, int k0) {
+        v.zero();
+        int64_t at = 0;
+        int valid = 0;
+        if (FORM == kForward) {
+            if (my_row >= 0 && k0 + kc < k_end) v.load(x + int64_t(my_row) * g.n_in + k0 + kc, k_end - k0 - kc);
+            return;
+        }
+        if (FORM == kDx) {
+            if (my_row >= 0 && k0 + kc < k_end) at = int64_t(my_row) * g.n_out + k0 + kc, valid = k_end - k0 - kc;
+        } else if (k0 + ck < k_end && cr < b_count) {
+            at = int64_t(order[k0 + ck]) * g.n_out + b0 + cr, valid = b_count - cr;
+        }
+        if (valid > 0) {
+            v.load(dy + at, valid);
+            if (g.relu) {
+                Oct<T> s;
+                s.load(ys + at, valid);
+                v.keep_positive(s);
+            }
+        }
+    };
+    auto stage = [&](unsigned short (&s)[P][kT][kPitch], const Oct<T>& v, bool cols) {
+        u32x4 p[P];
+        v.terms(sel, p);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if (!cols) {
+                *reinterpret_cast<u32x4*>(&s[i][kr][kc]) = p[i];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[i][cr + 2 * j][ck] = (unsigned short)p[i][j];
+                    s[i][cr + 2 * j + 1][ck] = (unsigned short)(p[i][j] >> 16);
+                }
+            }
+        }
+    };
+
+    f32x4 acc[2][2] = {};
+    f32x4 sum[2] = {};                                // dW: db of this wavefront's 32 outputs
+    const bool with_db = FORM == kDw && g.db && blockIdx.y == 0 && wa == 0;
+    const unsigned one = __is_same(T, Fp16) ? 0x3c003c00u : 0x3f803f80u;
+    const u32x4 ones = {one, one, one, one};
+    if (!none && k_begin < k_end) {
+        Oct<T> ra, rb;
+        load_a(ra, k_begin), load_b(rb, k_begin);
+        for (int k0 = k_begin; k0 < k_end; k0 += kK) {
+            stage(s_a, ra, a_cols), stage(s_b, rb, b_cols);
+            __syncthreads();
+            if (k0 + kK < k_end) load_a(ra, k0 + kK), load_b(rb, k0 + kK);
+            u32x4 fa[2][P], fb[2][P];
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    fa[m][i] = *reinterpret_cast<const u32x4*>(&s_a[i][wa + 16 * m + c][8 * q]);
+                    fb[m][i] = *reinterpret_cast<const u32x4*>(&s_b[i][wb + 16 * m + c][8 * q]);
+                }
+#pragma unroll
+            for (int ma = 0; ma < 2; ++ma)
+#pragma unroll
+                for (int mb = 0; mb < 2; ++mb) acc[ma][mb] = mfma_terms<T>(fa[ma], fb[mb], acc[ma][mb]);
+            if (with_db)
+#pragma unroll
+                for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+                    for (int i = P - 1; i >= 0; --i) sum[mb] = mfma16<T>(ones, fb[mb][i], sum[mb]);
+            __syncthreads();
+        }
+    }
+
+    // lane (c, q) holds outputs a0 + wa + 16 ma + 4 q .. + 3 of b row wb + 16 mb + c
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb) {
+        const int br = wb + 16 * mb + c;
+        if (br >= b_count) continue;
+#pragma unroll
+        for (int ma = 0; ma < 2; ++ma) {
+            const int a = a0 + wa + 16 * ma + 4 * q, valid = n_a - a;
+            if (valid <= 0) continue;
+            f32x4 v = acc[ma][mb];
+            if (FORM == kForward) {
+                if (g.bias && !none) {
+                    const elem* b = static_cast<const elem*>(g.bias) + int64_t(expert) * g.n_out + a;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (j < valid) v[j] += to_float(b[j], T{});
+                }
+                if (g.relu)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];   // NaN stays
+            }
+            if (FORM == kDw) {
+                const int64_t at = (int64_t(expert) * g.n_out + b0 + br) * g.n_in + a;
+                if (g.splits > 1) store4<Fp32>(g.partial + int64_t(blockIdx.x % g.splits) * g.E * g.n_out * g.n_in + at, v, valid);
+                else store4<T>(static_cast<elem*>(g.out) + at, v, valid);
+            } else {
+                store4<T>(static_cast<elem*>(g.out) + int64_t(s_rows[br]) * n_a + a, v, valid);
+            }
+        }
+        if (with_db && q == 0) {
+            const int64_t at = int64_t(expert) * g.n_out + b0 + br;
+            if (g.splits > 1)
+                g.partial[int64_t(g.splits) * g.E * g.n_out * g.n_in + int64_t(blockIdx.x % g.splits) * g.E * g.n_out + at] = sum[mb][0];
+            else
+                static_cast<elem*>(g.db)[at] = from_float(sum[mb][0], T{});
+        }
+    }
+}
+
+// out[i] = sum over the splits, in their order
+template <class T>
+__global__ __launch_bounds__(256) void expert_reduce_kernel(const float* __restrict__ partial, int64_t count, int splits, void* out) {
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count; i += int64_t(gridDim.x) * 256) {
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += partial[s * count + i];
+        static_cast<typename Traits<T>::elem*>(out)[i] = from_float(v, T{});
+    }
+}
+
+// How many parts the sum over an expert's rows is cut into: enough workgroups for the chip where the outputs alone give too
+// few, none shorter than 256 rows of the average expert.
+int dw_splits(int64_t n, int E, int n_in, int n_out) {
+    const int64_t tiles = int64_t(E) * ((n_in + kT - 1) / kT) * ((n_out + kT - 1) / kT);
+    const int64_t want = (1024 + tiles - 1) / tiles, most = n / E / 256;
+    const int64_t s = want < most ? want : most;
+    return s < 1 ? 1 : s > 64 ? 64 : int(s);
+}
+
+template <int FORM>
+void launch_tile(int dtype, dim3 grid, const ExpertArgs& g, hipStream_t stream) {
+    if (dtype == NRF_DTYPE_FP32) expert_tile_kernel<Fp32, FORM><<<grid, 256, 0, stream>>>(g);
+    else if (dtype == NRF_DTYPE_BF16) expert_tile_kernel<Bf16, FORM><<<grid, 256, 0, stream>>>(g);
+    else expert_tile_kernel<Fp16, FORM><<<grid, 256, 0, stream>>>(g);
+}
+
+void launch_reduce(int dtype, const float* partial, int64_t count, int splits, void* out, hipStream_t stream) {
+    const int64_t blocks = (count + 255) / 256;
+    const dim3 grid(unsigned(blocks < 4096 ? blocks : 4096));
+    if (dtype == NRF_DTYPE_FP32) expert_reduce_kernel<Fp32><<<grid, 256, 0, stream>>>(partial, count, splits, out);
+    else if (dtype == NRF_DTYPE_BF16) expert_reduce_kernel<Bf16><<<grid, 256, 0, stream>>>(partial, count, splits, out);
+    else expert_reduce_kernel<Fp16><<<grid, 256, 0, stream>>>(partial, count, splits, out);
+}
+
+bool shapes_ok(int64_t n, int E, int n_in, int n_out, int dtype, int act) {
+    return n >= 0 && n <= nrf::kMaxExpertRows && E >= 1 && E <= nrf::kMaxExperts && n_in >= 1 && n_in <= 65536 && n_out >= 1 &&
+           n_out <= 65536 && dtype >= NRF_DTYPE_FP32 && dtype <= NRF_DTYPE_FP16 && (act == NRF_ACT_NONE || act == NRF_ACT_RELU);
+}
+
+bool elem_aligned(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == NRF_DTYPE_FP32 ? 3u : 1u)) == 0; }
+
+}  // namespace
+
+NRF_EXPORT int nrf_expert_linear(const void* x, const void* weight, const void* bias, const void* plan, int64_t n_rows,
+                                 int num_experts, int n_in, int n_out, int dtype, int act, void* y, nrf_stream_t stream) {
+    if (!shapes_ok(n_rows, num_experts, n_in, n_out, dtype, act)) return NRF_ERR_SHAPE;
+    if (n_rows == 0) return NRF_OK;
+    if (!x || !weight || !plan || !y) return NRF_ERR_NULL;
+    if (!elem_aligned(x, dtype) || !elem_aligned(weight, dtype) || !elem_aligned(bias, dtype) || !elem_aligned(y, dtype) ||
+        !nrf_aligned16(plan))
+        return NRF_ERR_ALIGN;
+    ExpertArgs g{};
+    g.x = x, g.w = weight, g.bias = bias, g.plan = static_cast<const int*>(plan), g.out = y;
+    g.n = n_rows, g.E = num_experts, g.n_in = n_in, g.n_out = n_out, g.relu = act == NRF_ACT_RELU, g.splits = 1;
+    nrf_launch_begin();
+    launch_tile<kForward>(dtype, dim3(unsigned(PlanLayout::slots(n_rows, num_experts, 1)), (n_out + kT - 1) / kT), g,
+                          static_cast<hipStream_t>(stream));
+    return nrf_launch_status();
+}
+
+NRF_EXPORT int64_t nrf_expert_linear_backward_workspace_bytes(int64_t n_rows, int num_experts, int n_in, int n_out, int dtype) {
+    if (!shapes_ok(n_rows, num_experts, n_in, n_out, dtype, NRF_ACT_NONE)) return -1;
+    const int splits = dw_splits(n_rows, num_experts, n_in, n_out);
+    return splits > 1 ? int64_t(splits) * num_experts * n_out * (n_in + 1) * 4 : 0;
+}
+
+NRF_EXPORT int nrf_expert_linear_backward(const void* grad_y, const void* x, const void* weight, const void* y, const void* plan,
+                                          int64_t n_rows, int num_experts, int n_in, int n_out, int dtype, int act, void* grad_x,
+                                          void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes,
+                                          nrf_stream_t stream_) {
+    if (!shapes_ok(n_rows, num_experts, n_in, n_out, dtype, act)) return NRF_ERR_SHAPE;
+    if (!grad_x && !grad_weight && !grad_bias) return NRF_OK;
+    if (!plan || (n_rows > 0 && (!grad_y || !x || !weight || (act == NRF_ACT_RELU && !y)))) return NRF_ERR_NULL;
+    if (grad_bias && !grad_weight) return NRF_ERR_NULL;   // the bias sums ride in the weight product
+    const void* elems[] = {grad_y, x, weight, y, grad_x, grad_weight, grad_bias};
+    for (const void* p : elems)
+        if (!elem_aligned(p, dtype)) return NRF_ERR_ALIGN;
+    if (!nrf_aligned16(plan) || !nrf_aligned16(workspace)) return NRF_ERR_ALIGN;
+    const int64_t need = nrf_expert_linear_backward_workspace_bytes(n_rows, num_experts, n_in, n_out, dtype);
+    if (grad_weight && need > 0 && (!workspace || workspace_bytes < need)) return NRF_ERR_WORKSPACE;
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    ExpertArgs g{};
+    g.x = x, g.w = weight, g.y = y, g.g = grad_y, g.plan = static_cast<const int*>(plan);
+    g.n = n_rows, g.E = num_experts, g.n_in = n_in, g.n_out = n_out, g.relu = act == NRF_ACT_RELU;
+    const int tiles_in = (n_in + kT - 1) / kT, tiles_out = (n_out + kT - 1) / kT;
+    nrf_launch_begin();
+    if (grad_x && n_rows > 0) {
+        g.out = grad_x, g.splits = 1;
+        launch_tile<kDx>(dtype, dim3(unsigned(PlanLayout::slots(n_rows, num_experts, 1)), tiles_in), g, stream);
+    }
+    if (grad_weight) {
+        const int64_t count = int64_t(num_experts) * n_out * n_in;
+        g.splits = dw_splits(n_rows, num_experts, n_in, n_out);
+        g.out = grad_weight, g.db = grad_bias, g.partial = static_cast<float*>(workspace);
+        launch_tile<kDw>(dtype, dim3(unsigned(num_experts) * unsigned(g.splits), tiles_in, tiles_out), g, stream);
+        if (g.splits > 1) {
+            launch_reduce(dtype, g.partial, count, g.splits, grad_weight, stream);
+            if (grad_bias)
+                launch_reduce(dtype, g.partial + g.splits * count, int64_t(num_experts) * n_out, g.splits, grad_bias, stream);
+        }
+    }
+    return nrf_launch_status();
+}
