@@ -38,6 +38,7 @@ SYMBOLS = (
     "nrf_occ_bricks_bytes", "nrf_occ_pack_bricks", "nrf_kilo_march_count_bricks",
     "nrf_expert_plan_bytes", "nrf_expert_plan_workspace_bytes", "nrf_expert_plan", "nrf_expert_linear",
     "nrf_expert_linear_backward_workspace_bytes", "nrf_expert_linear_backward",
+    "nrf_newton_schulz_workspace_bytes", "nrf_newton_schulz", "nrf_muon_update",
 )
 
 P = C.c_void_p
@@ -243,7 +244,11 @@ def lib() -> C.CDLL:
     L.nrf_expert_linear_backward_workspace_bytes.restype = I64
     L.nrf_expert_linear_backward_workspace_bytes.argtypes = [I64, INT, INT, INT, INT]
     L.nrf_expert_linear_backward.argtypes = [P, P, P, P, P, I64, INT, INT, INT, INT, INT, P, P, P, P, I64, P]
-    for name in ("nrf_expert_plan", "nrf_expert_linear", "nrf_expert_linear_backward"):
+    L.nrf_newton_schulz_workspace_bytes.restype = I64
+    L.nrf_newton_schulz_workspace_bytes.argtypes = [I64, INT, INT]
+    L.nrf_newton_schulz.argtypes = [P, P, I64, INT, INT, INT, INT, F, F, F, F, P, I64, P]
+    L.nrf_muon_update.argtypes = [P, P, P, INT, I64, INT, INT, F, F, F, INT, F, F, INT, F, F, F, F, P, I64, P]
+    for name in ("nrf_expert_plan", "nrf_expert_linear", "nrf_expert_linear_backward", "nrf_newton_schulz", "nrf_muon_update"):
         getattr(L, name).restype = INT
     for name in ("nrf_kilo_pack_weights_transposed", "nrf_kilo_composite_backward", "nrf_kilo_backward", "nrf_l2_reg"):
         getattr(L, name).restype = INT

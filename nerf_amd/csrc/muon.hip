@@ -1,0 +1,550 @@
+// Orthogonalising a matrix by Newton-Schulz products, and the Muon update built on it.
+//
+//   X = G / max(|G|_F, eps);  `steps` times X <- (a I + b A + c A^2) X with A = X X^T   (X the wide orientation of G)
+//
+// A step maps every singular value s to a s + b s^3 + c s^5 and leaves the singular vectors: all of them are driven towards 1.
+//
+// Arithmetic.  Small singular values grow by a in every step (3.4445^5 = 485 with the usual coefficients) and rounding
+// errors with them, so 8 significand bits per operand end 1.6e-2 off (256 x 256).  Every operand here is two fp16 terms of
+// its value times 2^12, hi + lo (22 significand bits), every product hi.hi + hi.lo + lo.hi with fp32 sums: 1.8e-6 off
+// float64 at 256 x 256, where the same iteration in fp32 is 1.7e-6 off.  X, A and Q = a I + b A + c A^2 are kept as those
+// two terms between the products: the next product reads nothing finer, and with a I inside Q there is no other reader.
+// The scale keeps lo a normal fp16 number for every entry above 2^-15 and the largest entry possible (|X| <= 1.3,
+// |A| <= 1.6, |Q| <= 8 for the coefficients the entry points admit) below fp16's 65504.  |G|_F is summed in float64.
+//
+// Two paths, by the shorter side M and the longer side N:
+//   M <= 32, N <= 128   one wavefront per matrix, everything in registers (schulz_small_kernel);
+//   otherwise           the matrices' terms in the workspace, three launches per step (schulz_product_kernel).
+#include "dma_gemm.h"
+#include "split2h.h"
+
+namespace {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kScale = 4096.f, kUnscale = 1.f / 4096.f;
+constexpr int kMaxTensors = 32, kMaxSteps = 16;
+
+struct Out32 {};
+struct OutBf16 {};
+struct OutFp16 {};
+struct OutMuon {};   // g = the gradient (fp32), the parameters and the momentum updated in place
+template <class T> struct Elem { typedef float type; };
+template <> struct Elem<OutBf16> { typedef __bf16 type; };
+template <> struct Elem<OutFp16> { typedef _Float16 type; };
+
+struct SchulzArgs {
+    const void* g[kMaxTensors];   // each (per, rows, cols)
+    void* out[kMaxTensors];       // the orthogonalised matrices, or the parameters
+    float* mom[kMaxTensors];
+    int64_t batch;
+    int per, rows, cols, steps, nesterov;
+    float a, b, c, eps;
+    float grad_scale, clip, mu, decay, rate;   // Muon: p <- decay p - rate O
+};
+
+__device__ __forceinline__ float clamp_grad(float g, const SchulzArgs& s) {
+    g *= s.grad_scale;
+    return g > s.clip ? s.clip : g < -s.clip ? -s.clip : g;   // NaN stays
+}
+// the matrix to orthogonalise, at element i of tensor t; Muon: from the gradient and the momentum before (NEW: after) its update
+template <class T, bool NEW>
+__device__ __forceinline__ float element(const SchulzArgs& s, int t, int64_t i, float* momentum) {
+    if constexpr (__is_same(T, OutMuon)) {
+        const float g = clamp_grad(static_cast<const float*>(s.g[t])[i], s);
+        const float old = s.mom[t][i];
+        const float m = NEW ? old : __fmaf_rn(s.mu, old, g);
+        if (momentum) *momentum = m;
+        return s.nesterov ? __fmaf_rn(s.mu, m, g) : m;
+    } else {
+        return float(static_cast<const typename Elem<T>::type*>(s.g[t])[i]);
+    }
+}
+template <class T>
+__device__ __forceinline__ void emit(const SchulzArgs& s, int t, int64_t i, float v) {
+    if constexpr (__is_same(T, OutMuon)) {
+        float* p = static_cast<float*>(s.out[t]) + i;
+        *p = __fmaf_rn(-s.rate, v, s.decay * *p);
+    } else {
+        static_cast<typename Elem<T>::type*>(s.out[t])[i] = (typename Elem<T>::type)v;
+    }
+}
+// 4096 / max(norm, eps); a norm that is not a number stays one
+__device__ __forceinline__ float start_scale(double sum, float eps) {
+    double norm = sqrt(sum);
+    if (norm < double(eps)) norm = double(eps);
+    return float(4096.0 / norm);
+}
+
+// a, b -> the packed pairs of their terms hi and lo (a, b already scaled; results of vector arithmetic, not of an MFMA).  The
+// residual is taken from the packed word itself: written as a - float((_Float16)a), the compiler converts twice, once with
+// the scaling folded in, and where the two round a tie apart lo belongs to another hi (2^-11 off, one entry in some thousands).
+__device__ __forceinline__ void split_pair_h2(float a, float b, unsigned& hi, unsigned& lo) {
+    hi = pk_f16(a, b);
+    lo = pk_f16(f16_residual_lo(a, hi), f16_residual_hi(b, hi));
+}
+__device__ __forceinline__ float pair_lo(unsigned w) { return float(__builtin_bit_cast(f16x2, w)[0]); }
+__device__ __forceinline__ float pair_hi(unsigned w) { return float(__builtin_bit_cast(f16x2, w)[1]); }
+
+// ---- one wavefront per matrix ------------------------------------------------------------------------------------------
+// A 32 x 32 block V is held as an MFMA accumulator holds it: register t of lane (c, h) is V[acc_row(t, h)][c].  Its sixteen
+// registers as two fragments of eight are, as either operand of v_mfma_f32_32x32x16_f16, the matrix P[r][k] = V[k][r] with k
+// running through acc_row (both operands run through it alike).  So a symmetric V multiplies as it lies, and with X kept in
+// both orientations (X_j: columns 32 j.. of X, Y_j = X_j^T) every product of a step is made from registers:
+//   A = sum_j X_j X_j^T: operands Y_j, Y_j     A^2: A, A     X_j' = Q X_j: Q, X_j   (a tall matrix: Y_j' = Y_j Q: X_j, Q)
+// The other orientation of the new X is turned through LDS (36-word rows: 16 single-word writes, 4 vector reads, no bank
+// conflicts), not multiplied again: orientations that round apart would no longer damp each other's errors.
+struct Frag {
+    u32x4 hi[2], lo[2];
+};
+__device__ __forceinline__ Frag split_block(const f32x16& v) {
+    Frag f;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            unsigned hi, lo;
+            split_pair_h2(v[8 * s + 2 * i], v[8 * s + 2 * i + 1], hi, lo);
+            f.hi[s][i] = hi, f.lo[s][i] = lo;
+        }
+    return f;
+}
+__device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_g, a), __builtin_bit_cast(f16x8_g, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 product(const Frag& a, const Frag& b, f32x16 c) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) c = mfma32(a.hi[s], b.lo[s], c), c = mfma32(a.lo[s], b.hi[s], c);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) c = mfma32(a.hi[s], b.hi[s], c);
+    return c;
+}
+
+constexpr int kTurnPitch = 36;
+// the fragments of V^T from those of V: element pairs {hi, lo} as words through this wavefront's piece of LDS
+__device__ __forceinline__ Frag turn_block(const Frag& f, unsigned* s_turn, int c, int h) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = 8 * s + 2 * i;
+            s_turn[nrf::acc_row(t, h) * kTurnPitch + c] = __builtin_amdgcn_perm(f.lo[s][i], f.hi[s][i], 0x05040100u);
+            s_turn[nrf::acc_row(t + 1, h) * kTurnPitch + c] = __builtin_amdgcn_perm(f.lo[s][i], f.hi[s][i], 0x07060302u);
+        }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");   // one wavefront, LDS in order
+    __builtin_amdgcn_wave_barrier();
+    Frag o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {   // registers 4 j .. 4 j + 3: V[c][8 j + 4 h ..]
+        const u32x4 w = *reinterpret_cast<const u32x4*>(s_turn + c * kTurnPitch + 8 * j + 4 * h);
+        o.hi[j >> 1][2 * (j & 1)] = __builtin_amdgcn_perm(w[1], w[0], 0x05040100u);
+        o.hi[j >> 1][2 * (j & 1) + 1] = __builtin_amdgcn_perm(w[3], w[2], 0x05040100u);
+        o.lo[j >> 1][2 * (j & 1)] = __builtin_amdgcn_perm(w[1], w[0], 0x07060302u);
+        o.lo[j >> 1][2 * (j & 1) + 1] = __builtin_amdgcn_perm(w[3], w[2], 0x07060302u);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    return o;
+}
+
+template <class T, int NB, bool TALL>
+__global__ __launch_bounds__(256) void schulz_small_kernel(SchulzArgs s) {
+    __shared__ __align__(16) unsigned s_all[4][32 * kTurnPitch];
+    const int64_t m = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (m >= s.batch) return;                      // no barrier below: every wavefront works alone
+    unsigned* s_turn = s_all[threadIdx.x >> 6];
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int t0 = int(m / s.per);
+    const int64_t base = (m % s.per) * int64_t(s.rows) * s.cols;
+
+    // G in blocks along its longer side, lanes along its rows: X_j of a wide matrix, Y_j of a tall one (X = G^T)
+    f32x16 v[NB];
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            const int r = (TALL ? 32 * j : 0) + nrf::acc_row(t, h), q = TALL ? c : 32 * j + c;
+            v[j][t] = 0.f;
+            if (r < s.rows && q < s.cols) {
+                const int64_t i = base + int64_t(r) * s.cols + q;
+                float mom = 0.f;
+                v[j][t] = element<T, false>(s, t0, i, &mom);
+                if constexpr (__is_same(T, OutMuon)) s.mom[t0][i] = mom;
+            }
+            sum = __builtin_fma(double(v[j][t]), double(v[j][t]), sum);
+        }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+    const float scale = start_scale(sum, s.eps);
+    Frag here[NB], turned[NB];                     // of X_j and Y_j for a wide matrix, of Y_j and X_j for a tall one
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        v[j] = v[j] * scale;
+        here[j] = split_block(v[j]);
+        turned[j] = turn_block(here[j], s_turn, c, h);
+        v[j] = v[j] * kScale;                      // no step at all: the scaled matrix
+    }
+    for (int k = 0; k < s.steps; ++k) {
+        f32x16 acc = {};
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc = TALL ? product(here[j], here[j], acc) : product(turned[j], turned[j], acc);
+        const f32x16 gram = acc * kUnscale;
+        const Frag fg = split_block(gram);
+        acc = product(fg, fg, (f32x16){});
+        f32x16 poly = s.b * gram + (s.c * kUnscale) * acc;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) poly[t] += nrf::acc_row(t, h) == c ? s.a * kScale : 0.f;
+        const Frag fq = split_block(poly);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) v[j] = TALL ? product(turned[j], fq, (f32x16){}) : product(fq, here[j], (f32x16){});
+        if (k + 1 < s.steps)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                here[j] = split_block(v[j] * kUnscale);
+                turned[j] = turn_block(here[j], s_turn, c, h);
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            const int r = (TALL ? 32 * j : 0) + nrf::acc_row(t, h), q = TALL ? c : 32 * j + c;
+            if (r < s.rows && q < s.cols) emit<T>(s, t0, base + int64_t(r) * s.cols + q, v[j][t] * (kUnscale * kUnscale));
+        }
+}
+
+// ---- larger matrices ----------------------------------------------------------------------------------------------------
+// The workspace of a matrix, in fp16 elements, M and N padded with zeros (which every product keeps) to the tile: X [2 terms]
+// [M][N] and X^T [2][N][M], both twice (a step reads one and writes the other), A and Q [2][M][M].
+struct LargeShape {
+    int M, N, Mp, Np, tile, chunks;
+    __host__ __device__ int64_t x_size() const { return int64_t(2) * Mp * Np; }
+    __host__ __device__ int64_t s_size() const { return int64_t(2) * Mp * Mp; }
+    __host__ __device__ int64_t per_matrix() const { return 4 * x_size() + 2 * s_size(); }
+    __host__ __device__ int64_t x_at(int which) const { return which * 2 * x_size(); }
+    __host__ __device__ int64_t xt_at(int which) const { return which * 2 * x_size() + x_size(); }
+    __host__ __device__ int64_t gram_at() const { return 4 * x_size(); }
+    __host__ __device__ int64_t poly_at() const { return 4 * x_size() + s_size(); }
+};
+constexpr int kNormChunk = 16384;   // elements a workgroup sums
+
+// |G|_F^2 in parts; Muon: the momentum's update
+template <class T>
+__global__ __launch_bounds__(256) void schulz_norm_kernel(SchulzArgs s, LargeShape L, double* __restrict__ parts) {
+    const int64_t m = blockIdx.y, count = int64_t(s.rows) * s.cols;
+    const int t = int(m / s.per);
+    const int64_t base = (m % s.per) * count;
+    const int64_t begin = int64_t(blockIdx.x) * kNormChunk, end = begin + kNormChunk < count ? begin + kNormChunk : count;
+    double sum = 0.0;
+    for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
+        float mom = 0.f;
+        const float v = element<T, false>(s, t, base + i, &mom);
+        if constexpr (__is_same(T, OutMuon)) s.mom[t][base + i] = mom;
+        sum = __builtin_fma(double(v), double(v), sum);
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+    __shared__ double s_sum[4];
+    if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) parts[m * L.chunks + blockIdx.x] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+}
+
+// X and X^T from G: one 64 x 64 tile of G's padded (rows, cols) per workgroup
+template <class T>
+__global__ __launch_bounds__(256) void schulz_start_kernel(SchulzArgs s, LargeShape L, const double* __restrict__ parts,
+                                                           _Float16* __restrict__ work) {
+    __shared__ float s_tile[64][65];
+    __shared__ float s_scale;
+    const int64_t m = blockIdx.z, count = int64_t(s.rows) * s.cols;
+    if (threadIdx.x < 64) {
+        double sum = 0.0;
+        for (int i = threadIdx.x; i < L.chunks; i += 64) sum += parts[m * L.chunks + i];
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+        if (threadIdx.x == 0) s_scale = start_scale(sum, s.eps);
+    }
+    __syncthreads();
+    const float scale = s_scale;
+    const bool tall = s.rows > s.cols;
+    const int t = int(m / s.per), r0 = blockIdx.y * 64, q0 = blockIdx.x * 64;
+    const int64_t base = (m % s.per) * count;
+    const int rp = tall ? L.Np : L.Mp, cp = tall ? L.Mp : L.Np;      // padded rows and columns of G
+    _Float16* w = work + m * L.per_matrix();
+    _Float16* straight = w + (tall ? L.xt_at(0) : L.x_at(0));        // [rp][cp]
+    _Float16* turned = w + (tall ? L.x_at(0) : L.xt_at(0));          // [cp][rp]
+    unsigned *straight32 = reinterpret_cast<unsigned*>(straight), *turned32 = reinterpret_cast<unsigned*>(turned);
+    const int q = (threadIdx.x & 31) * 2;                            // a pair of columns
+    for (int r = threadIdx.x >> 5; r < 64; r += 8) {
+        float v[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            v[i] = 0.f;
+            if (r0 + r < s.rows && q0 + q + i < s.cols)
+                v[i] = element<T, true>(s, t, base + int64_t(r0 + r) * s.cols + q0 + q + i, nullptr) * scale;
+            s_tile[r][q + i] = v[i];
+        }
+        unsigned hi, lo;
+        split_pair_h2(v[0], v[1], hi, lo);
+        const int64_t at = int64_t(r0 + r) * cp + q0 + q;
+        straight32[at >> 1] = hi, straight32[(int64_t(rp) * cp + at) >> 1] = lo;
+    }
+    __syncthreads();
+    for (int r = threadIdx.x >> 5; r < 64; r += 8) {
+        unsigned hi, lo;
+        split_pair_h2(s_tile[q][r], s_tile[q + 1][r], hi, lo);
+        const int64_t at = int64_t(q0 + r) * rp + r0 + q;
+        turned32[at >> 1] = hi, turned32[(int64_t(rp) * cp + at) >> 1] = lo;
+    }
+}
+
+enum Product { kGram, kPoly, kApply, kLast };
+
+// four values of consecutive a as their two terms: at dst (plane stride `plane`), or down a column of rows of `pitch`
+struct Terms {
+    u32x2 hi, lo;
+};
+__device__ __forceinline__ Terms terms_of(const f32x4& v) {
+    unsigned h0, l0, h1, l1;
+    split_pair_h2(v[0], v[1], h0, l0);
+    split_pair_h2(v[2], v[3], h1, l1);
+    return {{h0, h1}, {l0, l1}};
+}
+__device__ __forceinline__ void store_terms(_Float16* dst, int64_t plane, const Terms& v) {
+    *reinterpret_cast<u32x2*>(dst) = v.hi;
+    *reinterpret_cast<u32x2*>(dst + plane) = v.lo;
+}
+__device__ __forceinline__ void store_terms_down(_Float16* dst, int64_t plane, int64_t pitch, const Terms& v) {
+    unsigned short* d = reinterpret_cast<unsigned short*>(dst);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        d[r * pitch] = (unsigned short)(v.hi[r >> 1] >> (16 * (r & 1)));
+        d[plane + r * pitch] = (unsigned short)(v.lo[r >> 1] >> (16 * (r & 1)));
+    }
+}
+
+// One product of a step: A = X X^T and Q = a I + b A + c A A (symmetric: the tiles on and over the diagonal, each written to
+// both places), X' = Q X (to X' and X'^T; the last step: to the output).
+template <class T, int WHAT, int TT>
+__global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, LargeShape L, _Float16* __restrict__ work, int which) {
+    typedef DmaGemm<false, TT, TT, 2, 2, 2, 32, 3> Gemm;
+    extern __shared__ __align__(16) char smem[];
+    const int64_t m = blockIdx.y;
+    _Float16* w = work + m * L.per_matrix();
+    const int tiles_m = L.Mp / TT;
+    int ta, tb;
+    if (WHAT == kGram || WHAT == kPoly) {   // tile pairs (ta <= tb), tb-th row has tb + 1
+        int left = blockIdx.x;
+        for (tb = 0; left > tb; ++tb) left -= tb + 1;
+        ta = left;
+    } else {
+        ta = blockIdx.x % tiles_m, tb = blockIdx.x / tiles_m;
+    }
+    const int a0 = ta * TT, b0 = tb * TT;
+    const int K = WHAT == kGram ? L.Np : L.Mp;
+    const _Float16* pa = w + (WHAT == kGram ? L.x_at(which) : WHAT == kPoly ? L.gram_at() : L.poly_at());
+    const _Float16* pb = w + (WHAT == kGram ? L.x_at(which) : WHAT == kPoly ? L.gram_at() : L.xt_at(which));
+    const int64_t plane_a = int64_t(L.Mp) * K, plane_b = int64_t(WHAT == kGram || WHAT == kPoly ? L.Mp : L.Np) * K;
+    Gemm gemm;
+    gemm.start(smem, [&](bool is_b, int plane, int row) {
+        return is_b ? pb + plane * plane_b + int64_t(b0 + row) * K : pa + plane * plane_a + int64_t(a0 + row) * K;
+    });
+    f32x4 acc[Gemm::kMA][Gemm::kMB] = {};
+    gemm.run(smem, K / 32, acc);
+
+    const int c = gemm.lane & 15, q = gemm.lane >> 4, t = int(m / s.per);
+    const int64_t base = (m % s.per) * int64_t(s.rows) * s.cols;
+    const bool tall = s.rows > s.cols;
+    _Float16* sym = w + (WHAT == kGram ? L.gram_at() : L.poly_at());
+    _Float16 *xn = w + L.x_at(which ^ 1), *xtn = w + L.xt_at(which ^ 1);
+#pragma unroll
+    for (int ma = 0; ma < Gemm::kMA; ++ma)
+#pragma unroll
+        for (int mb = 0; mb < Gemm::kMB; ++mb) {
+            const int a = a0 + gemm.wave_a() + 16 * ma + 4 * q, b = b0 + gemm.wave_b() + 16 * mb + c;
+            f32x4 v = acc[ma][mb] * kUnscale;
+            if (WHAT == kGram || WHAT == kPoly) {
+                const int64_t plane = int64_t(L.Mp) * L.Mp, at = int64_t(b) * L.Mp + a;
+                if (WHAT == kPoly) {
+                    const u32x2 hi = *reinterpret_cast<const u32x2*>(w + L.gram_at() + at);
+                    const u32x2 lo = *reinterpret_cast<const u32x2*>(w + L.gram_at() + plane + at);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float g = r & 1 ? pair_hi(hi[r >> 1]) + pair_hi(lo[r >> 1]) : pair_lo(hi[r >> 1]) + pair_lo(lo[r >> 1]);
+                        v[r] = s.b * g + s.c * v[r] + (a + r == b ? s.a * kScale : 0.f);
+                    }
+                }
+                const Terms o = terms_of(v);
+                store_terms(sym + at, plane, o);
+                if (ta != tb) store_terms_down(sym + int64_t(a) * L.Mp + b, plane, L.Mp, o);
+            } else if (WHAT == kApply) {   // a: row of X', b: column
+                const int64_t plane = int64_t(L.Mp) * L.Np;
+                const Terms o = terms_of(v);
+                store_terms(xtn + int64_t(b) * L.Mp + a, plane, o);
+                store_terms_down(xn + int64_t(a) * L.Np + b, plane, L.Np, o);
+            } else if (b < L.N) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (a + r < L.M)
+                        emit<T>(s, t, base + (tall ? int64_t(b) * s.cols + a + r : int64_t(a + r) * s.cols + b), v[r] * kUnscale);
+            }
+        }
+}
+
+// no step at all: the scaled matrix itself
+template <class T>
+__global__ __launch_bounds__(256) void schulz_copy_kernel(SchulzArgs s, LargeShape L, const double* __restrict__ parts) {
+    const int64_t m = blockIdx.y, count = int64_t(s.rows) * s.cols;
+    double sum = 0.0;
+    for (int i = 0; i < L.chunks; ++i) sum += parts[m * L.chunks + i];
+    const float scale = start_scale(sum, s.eps) * kUnscale;
+    const int t = int(m / s.per);
+    const int64_t base = (m % s.per) * count;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count; i += int64_t(gridDim.x) * 256)
+        emit<T>(s, t, base + i, element<T, true>(s, t, base + i, nullptr) * scale);
+}
+
+bool small_path(int rows, int cols) {
+    const int lo = rows < cols ? rows : cols, hi = rows < cols ? cols : rows;
+    return lo <= 32 && hi <= 128;
+}
+
+LargeShape large_shape(int rows, int cols) {
+    LargeShape L;
+    L.M = rows < cols ? rows : cols, L.N = rows < cols ? cols : rows;
+    L.tile = L.M > 512 ? 128 : 64;
+    L.Mp = (L.M + L.tile - 1) / L.tile * L.tile, L.Np = (L.N + L.tile - 1) / L.tile * L.tile;
+    L.chunks = int((int64_t(rows) * cols + kNormChunk - 1) / kNormChunk);
+    return L;
+}
+
+template <class T, bool TALL>
+void launch_small(const SchulzArgs& s, hipStream_t stream) {
+    const int longer = s.rows < s.cols ? s.cols : s.rows;
+    const dim3 grid(unsigned((s.batch + 3) / 4));
+    if (longer <= 32) schulz_small_kernel<T, 1, TALL><<<grid, 256, 0, stream>>>(s);
+    else if (longer <= 64) schulz_small_kernel<T, 2, TALL><<<grid, 256, 0, stream>>>(s);
+    else schulz_small_kernel<T, 4, TALL><<<grid, 256, 0, stream>>>(s);
+}
+
+template <class T, int WHAT, int TT>
+int launch_product(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream) {
+    typedef DmaGemm<false, TT, TT, 2, 2, 2, 32, 3> Gemm;
+    const int m = L.Mp / TT, n = L.Np / TT;
+    const int64_t tiles = WHAT == kGram || WHAT == kPoly ? int64_t(m) * (m + 1) / 2 : int64_t(m) * n;
+    auto kernel = &schulz_product_kernel<T, WHAT, TT>;
+    if (Gemm::kLds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                  Gemm::kLds) != hipSuccess)
+        return NRF_ERR_LAUNCH;
+    kernel<<<dim3(unsigned(tiles), unsigned(s.batch)), 256, Gemm::kLds, stream>>>(s, L, work, which);
+    return NRF_OK;
+}
+
+template <class T, int TT>
+int run_large(const SchulzArgs& s, const LargeShape& L, double* parts, _Float16* work, hipStream_t stream) {
+    const dim3 cover(unsigned((s.rows > s.cols ? L.Mp : L.Np) / 64), unsigned((s.rows > s.cols ? L.Np : L.Mp) / 64), unsigned(s.batch));
+    schulz_norm_kernel<T><<<dim3(unsigned(L.chunks), unsigned(s.batch)), 256, 0, stream>>>(s, L, parts);
+    if (s.steps == 0) {
+        schulz_copy_kernel<T><<<dim3(unsigned(L.chunks), unsigned(s.batch)), 256, 0, stream>>>(s, L, parts);
+        return NRF_OK;
+    }
+    schulz_start_kernel<T><<<cover, 256, 0, stream>>>(s, L, parts, work);
+    for (int k = 0; k < s.steps; ++k) {
+        int st = launch_product<Out32, kGram, TT>(s, L, work, k & 1, stream);   // the output's type matters to kLast alone
+        if (st == NRF_OK) st = launch_product<Out32, kPoly, TT>(s, L, work, k & 1, stream);
+        if (st == NRF_OK)
+            st = k + 1 < s.steps ? launch_product<Out32, kApply, TT>(s, L, work, k & 1, stream)
+                                 : launch_product<T, kLast, TT>(s, L, work, k & 1, stream);
+        if (st != NRF_OK) return st;
+    }
+    return NRF_OK;
+}
+
+template <class T>
+int run(const SchulzArgs& s, void* workspace, hipStream_t stream) {
+    nrf_launch_begin();
+    if (small_path(s.rows, s.cols)) {
+        if (s.rows > s.cols) launch_small<T, true>(s, stream);
+        else launch_small<T, false>(s, stream);
+        return nrf_launch_status();
+    }
+    const LargeShape L = large_shape(s.rows, s.cols);
+    double* parts = static_cast<double*>(workspace);
+    _Float16* work = reinterpret_cast<_Float16*>(parts + ((s.batch * L.chunks + 31) & ~int64_t(31)));
+    const int st = L.tile == 128 ? run_large<T, 128>(s, L, parts, work, stream) : run_large<T, 64>(s, L, parts, work, stream);
+    return st != NRF_OK ? st : nrf_launch_status();
+}
+
+bool schulz_shape_ok(int64_t batch, int rows, int cols) {
+    if (batch < 0 || rows < 1 || cols < 1 || rows > 65536 || cols > 65536) return false;
+    if (small_path(rows, cols)) return batch <= int64_t(1) << 24;
+    return batch <= 65535;
+}
+// the iteration on the singular values, which start in [0, 1]: entries of X, A and Q must stay inside fp16 at scale 2^12
+bool coefficients_ok(int steps, float a, float b, float c) {
+    if (steps < 0 || steps > kMaxSteps) return false;
+    for (int i = 0; i <= 256; ++i) {
+        double v = i / 256.0;
+        for (int k = 0; k < steps; ++k) {
+            const double q = a + (b + c * v * v) * v * v;
+            v *= q;
+            if (!(v >= -1.5 && v <= 1.5) || !(q >= -12.0 && q <= 12.0)) return false;
+        }
+    }
+    return true;
+}
+
+}  // namespace
+
+NRF_EXPORT int64_t nrf_newton_schulz_workspace_bytes(int64_t batch, int rows, int cols) {
+    if (!schulz_shape_ok(batch, rows, cols)) return -1;
+    if (small_path(rows, cols)) return 0;
+    const LargeShape L = large_shape(rows, cols);
+    return ((batch * L.chunks + 31) & ~int64_t(31)) * 8 + batch * L.per_matrix() * 2;
+}
+
+NRF_EXPORT int nrf_newton_schulz(const void* g, void* out, int64_t batch, int rows, int cols, int dtype, int steps, float a,
+                                 float b, float c, float eps, void* workspace, int64_t workspace_bytes, nrf_stream_t stream_) {
+    const int64_t need = nrf_newton_schulz_workspace_bytes(batch, rows, cols);
+    if (need < 0 || dtype < NRF_DTYPE_FP32 || dtype > NRF_DTYPE_FP16 || !(eps >= 1e-30f) || !coefficients_ok(steps, a, b, c))
+        return NRF_ERR_SHAPE;
+    if (batch == 0) return NRF_OK;
+    if (!g || !out || (need > 0 && !workspace)) return NRF_ERR_NULL;
+    if (workspace_bytes < need) return NRF_ERR_WORKSPACE;
+    const uintptr_t low = dtype == NRF_DTYPE_FP32 ? 3 : 1;
+    if ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(out)) & low || (need > 0 && !nrf_aligned16(workspace)))
+        return NRF_ERR_ALIGN;
+    SchulzArgs s{};
+    s.g[0] = g, s.out[0] = out, s.batch = batch, s.per = int(batch), s.rows = rows, s.cols = cols, s.steps = steps;
+    s.a = a, s.b = b, s.c = c, s.eps = eps;
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    if (dtype == NRF_DTYPE_FP32) return run<Out32>(s, workspace, stream);
+    if (dtype == NRF_DTYPE_BF16) return run<OutBf16>(s, workspace, stream);
+    return run<OutFp16>(s, workspace, stream);
+}
+
+NRF_EXPORT int nrf_muon_update(float* const* params, const float* const* grads, float* const* momentum, int n_tensors, int64_t batch,
+                               int rows, int cols, float grad_scale, float clip_value, float mu, int nesterov, float lr,
+                               float weight_decay, int steps, float a, float b, float c, float eps, void* workspace,
+                               int64_t workspace_bytes, nrf_stream_t stream) {
+    if (n_tensors < 0 || n_tensors > kMaxTensors || batch < 0 || batch > (int64_t(1) << 24)) return NRF_ERR_SHAPE;
+    const int64_t need = nrf_newton_schulz_workspace_bytes(batch * n_tensors, rows, cols);
+    if (need < 0 || !(eps >= 1e-30f) || !(clip_value > 0.f) || !(mu >= 0.f && mu < 1.f) || !coefficients_ok(steps, a, b, c)) return NRF_ERR_SHAPE;
+    if (batch == 0 || n_tensors == 0) return NRF_OK;
+    if (!params || !grads || !momentum || (need > 0 && !workspace)) return NRF_ERR_NULL;
+    if (workspace_bytes < need) return NRF_ERR_WORKSPACE;
+    if (need > 0 && !nrf_aligned16(workspace)) return NRF_ERR_ALIGN;
+    SchulzArgs s{};
+    for (int i = 0; i < n_tensors; ++i) {
+        if (!params[i] || !grads[i] || !momentum[i]) return NRF_ERR_NULL;
+        if ((reinterpret_cast<uintptr_t>(params[i]) | reinterpret_cast<uintptr_t>(grads[i]) | reinterpret_cast<uintptr_t>(momentum[i])) & 3)
+            return NRF_ERR_ALIGN;
+        s.g[i] = grads[i], s.out[i] = params[i], s.mom[i] = momentum[i];
+    }
+    s.batch = batch * n_tensors, s.per = int(batch), s.rows = rows, s.cols = cols, s.steps = steps, s.nesterov = nesterov != 0;
+    s.a = a, s.b = b, s.c = c, s.eps = eps, s.grad_scale = grad_scale, s.clip = clip_value, s.mu = mu;
+    s.decay = float(1.0 - double(lr) * double(weight_decay));
+    s.rate = float(double(lr) * sqrt(rows > cols ? double(rows) / cols : 1.0));
+    return run<OutMuon>(s, workspace, static_cast<hipStream_t>(stream));
+}
