@@ -11,6 +11,7 @@
 // bf16 / fp16 operands go to the matrix cores as they are.  fp32 operands are split into three bf16 terms on their way into
 // LDS (split3.h: 24 significand bits, six products, fp32 sums): an operand that is not finite gives NaN.  Sums are fp32;
 // an output is rounded to its type once, after bias and relu.
+#include "dma_gemm.h"
 #include "experts.h"
 #include "split3.h"
 
@@ -161,10 +162,10 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
         b0 = blockIdx.z * kT;
         b_count = g.n_out - b0 < kT ? g.n_out - b0 : kT;
     } else {
+        if (int(blockIdx.x) >= g.plan[L.runs + 2 * 1 + 1]) return;
         const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[1])[blockIdx.x];
         b_count = tile.y >> 16;
         expert = tile.y & 0xffff;
-        if (b_count == 0) return;
         if (t < kT) s_rows[t] = t < b_count ? order[tile.x + t] : -1;
         __syncthreads();
         k_end = FORM == kForward ? g.n_in : g.n_out;
@@ -303,6 +304,188 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
     }
 }
 
+// ---- bf16 / fp16, wide layers ----------------------------------------------------------------------------------------------
+// Consecutive workgroups go to different XCDs: each XCD takes a contiguous eighth of the whole row runs and of the rests (an
+// expert's runs share its weights in that XCD's L2).  -> the `local`-th run of this one, -1 past its last.
+__device__ __forceinline__ int xcd_run(const int* runs, int xcd, int local) {
+    const int whole = runs[0], rests = runs[1] - whole;
+    int begin = int(int64_t(whole) * xcd / 8), end = int(int64_t(whole) * (xcd + 1) / 8);
+    if (local < end - begin) return begin + local;
+    local -= end - begin;
+    begin = int(int64_t(rests) * xcd / 8), end = int(int64_t(rests) * (xcd + 1) / 8);
+    return local < end - begin ? whole + begin + local : -1;
+}
+__host__ __device__ constexpr int64_t xcd_blocks(int64_t slots, int a_tiles) { return (slots / 8 + 2) * 8 * a_tiles; }
+
+// four consecutive outputs of a product, after bias and relu
+template <class T>
+__device__ __forceinline__ void finish_row(typename Traits<T>::elem* out, f32x4 v, int valid, const typename Traits<T>::elem* bias, int relu) {
+    if (bias)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < valid) v[j] += to_float(bias[j], T{});
+    if (relu)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];   // NaN stays
+    store4<T>(out, v, valid);
+}
+
+// Forward and dx: 256 output columns x 256 batch rows, eight wavefronts of 128 x 64 (12 KiB of LDS reads to 32 MFMAs), two
+// steps of 64 k in LDS (128 KiB).  dx reads the weights' columns (DmaGemm: kCols); g.g holds dz.
+template <class T, int FORM> struct WideRows {
+    static constexpr int kA = 256, kB = 256, kTable = 3;
+    typedef DmaGemm<__is_same(T, Bf16), FORM == kForward ? kRows : kCols, kRows, kA, kB, 2, 4, 1, 64, 2> Gemm;
+};
+template <class T, int FORM>
+__global__ __launch_bounds__(512) void expert_wide_rows_kernel(ExpertArgs g, int a_tiles) {
+    typedef WideRows<T, FORM> W;
+    typedef typename W::Gemm Gemm;
+    typedef unsigned short elem;
+    extern __shared__ __align__(16) char smem[];
+    const PlanLayout L(g.n, g.E);
+    const int local = blockIdx.x / 8, at = xcd_run(g.plan + L.runs + 2 * W::kTable, blockIdx.x % 8, local / a_tiles);
+    if (at < 0) return;
+    const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[W::kTable])[at];
+    const int b_count = tile.y >> 16, expert = tile.y & 0xffff, a0 = local % a_tiles * W::kA;
+    const int* order = g.plan + L.order + tile.x;
+    const bool none = expert == g.E;
+    const int n_a = FORM == kForward ? g.n_out : g.n_in, n_k = FORM == kForward ? g.n_in : g.n_out;
+    const elem* w = static_cast<const elem*>(g.w) + int64_t(none ? 0 : expert) * g.n_out * g.n_in;
+    Gemm gemm;
+    f32x4 acc[Gemm::kMA][Gemm::kMB] = {};
+    if (!none) {
+        const unsigned pitch = unsigned(n_k) * 2u;
+        if constexpr (FORM == kForward) {
+            gemm.a.start_rows(gemm.wave, gemm.lane, w, [&](int, int row) { return unsigned(a0 + row < n_a ? a0 + row : n_a - 1) * pitch; });
+        } else {
+            gemm.pitch_a = unsigned(n_a) * 2u, gemm.step_a = int64_t(n_a) * 128;
+            gemm.a.start_cols(gemm.wave, gemm.lane, w + a0, gemm.pitch_a, (n_a - a0) / 8);
+        }
+        gemm.b.start_rows(gemm.wave, gemm.lane, FORM == kForward ? g.x : g.g, [&](int, int row) { return unsigned(order[row < b_count ? row : 0]) * pitch; });
+        gemm.idle = gemm.wave_b() >= b_count || a0 + gemm.wave_a() >= n_a;
+        gemm.run(smem, n_k, acc);
+    }
+    const int c = gemm.lane & 15, q = gemm.lane >> 4;
+#pragma unroll
+    for (int mb = 0; mb < Gemm::kMB; ++mb) {
+        const int br = gemm.wave_b() + 16 * mb + c;
+        if (br >= b_count) continue;
+        elem* out = static_cast<elem*>(g.out) + int64_t(order[br]) * n_a;
+#pragma unroll
+        for (int ma = 0; ma < Gemm::kMA; ++ma) {
+            const int a = a0 + gemm.wave_a() + 16 * ma + 4 * q, valid = n_a - a;
+            if (valid <= 0) continue;
+            const elem* bias = FORM == kForward && g.bias && !none ? static_cast<const elem*>(g.bias) + int64_t(expert) * g.n_out + a : nullptr;
+            finish_row<T>(out + a, acc[ma][mb], valid, bias, FORM == kForward ? g.relu : 0);
+        }
+    }
+}
+
+// dW: 256 input columns x DWB output columns, k the expert's rows through the list of them in LDS, kListRows at a time.
+#ifndef DWB
+#define DWB 128
+#endif
+constexpr int kListRows = 4096;
+template <class T> struct WideDw {
+    static constexpr int kA = 256, kB = DWB;
+    typedef DmaGemm<__is_same(T, Bf16), kGather, kGather, kA, kB, DWB == 256 ? 2 : 4, DWB == 256 ? 4 : 2, 1, 64, 2, true> Gemm;
+    static constexpr int kLds = Gemm::kLds + kListRows * 4;
+};
+template <class T>
+__global__ __launch_bounds__(512) void expert_wide_dw_kernel(ExpertArgs g, int a_tiles, int b_tiles) {
+    typedef WideDw<T> W;
+    typedef typename W::Gemm Gemm;
+    typedef unsigned short elem;
+    extern __shared__ __align__(16) char smem[];
+    int* s_list = reinterpret_cast<int*>(smem + Gemm::kLds);
+    const PlanLayout L(g.n, g.E);
+    // an expert's tiles stay on one XCD, which keeps the expert's rows in its L2
+    const int tiles = a_tiles * b_tiles * g.splits, local = blockIdx.x / 8, expert = local / tiles * 8 + blockIdx.x % 8;
+    if (expert >= g.E) return;
+    const int split = local % tiles / (a_tiles * b_tiles), tile = local % (a_tiles * b_tiles);
+    const int a0 = tile % a_tiles * W::kA, b0 = tile / a_tiles * W::kB;
+    const int rows = g.plan[expert], per = ((rows + g.splits - 1) / g.splits + 63) / 64 * 64;
+    const int begin = split * per < rows ? split * per : rows, end = begin + per < rows ? begin + per : rows;
+    const int* order = g.plan + L.order + g.plan[L.offsets + expert];
+    Gemm gemm;
+    f32x4 acc[Gemm::kMA][Gemm::kMB] = {}, sum[Gemm::kMB] = {};
+    gemm.pitch_a = unsigned(g.n_in) * 2u, gemm.pitch_b = unsigned(g.n_out) * 2u;
+    gemm.a.start_cols(gemm.wave, gemm.lane, static_cast<const elem*>(g.x) + a0, 0, (g.n_in - a0) / 8);
+    gemm.b.start_cols(gemm.wave, gemm.lane, static_cast<const elem*>(g.g) + b0, 0, (g.n_out - b0) / 8);
+    gemm.idle = b0 + gemm.wave_b() >= g.n_out || a0 + gemm.wave_a() >= g.n_in;
+    const bool with_db = g.db && a0 == 0 && gemm.wave_a() == 0;
+    for (int r0 = begin; r0 < end; r0 += kListRows) {
+        const int count = end - r0 < kListRows ? end - r0 : kListRows;
+        __syncthreads();
+        for (int i = threadIdx.x; i < count; i += 512) s_list[i] = order[r0 + i];
+        __syncthreads();
+        gemm.run(smem, count, acc, s_list, &sum, with_db);
+    }
+    const int c = gemm.lane & 15, q = gemm.lane >> 4;
+    const int64_t weights = int64_t(g.E) * g.n_out * g.n_in;
+#pragma unroll
+    for (int mb = 0; mb < Gemm::kMB; ++mb) {
+        const int br = b0 + gemm.wave_b() + 16 * mb + c;
+        if (br >= g.n_out) continue;
+        const int64_t row = int64_t(expert) * g.n_out + br;
+#pragma unroll
+        for (int ma = 0; ma < Gemm::kMA; ++ma) {
+            const int a = a0 + gemm.wave_a() + 16 * ma + 4 * q, valid = g.n_in - a;
+            if (valid <= 0) continue;
+            if (g.splits > 1) store4<Fp32>(g.partial + split * weights + row * g.n_in + a, acc[ma][mb], valid);
+            else store4<T>(static_cast<elem*>(g.out) + row * g.n_in + a, acc[ma][mb], valid);
+        }
+        if (with_db && q == 0) {
+            if (g.splits > 1) g.partial[g.splits * weights + split * int64_t(g.E) * g.n_out + row] = sum[mb][0];
+            else static_cast<elem*>(g.db)[row] = from_float(sum[mb][0], T{});
+        }
+    }
+}
+
+// dz = dy where y > 0: read twice by the products, which move their operands without looking at them
+template <class T>
+__global__ __launch_bounds__(256) void expert_mask_kernel(const u32x4* __restrict__ dy, const u32x4* __restrict__ y, int64_t octets,
+                                                          u32x4* __restrict__ dz) {
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < octets; i += int64_t(gridDim.x) * 256) {
+        Oct<T> v, s;
+        v.v = dy[i], s.v = y[i];
+        v.keep_positive(s);
+        dz[i] = v.v;
+    }
+}
+
+int allow_lds(const void* kernel, int bytes) {
+    return bytes <= 65536 || hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? NRF_OK : NRF_ERR_LAUNCH;
+}
+
+template <class T, int FORM>
+int launch_wide_rows(const ExpertArgs& g, hipStream_t stream) {
+    typedef WideRows<T, FORM> W;
+    const int a_tiles = ((FORM == kForward ? g.n_out : g.n_in) + W::kA - 1) / W::kA;
+    auto kernel = &expert_wide_rows_kernel<T, FORM>;
+    const int st = allow_lds(reinterpret_cast<const void*>(kernel), W::Gemm::kLds);
+    if (st != NRF_OK) return st;
+    kernel<<<dim3(unsigned(xcd_blocks(PlanLayout::slots(g.n, g.E, W::kTable), a_tiles))), 512, W::Gemm::kLds, stream>>>(g, a_tiles);
+    return NRF_OK;
+}
+template <class T>
+int launch_wide_dw(const ExpertArgs& g, hipStream_t stream) {
+    typedef WideDw<T> W;
+    const int a_tiles = (g.n_in + W::kA - 1) / W::kA, b_tiles = (g.n_out + W::kB - 1) / W::kB;
+    auto kernel = &expert_wide_dw_kernel<T>;
+    const int st = allow_lds(reinterpret_cast<const void*>(kernel), W::kLds);
+    if (st != NRF_OK) return st;
+    kernel<<<dim3(unsigned((g.E + 7) / 8 * 8) * unsigned(a_tiles * b_tiles * g.splits)), 512, W::kLds, stream>>>(g, a_tiles, b_tiles);
+    return NRF_OK;
+}
+
+// Whether the wide kernels take a product: octets that do not straddle rows, operands under 4 GiB, at least half a tile's
+// rows per expert and half a tile's columns.
+bool wide(int64_t n, int E, int n_in, int n_out, int dtype) {
+    return dtype != NRF_DTYPE_FP32 && n_in % 8 == 0 && n_out % 8 == 0 && n_in >= 128 && n_out >= 128 && n / E >= 64 &&
+           n * (n_in > n_out ? n_in : n_out) < int64_t(1) << 31 && int64_t(n_out) * n_in < int64_t(1) << 31;
+}
+
 // out[i] = sum over the splits, in their order
 template <class T>
 __global__ __launch_bounds__(256) void expert_reduce_kernel(const float* __restrict__ partial, int64_t count, int splits, void* out) {
@@ -315,7 +498,13 @@ __global__ __launch_bounds__(256) void expert_reduce_kernel(const float* __restr
 
 // How many parts the sum over an expert's rows is cut into: enough workgroups for the chip where the outputs alone give too
 // few, none shorter than 256 rows of the average expert.
-int dw_splits(int64_t n, int E, int n_in, int n_out) {
+int dw_splits(int64_t n, int E, int n_in, int n_out, bool is_wide) {
+    if (is_wide) {
+        typedef WideDw<Bf16> W;
+        const int64_t tiles = int64_t(E) * ((n_in + W::kA - 1) / W::kA) * ((n_out + W::kB - 1) / W::kB);
+        const int64_t want = (256 + tiles - 1) / tiles, most = n / E / 512;
+        return int(want < most ? want : most < 1 ? 1 : most);
+    }
     const int64_t tiles = int64_t(E) * ((n_in + kT - 1) / kT) * ((n_out + kT - 1) / kT);
     const int64_t want = (1024 + tiles - 1) / tiles, most = n / E / 256;
     const int64_t s = want < most ? want : most;
@@ -358,15 +547,35 @@ NRF_EXPORT int nrf_expert_linear(const void* x, const void* weight, const void* 
     g.x = x, g.w = weight, g.bias = bias, g.plan = static_cast<const int*>(plan), g.out = y;
     g.n = n_rows, g.E = num_experts, g.n_in = n_in, g.n_out = n_out, g.relu = act == NRF_ACT_RELU, g.splits = 1;
     nrf_launch_begin();
+    if (wide(n_rows, num_experts, n_in, n_out, dtype) && nrf_aligned16(x) && nrf_aligned16(weight)) {
+        const int st = dtype == NRF_DTYPE_BF16 ? launch_wide_rows<Bf16, kForward>(g, static_cast<hipStream_t>(stream))
+                                               : launch_wide_rows<Fp16, kForward>(g, static_cast<hipStream_t>(stream));
+        return st != NRF_OK ? st : nrf_launch_status();
+    }
     launch_tile<kForward>(dtype, dim3(unsigned(PlanLayout::slots(n_rows, num_experts, 1)), (n_out + kT - 1) / kT), g,
                           static_cast<hipStream_t>(stream));
     return nrf_launch_status();
 }
 
+namespace {
+// the backward's workspace: the masked gradient (wide kernels behind a relu), then the partial sums of dW and db
+struct BackwardWork {
+    int splits;
+    int64_t dz, partial;
+    BackwardWork(int64_t n, int E, int n_in, int n_out, int dtype) {
+        const bool is_wide = wide(n, E, n_in, n_out, dtype);
+        const int tile_splits = dw_splits(n, E, n_in, n_out, false), wide_splits = is_wide ? dw_splits(n, E, n_in, n_out, true) : 1;
+        splits = tile_splits > wide_splits ? tile_splits : wide_splits;   // either kernel may run: alignment is known at the call
+        dz = is_wide ? (n * n_out * 2 + 255) & ~int64_t(255) : 0;
+        partial = splits > 1 ? int64_t(splits) * E * n_out * (n_in + 1) * 4 : 0;
+    }
+};
+}  // namespace
+
 NRF_EXPORT int64_t nrf_expert_linear_backward_workspace_bytes(int64_t n_rows, int num_experts, int n_in, int n_out, int dtype) {
     if (!shapes_ok(n_rows, num_experts, n_in, n_out, dtype, NRF_ACT_NONE)) return -1;
-    const int splits = dw_splits(n_rows, num_experts, n_in, n_out);
-    return splits > 1 ? int64_t(splits) * num_experts * n_out * (n_in + 1) * 4 : 0;
+    const BackwardWork work(n_rows, num_experts, n_in, n_out, dtype);
+    return work.dz + work.partial;
 }
 
 NRF_EXPORT int nrf_expert_linear_backward(const void* grad_y, const void* x, const void* weight, const void* y, const void* plan,
@@ -381,28 +590,43 @@ NRF_EXPORT int nrf_expert_linear_backward(const void* grad_y, const void* x, con
     for (const void* p : elems)
         if (!elem_aligned(p, dtype)) return NRF_ERR_ALIGN;
     if (!nrf_aligned16(plan) || !nrf_aligned16(workspace)) return NRF_ERR_ALIGN;
-    const int64_t need = nrf_expert_linear_backward_workspace_bytes(n_rows, num_experts, n_in, n_out, dtype);
-    if (grad_weight && need > 0 && (!workspace || workspace_bytes < need)) return NRF_ERR_WORKSPACE;
+    const BackwardWork work(n_rows, num_experts, n_in, n_out, dtype);
+    if (work.dz + work.partial > 0 && (!workspace || workspace_bytes < work.dz + work.partial)) return NRF_ERR_WORKSPACE;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     ExpertArgs g{};
     g.x = x, g.w = weight, g.y = y, g.g = grad_y, g.plan = static_cast<const int*>(plan);
     g.n = n_rows, g.E = num_experts, g.n_in = n_in, g.n_out = n_out, g.relu = act == NRF_ACT_RELU;
+    g.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + work.dz);
+    const bool is_wide = work.dz > 0 && n_rows > 0 && nrf_aligned16(grad_y) && nrf_aligned16(x) && nrf_aligned16(weight) &&
+                         nrf_aligned16(y);
     const int tiles_in = (n_in + kT - 1) / kT, tiles_out = (n_out + kT - 1) / kT;
+    int st = NRF_OK;
     nrf_launch_begin();
+    if (is_wide && g.relu) {
+        const int64_t octets = n_rows * n_out / 8, blocks = (octets + 255) / 256;
+        const dim3 grid(unsigned(blocks < 8192 ? blocks : 8192));
+        const u32x4 *dy = static_cast<const u32x4*>(grad_y), *ys = static_cast<const u32x4*>(y);
+        u32x4* dz = static_cast<u32x4*>(workspace);
+        if (dtype == NRF_DTYPE_BF16) expert_mask_kernel<Bf16><<<grid, 256, 0, stream>>>(dy, ys, octets, dz);
+        else expert_mask_kernel<Fp16><<<grid, 256, 0, stream>>>(dy, ys, octets, dz);
+        g.g = dz, g.relu = 0;
+    }
     if (grad_x && n_rows > 0) {
         g.out = grad_x, g.splits = 1;
-        launch_tile<kDx>(dtype, dim3(unsigned(PlanLayout::slots(n_rows, num_experts, 1)), tiles_in), g, stream);
+        if (!is_wide) launch_tile<kDx>(dtype, dim3(unsigned(PlanLayout::slots(n_rows, num_experts, 1)), tiles_in), g, stream);
+        else st = dtype == NRF_DTYPE_BF16 ? launch_wide_rows<Bf16, kDx>(g, stream) : launch_wide_rows<Fp16, kDx>(g, stream);
     }
-    if (grad_weight) {
+    if (grad_weight && st == NRF_OK) {
         const int64_t count = int64_t(num_experts) * n_out * n_in;
-        g.splits = dw_splits(n_rows, num_experts, n_in, n_out);
-        g.out = grad_weight, g.db = grad_bias, g.partial = static_cast<float*>(workspace);
-        launch_tile<kDw>(dtype, dim3(unsigned(num_experts) * unsigned(g.splits), tiles_in, tiles_out), g, stream);
+        g.splits = dw_splits(n_rows, num_experts, n_in, n_out, is_wide);
+        g.out = grad_weight, g.db = grad_bias;
+        if (!is_wide) launch_tile<kDw>(dtype, dim3(unsigned(num_experts) * unsigned(g.splits), tiles_in, tiles_out), g, stream);
+        else st = dtype == NRF_DTYPE_BF16 ? launch_wide_dw<Bf16>(g, stream) : launch_wide_dw<Fp16>(g, stream);
         if (g.splits > 1) {
             launch_reduce(dtype, g.partial, count, g.splits, grad_weight, stream);
             if (grad_bias)
                 launch_reduce(dtype, g.partial + g.splits * count, int64_t(num_experts) * n_out, g.splits, grad_bias, stream);
         }
     }
-    return nrf_launch_status();
+    return st != NRF_OK ? st : nrf_launch_status();
 }

@@ -96,7 +96,8 @@ __global__ __launch_bounds__(WAVES * 64) void plan_place_kernel(const int* __res
     __shared__ int s_part[WAVES];
     const int keys = E + 1, stride = (keys + 1) & ~1;      // 16-bit counters, an even number per wavefront
     int* s_off = s_mem;                                    // [keys + 1]
-    unsigned* s_cnt32 = reinterpret_cast<unsigned*>(s_mem + ((keys + 1 + 1) & ~1));
+    int* s_run = s_mem + ((keys + 2) & ~1);                // [keys + 1]
+    unsigned* s_cnt32 = reinterpret_cast<unsigned*>(s_mem + 2 * ((keys + 2) & ~1));
     unsigned short* s_cnt = reinterpret_cast<unsigned short*>(s_cnt32);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
@@ -132,21 +133,33 @@ __global__ __launch_bounds__(WAVES * 64) void plan_place_kernel(const int* __res
         plan[L.offsets + k] = s_off[k];
         if (k < E) plan[k] = s_off[k + 1] - s_off[k];
     }
+    // the tables: whole runs look their key up in the keys' sums, then every key with a rest has one run more
     for (int t = 0; t < nrf::kTileTables; ++t) {
         const int s = nrf::kTileShift0 + t;
-        const int64_t slots = PlanLayout::slots(n, E, t);
         int2* out = reinterpret_cast<int2*>(plan + L.tiles[t]);
-        for (int64_t slot = int64_t(blockIdx.x) * THREADS + threadIdx.x; slot < slots; slot += int64_t(gridDim.x) * THREADS) {
-            int lo = 0, hi = E;   // the largest key whose first slot is not past this one
+        for (int k = threadIdx.x; k < keys; k += THREADS) s_run[k] = (s_off[k + 1] - s_off[k]) >> s;
+        __syncthreads();
+        block_exclusive<THREADS>(s_run, keys, s_part);
+        const int whole = s_run[keys];
+        for (int run = blockIdx.x * THREADS + threadIdx.x; run < whole; run += gridDim.x * THREADS) {
+            int lo = 0, hi = E;   // the last key whose first run is not past this one: it has a run
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
-                if ((s_off[mid] >> s) + mid <= slot) lo = mid;
+                if (s_run[mid] <= run) lo = mid;
                 else hi = mid - 1;
             }
-            const int first = s_off[lo] + int(slot - ((s_off[lo] >> s) + lo)) * (1 << s);
-            const int left = s_off[lo + 1] - first, rows = left < 0 ? 0 : left < (1 << s) ? left : (1 << s);
-            out[slot] = make_int2(rows ? first : 0, rows << 16 | lo);
+            out[run] = make_int2(s_off[lo] + ((run - s_run[lo]) << s), 1 << (16 + s) | lo);
         }
+        __syncthreads();
+        for (int k = threadIdx.x; k < keys; k += THREADS) s_run[k] = ((s_off[k + 1] - s_off[k]) & ((1 << s) - 1)) != 0;
+        __syncthreads();
+        block_exclusive<THREADS>(s_run, keys, s_part);
+        for (int k = blockIdx.x * THREADS + threadIdx.x; k < keys; k += gridDim.x * THREADS) {
+            const int rest = (s_off[k + 1] - s_off[k]) & ((1 << s) - 1);
+            if (rest) out[whole + s_run[k]] = make_int2(s_off[k + 1] - rest, rest << 16 | k);
+        }
+        if (blockIdx.x == 0 && threadIdx.x == 0) plan[L.runs + 2 * t] = whole, plan[L.runs + 2 * t + 1] = whole + s_run[keys];
+        __syncthreads();
     }
     if (!SINGLE) {
         __syncthreads();
@@ -186,7 +199,7 @@ int64_t plan_chunk(int64_t n) {
 bool plan_single(int64_t n) { return n <= kSingleRows; }
 
 size_t place_lds(int E, int waves) {
-    return size_t((E + 3) & ~1) * 4 + size_t(waves) * ((E + 2) & ~1) * 2;
+    return size_t((E + 3) & ~1) * 8 + size_t(waves) * ((E + 2) & ~1) * 2;
 }
 
 template <int WAVES, bool SINGLE>
@@ -225,12 +238,12 @@ NRF_EXPORT int nrf_expert_plan(const int32_t* index, int64_t n_rows, int num_exp
     if (!nrf_aligned16(plan) || (work > 0 && !nrf_aligned16(workspace))) return NRF_ERR_ALIGN;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     const int E = num_experts;
-    const bool wide = E > 4096;               // eight wavefronts' counters up to 4096 experts, two beyond
+    const bool wide = E > 4096;               // eight wavefronts' counters fit in LDS up to 4096 experts, one's beyond
     int* out = static_cast<int*>(plan);
     nrf_launch_begin();
     if (plan_single(n_rows)) {
         const int64_t chunk = n_rows > 0 ? n_rows : 1;
-        const int st = wide ? launch_place<2, true>(index, n_rows, E, chunk, 1, nullptr, nullptr, out, stream)
+        const int st = wide ? launch_place<1, true>(index, n_rows, E, chunk, 1, nullptr, nullptr, out, stream)
                             : launch_place<8, true>(index, n_rows, E, chunk, 1, nullptr, nullptr, out, stream);
         return st != NRF_OK ? st : nrf_launch_status();
     }
@@ -243,7 +256,7 @@ NRF_EXPORT int nrf_expert_plan(const int32_t* index, int64_t n_rows, int num_exp
         return NRF_ERR_LAUNCH;
     plan_hist_kernel<<<dim3(unsigned(chunks)), 512, hist_lds, stream>>>(index, n_rows, E, chunk, hist);
     plan_chunks_kernel<<<dim3(unsigned(E / 64 + 1)), 1024, 0, stream>>>(hist, int(chunks), E, totals);
-    const int st = wide ? launch_place<2, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream)
+    const int st = wide ? launch_place<1, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream)
                         : launch_place<8, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream);
     return st != NRF_OK ? st : nrf_launch_status();
 }

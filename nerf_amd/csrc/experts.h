@@ -4,27 +4,29 @@
 //   offsets  [E + 1]             first grouped place of expert e; offsets[E] = rows that have an expert
 //   order    [n]                 the row at each grouped place: expert 0's rows ascending, expert 1's, ..., then the rows
 //                                of no expert (index outside [0, E)) ascending
-//   tiles    for 32, 64 and 128 rows: {first grouped place, rows << 16 | expert} of every run of at most that many rows of
-//            one expert ("expert" E: the rows of no expert); rows = 0 marks an unused slot.
-// Expert e's runs of 2^s rows sit at slots (offsets[e] >> s) + e onwards: since ceil(c / 2^s) <= ((o + c) >> s) - (o >> s) + 1
-// no two experts share a slot, so the table needs no scan of its own and its length (n >> s) + E + 1 is known on the host,
-// which sizes the products' grids with it and never reads a count back.
+//   runs     [4][2]              for each of the tables below: how many whole runs it holds, and how many in all
+//   tiles    for 32, 64, 128 and 256 rows: {first grouped place, rows << 16 | expert} of the runs of at most that many rows of
+//            one expert ("expert" E: the rows of no expert): first the whole runs in grouped order, then the experts' rests
+//            (a product's last workgroups are then its shortest)
+// A table of runs of 2^s rows has at most (n >> s) + E + 1 entries: the host sizes the products' grids with that and never
+// reads a count back; workgroups past the table's count leave at once.
 #pragma once
 #include "nrf_common.h"
 
 namespace nrf {
 
-constexpr int kMaxExperts = 16384;            // 15 bits of a tile word; the keys' counters of a workgroup fit in LDS
+constexpr int kMaxExperts = 16000;            // 15 bits of a tile word; the keys' counters of a workgroup fit in LDS
 constexpr int64_t kMaxExpertRows = 1ll << 28;
-constexpr int kTileShift0 = 5, kTileTables = 3;   // 32, 64, 128 rows
+constexpr int kTileShift0 = 5, kTileTables = 4;   // 32, 64, 128, 256 rows
 
 struct PlanLayout {
-    int64_t offsets, order, tiles[kTileTables], total;   // in int32 words; counts at 0
+    int64_t offsets, order, runs, tiles[kTileTables], total;   // in int32 words; counts at 0
     __host__ __device__ static constexpr int64_t up4(int64_t v) { return (v + 3) & ~int64_t(3); }
     __host__ __device__ static constexpr int64_t slots(int64_t n, int E, int table) { return (n >> (kTileShift0 + table)) + E + 1; }
-    __host__ __device__ constexpr PlanLayout(int64_t n, int E) : offsets(up4(E)), order(0), tiles{0, 0, 0}, total(0) {
+    __host__ __device__ constexpr PlanLayout(int64_t n, int E) : offsets(up4(E)), order(0), runs(0), tiles{0, 0, 0, 0}, total(0) {
         order = offsets + up4(E + 1);
-        int64_t at = order + up4(n);
+        runs = order + up4(n);
+        int64_t at = runs + 2 * kTileTables;
         for (int t = 0; t < kTileTables; ++t) {
             tiles[t] = at;
             at += up4(2 * slots(n, E, t));

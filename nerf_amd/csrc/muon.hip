@@ -328,7 +328,7 @@ __device__ __forceinline__ void store_terms_down(_Float16* dst, int64_t plane, i
 // both places), X' = Q X (to X' and X'^T; the last step: to the output).
 template <class T, int WHAT, int TT>
 __global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, LargeShape L, _Float16* __restrict__ work, int which) {
-    typedef DmaGemm<false, TT, TT, 2, 2, 2, 32, 3> Gemm;
+    typedef DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2> Gemm;
     extern __shared__ __align__(16) char smem[];
     const int64_t m = blockIdx.y;
     _Float16* w = work + m * L.per_matrix();
@@ -347,11 +347,10 @@ __global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, Large
     const _Float16* pb = w + (WHAT == kGram ? L.x_at(which) : WHAT == kPoly ? L.gram_at() : L.xt_at(which));
     const int64_t plane_a = int64_t(L.Mp) * K, plane_b = int64_t(WHAT == kGram || WHAT == kPoly ? L.Mp : L.Np) * K;
     Gemm gemm;
-    gemm.start(smem, [&](bool is_b, int plane, int row) {
-        return is_b ? pb + plane * plane_b + int64_t(b0 + row) * K : pa + plane * plane_a + int64_t(a0 + row) * K;
-    });
+    gemm.a.start_rows(gemm.wave, gemm.lane, pa, [&](int plane, int row) { return unsigned(plane * plane_a + int64_t(a0 + row) * K) * 2u; });
+    gemm.b.start_rows(gemm.wave, gemm.lane, pb, [&](int plane, int row) { return unsigned(plane * plane_b + int64_t(b0 + row) * K) * 2u; });
     f32x4 acc[Gemm::kMA][Gemm::kMB] = {};
-    gemm.run(smem, K / 32, acc);
+    gemm.run(smem, K, acc);
 
     const int c = gemm.lane & 15, q = gemm.lane >> 4, t = int(m / s.per);
     const int64_t base = (m % s.per) * int64_t(s.rows) * s.cols;
@@ -430,7 +429,7 @@ void launch_small(const SchulzArgs& s, hipStream_t stream) {
 
 template <class T, int WHAT, int TT>
 int launch_product(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream) {
-    typedef DmaGemm<false, TT, TT, 2, 2, 2, 32, 3> Gemm;
+    typedef DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2> Gemm;
     const int m = L.Mp / TT, n = L.Np / TT;
     const int64_t tiles = WHAT == kGram || WHAT == kPoly ? int64_t(m) * (m + 1) / 2 : int64_t(m) * n;
     auto kernel = &schulz_product_kernel<T, WHAT, TT>;

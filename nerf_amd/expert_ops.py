@@ -3,7 +3,7 @@ expert, the product of every row with its expert's weights, and the gradients.  
 happens in libnerf_amd.so.
 
 The KiloNeRF kernels (``kilo_ops``) are the fused form for one fixed tiny network per cell; these take any layer size, fp32,
-bf16 or fp16, and up to 16384 experts."""
+bf16 or fp16, and up to 16000 experts."""
 from __future__ import annotations
 
 import ctypes as C
@@ -13,7 +13,7 @@ import torch
 from ._lib import NrfError, check, lib
 from .ops import _ptr, _stream
 
-MAX_EXPERTS = 16384
+MAX_EXPERTS = 16000
 MAX_ROWS = 1 << 28
 MAX_WIDTH = 65536
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # the C ABI's NRF_DTYPE_*
@@ -167,7 +167,7 @@ def expert_linear_backward(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.
     db = torch.empty(weight.shape[:2], dtype=x.dtype, device=x.device) if want_bias else None
     L = lib()
     n_in, n_out, dtype = x.shape[1], weight.shape[1], DTYPES[x.dtype]
-    need = L.nrf_expert_linear_backward_workspace_bytes(plan.n_rows, plan.num_experts, n_in, n_out, dtype) if want_weight else 0
+    need = L.nrf_expert_linear_backward_workspace_bytes(plan.n_rows, plan.num_experts, n_in, n_out, dtype)
     work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     with torch.cuda.device(x.device):
         check(L.nrf_expert_linear_backward(_ptr(grad_y), _ptr(x), _ptr(weight), _ptr(y), _ptr(plan.buffer), plan.n_rows,

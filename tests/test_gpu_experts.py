@@ -45,7 +45,7 @@ def plan_by_definition(index, E):
 
 
 @pytest.mark.parametrize("n,E", [(0, 3), (1, 1), (2, 5), (63, 1), (64, 2), (65, 4096), (1000, 7), (8192, 64), (8193, 64),
-                                 (8193, 4096), (40000, 4097), (5000, 16384), (100003, 16384), (300001, 1), (1200007, 4096)])
+                                 (8193, 4096), (40000, 4097), (5000, 16000), (100003, 16000), (300001, 1), (1200007, 4096)])
 @pytest.mark.parametrize("kind", ["uniform", "skew", "outside"])
 def test_plan(n, E, kind):
     index = index_of(n, E, kind, n + E)
@@ -54,17 +54,21 @@ def test_plan(n, E, kind):
     assert np.array_equal(plan.counts.cpu().numpy(), counts)
     assert np.array_equal(plan.offsets.cpu().numpy(), offsets)
     assert np.array_equal(plan.order.cpu().numpy(), order)
-    # the tile tables: every grouped place, the rows of no expert among them, in exactly one run of one expert
+    # the tile tables: every grouped place, the rows of no expert among them, in exactly one run of one expert, whole runs first
     at = expert_ops._up4(E) + expert_ops._up4(E + 1) + expert_ops._up4(n)
-    for shift in (5, 6, 7):
-        slots = (n >> shift) + E + 1
-        table = plan.buffer[at:at + 2 * slots].view(-1, 2).cpu().numpy().astype(np.int64)
-        at += expert_ops._up4(2 * slots)
+    runs = plan.buffer[at:at + 8].view(4, 2).tolist()
+    at += 8
+    ends = np.concatenate([offsets, [n]])
+    for shift, (whole, count) in zip((5, 6, 7, 8), runs):
+        assert whole == (np.diff(ends) >> shift).sum()
+        assert count == (-(-np.diff(ends) // (1 << shift))).sum() <= (n >> shift) + E + 1
+        table = plan.buffer[at:at + 2 * count].view(-1, 2).cpu().numpy().astype(np.int64)
+        at += expert_ops._up4(2 * ((n >> shift) + E + 1))
         first, rows, expert = table[:, 0], table[:, 1] >> 16, table[:, 1] & 0xffff
-        first, rows, expert = first[rows > 0], rows[rows > 0], expert[rows > 0]
-        assert (rows <= 1 << shift).all() and rows.sum() == n
-        assert np.array_equal(first, np.cumsum(rows) - rows)
-        ends = np.concatenate([offsets, [n]])
+        assert (rows[:whole] == 1 << shift).all() and (rows > 0).all() and (rows[whole:] < 1 << shift).all()
+        assert (np.diff(first[:whole]) > 0).all() and (np.diff(first[whole:]) > 0).all()
+        grouped = np.argsort(first)
+        assert rows.sum() == n and np.array_equal(first[grouped], np.cumsum(rows[grouped]) - rows[grouped])
         assert (first >= ends[expert]).all() and (first + rows <= ends[expert + 1]).all()
 
 
@@ -121,7 +125,8 @@ SHAPES = [  # n, E, n_in, n_out, kind
     (1, 1, 1, 1, "uniform"), (1, 4, 64, 32, "uniform"), (7, 3, 5, 3, "uniform"), (48, 32, 256, 128, "skew"),
     (33, 2, 63, 32, "uniform"), (300, 5, 32, 32, "outside"), (1000, 64, 63, 32, "skew"), (2000, 3, 319, 256, "uniform"),
     (129, 2, 130, 257, "one"), (64, 3, 16, 8, "none"), (2500, 8, 96, 100, "skew"), (515, 1, 1024, 40, "uniform"),
-    (700, 2, 512, 640, "uniform"),
+    (700, 2, 512, 640, "uniform"), (900, 3, 264, 136, "outside"), (1300, 2, 128, 520, "skew"), (5000, 1, 136, 128, "one"),
+    (640, 8, 200, 328, "skew"),
 ]
 
 
@@ -305,7 +310,7 @@ def test_refusals():
     for bad in (index.long(), index.view(2, 20), index.cpu()):
         with pytest.raises(E):
             expert_plan(bad, 2)
-    for experts in (0, -1, 16385):
+    for experts in (0, -1, 16001):
         with pytest.raises(E):
             expert_plan(index, experts)
     for args in ((x[:39], w, b, plan), (x, w[:1], b, plan), (x, w, b[:, :5], plan), (x, w[:, :, :7], b, plan),
