@@ -502,7 +502,7 @@ int nrf_kilo_clip_adam(float* const* params, float* const* grads, float* const* 
 /* ---- rows grouped by expert: matrix products with one weight matrix per expert -------------------------------------- */
 
 /* The general form of what nrf_kilo_forward does for its fixed tiny networks: row i of a batch goes through the weights of
- * expert index[i].  Any number of experts up to 16000, layer sizes up to 65536, up to 2^28 rows, three types.  (The reference
+ * expert index[i].  Any number of experts up to 16384, layer sizes up to 65536, up to 2^28 rows, three types.  (The reference
  * has no counterpart beyond BatchedKiloNeRF's bmm over padded cells, src/models/kilonerf/network.py:123-167.)  Pointers are
  * contiguous tensors of `dtype`, aligned to one element; the plan and workspaces to 16 bytes.  Every entry point may be
  * captured into a graph; nothing is read back. */

@@ -5,7 +5,7 @@
 // is the counter of its expert plus the number of lower lanes with the same expert (found with one ballot per bit of the
 // expert's number, no atomics), so equal keys keep their order and the result is the same on every run.
 // Up to kSingleRows rows are one workgroup and one launch.  Beyond, the rows are cut into chunks, one workgroup each: chunk
-// histograms (launch 1), an exclusive sum over the chunks per expert (launch 2), the walk (launch 3).
+// histograms (launch 1), an exclusive sum over the chunks per expert (launch 2), the walk and beside it the run tables (launch 3).
 #include "experts.h"
 
 namespace {
@@ -24,31 +24,82 @@ __device__ __forceinline__ int wave_scan_int(int v) {   // inclusive
     return v;
 }
 
-__device__ __forceinline__ int key_of(const int* __restrict__ index, int64_t row, int E) {
-    const int e = index[row];
-    return (unsigned)e < (unsigned)E ? e : E;
+// The keys of rows first, first + stride, ... (kAhead of them, their loads in flight together), -1 past `end`
+constexpr int kAhead = 8;
+__device__ __forceinline__ void load_keys(const int* __restrict__ index, int64_t first, int stride, int64_t end, int E, int (&key)[kAhead]) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) key[i] = first + i * stride < end ? index[first + i * stride] : 0;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const int k = (unsigned)key[i] < (unsigned)E ? key[i] : E;
+        key[i] = first + i * stride < end ? k : -1;
+    }
 }
 
-// In place: s[0 .. count) -> exclusive sums, s[count] = total.  All THREADS threads; `part` has THREADS / 64 ints.
-template <int THREADS>
-__device__ void block_exclusive(int* s, int count, int* part) {
-    const int per = (count + THREADS - 1) / THREADS, at = threadIdx.x * per;
-    int sum = 0;
-    for (int i = 0; i < per; ++i)
-        if (at + i < count) sum += s[at + i];
-    const int incl = wave_scan_int(sum);
-    if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = incl;
-    __syncthreads();
-    int run = incl - sum;
-    for (int w = 0; w < int(threadIdx.x >> 6); ++w) run += part[w];
-    for (int i = 0; i < per; ++i)
-        if (at + i < count) {
-            const int v = s[at + i];
-            s[at + i] = run;
-            run += v;
+// Exclusive sums over the keys' rows (and, TABLES, over their whole runs and rests of the four run lengths): thread i owns the
+// keys [i per, (i + 1) per).  before[]: the sums over all keys before this thread's; total[]: over all.  `part`: Q per wavefront.
+template <int WAVES, int Q, class F>
+__device__ __forceinline__ void key_sums(int keys, int* part, F rows_of, int (&before)[Q], int (&total)[Q], int table0 = 0) {
+    const int per = (keys + WAVES * 64 - 1) / (WAVES * 64), at = threadIdx.x * per, wave = threadIdx.x >> 6;
+    int sum[Q] = {};
+    for (int k = at; k < at + per && k < keys; ++k) {
+        const int c = rows_of(k);
+        sum[0] += c;
+#pragma unroll
+        for (int t = 0; t < (Q - 1) / 2; ++t) {
+            const int s = nrf::kTileShift0 + table0 + t;
+            sum[1 + 2 * t] += c >> s, sum[2 + 2 * t] += (c & ((1 << s) - 1)) != 0;
         }
-    if (threadIdx.x == THREADS - 1) s[count] = run;   // its range is the last one (empty ranges carry the sum on)
+    }
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+        const int incl = wave_scan_int(sum[i]);
+        before[i] = incl - sum[i];
+        if ((threadIdx.x & 63) == 63) part[wave * Q + i] = incl;
+    }
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+        total[i] = 0;
+        for (int w = 0; w < WAVES; ++w) {
+            if (w == wave) before[i] += total[i];
+            total[i] += part[w * Q + i];
+        }
+    }
+    __syncthreads();
+}
+
+// Key k's runs of 2^s rows in table `out` (whole ones from `first`, the rest at `last`): a key's first runs and its rest by its
+// own lane, where `mine`; further ones by the wavefront, share `share` of `shares`.  All 64 lanes call it; rows = 0 has none.
+__device__ __forceinline__ void fill_runs(int2* out, int s, int k, int off, int rows, int first, int last, bool mine, int share, int shares) {
+    const int whole = rows >> s, rest = rows & ((1 << s) - 1), direct = !mine ? 0 : whole < 16 ? whole : 16;
+    for (int r = 0; r < direct; ++r) out[first + r] = make_int2(off + (r << s), 1 << (16 + s) | k);
+    for (unsigned long long many = __ballot(whole > 16); many; many &= many - 1) {
+        const int l = __ffsll((long long)many) - 1;
+        const int w = __builtin_amdgcn_readlane(whole, l), f = __builtin_amdgcn_readlane(first, l),
+                  o = __builtin_amdgcn_readlane(off, l), key = __builtin_amdgcn_readlane(k, l);
+        for (int r = 16 + 64 * share + int(threadIdx.x & 63); r < w; r += 64 * shares) out[f + r] = make_int2(o + (r << s), 1 << (16 + s) | key);
+    }
+    if (mine && rest) out[last] = make_int2(off + rows - rest, rest << 16 | k);
+}
+constexpr int kSums = 1 + 2 * nrf::kTileTables;
+// counts, offsets and the run tables' lengths; at: this thread's sums before its key k, total: over all keys
+__device__ __forceinline__ void write_key(const PlanLayout& L, int* plan, int E, int k, int rows, int off) {
+    plan[L.offsets + k] = off;
+    if (k < E) plan[k] = rows;
+}
+__device__ __forceinline__ void write_lengths(const PlanLayout& L, int* plan, const int (&total)[kSums]) {
+#pragma unroll
+    for (int t = 0; t < nrf::kTileTables; ++t)
+        plan[L.runs + 2 * t] = total[1 + 2 * t], plan[L.runs + 2 * t + 1] = total[1 + 2 * t] + total[2 + 2 * t];
+}
+__device__ __forceinline__ void pass_key(int rows, int (&at)[kSums]) {
+    at[0] += rows;
+#pragma unroll
+    for (int t = 0; t < nrf::kTileTables; ++t) {
+        const int s = nrf::kTileShift0 + t;
+        at[1 + 2 * t] += rows >> s, at[2 + 2 * t] += (rows & ((1 << s) - 1)) != 0;
+    }
 }
 
 __global__ __launch_bounds__(512) void plan_hist_kernel(const int* __restrict__ index, int64_t n, int E, int64_t chunk,
@@ -57,7 +108,13 @@ __global__ __launch_bounds__(512) void plan_hist_kernel(const int* __restrict__ 
     for (int k = threadIdx.x; k <= E; k += 512) s_count[k] = 0;
     __syncthreads();
     const int64_t begin = blockIdx.x * chunk, end = begin + chunk < n ? begin + chunk : n;
-    for (int64_t r = begin + threadIdx.x; r < end; r += 512) atomicAdd(&s_count[key_of(index, r, E)], 1);
+    for (int64_t r = begin + threadIdx.x; r < end; r += 512 * kAhead) {
+        int key[kAhead];
+        load_keys(index, r, 512, end, E, key);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (key[i] >= 0) atomicAdd(&s_count[key[i]], 1);
+    }
     __syncthreads();
     for (int k = threadIdx.x; k <= E; k += 512) hist[int64_t(blockIdx.x) * (E + 1) + k] = s_count[k];
 }
@@ -69,137 +126,160 @@ __global__ __launch_bounds__(1024) void plan_chunks_kernel(int* __restrict__ his
     const int per = (chunks + 15) / 16, c0 = wave * per, c1 = c0 + per < chunks ? c0 + per : chunks;
     int sum = 0;
     if (key <= E)
-#pragma unroll 8
+#pragma unroll 16
         for (int c = c0; c < c1; ++c) sum += hist[int64_t(c) * (E + 1) + key];
     s_sum[wave][lane] = sum;
     __syncthreads();
     int run = 0;
     for (int w = 0; w < wave; ++w) run += s_sum[w][lane];
     if (key > E) return;
-#pragma unroll 8
+    if (wave == 15) totals[key] = run + sum;
+#pragma unroll 16
     for (int c = c0; c < c1; ++c) {
         int* p = hist + int64_t(c) * (E + 1) + key;
         const int v = *p;
         *p = run;
         run += v;
     }
-    if (wave == 15) totals[key] = run;
 }
 
-// The walk.  SINGLE: the one workgroup of a small batch, which also makes the totals.
+// Workgroups 0 .. kTableBlocks - 1: the run tables, kTableShares for each table; table 0's also write counts and offsets.  Those
+// behind them: the walk.  SINGLE: one workgroup does it all.
+constexpr int kTableShares = 8, kTableBlocks = nrf::kTileTables * kTableShares;
 template <int WAVES, bool SINGLE>
 __global__ __launch_bounds__(WAVES * 64) void plan_place_kernel(const int* __restrict__ index, int64_t n, int E, int64_t chunk,
                                                                 const int* __restrict__ hist, const int* __restrict__ totals,
                                                                 int* __restrict__ plan) {
     constexpr int THREADS = WAVES * 64;
     extern __shared__ int s_mem[];
-    __shared__ int s_part[WAVES];
+    __shared__ int s_part[WAVES * kSums];
+    const PlanLayout L(n, E);
     const int keys = E + 1, stride = (keys + 1) & ~1;      // 16-bit counters, an even number per wavefront
-    int* s_off = s_mem;                                    // [keys + 1]
-    int* s_run = s_mem + ((keys + 2) & ~1);                // [keys + 1]
-    unsigned* s_cnt32 = reinterpret_cast<unsigned*>(s_mem + 2 * ((keys + 2) & ~1));
+    const int each = (keys + THREADS - 1) / THREADS;
+    int* s_off = s_mem;                                    // [keys], rounded up to a pair: the keys' rows, then their places
+    if (!SINGLE) {
+#pragma unroll 8
+        for (int k = threadIdx.x; k < keys; k += THREADS) s_off[k] = totals[k];
+        if (blockIdx.x < kTableBlocks) {
+            const int t = blockIdx.x / kTableShares, share = blockIdx.x % kTableShares, s = nrf::kTileShift0 + t;
+            int2* out = reinterpret_cast<int2*>(plan + L.tiles[0] + (t > 0 ? L.tiles[1] - L.tiles[0] : 0) + (t > 1 ? L.tiles[2] - L.tiles[1] : 0) +
+                                                (t > 2 ? L.tiles[3] - L.tiles[2] : 0));
+            __syncthreads();
+            int at[3], total[3];
+            key_sums<WAVES, 3>(keys, s_part, [&](int k) { return s_off[k]; }, at, total, t);
+            for (int i = 0; i < each; ++i) {
+                const int k = threadIdx.x * each + i, rows = k < keys ? s_off[k] : 0;
+                const bool mine = i % kTableShares == share;
+                if (t == 0 && mine && k < keys) write_key(L, plan, E, k, rows, at[0]);
+                fill_runs(out, s, k, at[0], rows, at[1], total[1] + at[2], mine, share, kTableShares);
+                at[0] += rows, at[1] += rows >> s, at[2] += (rows & ((1 << s) - 1)) != 0;
+            }
+            if (share == 0 && threadIdx.x == 0) plan[L.runs + 2 * t] = total[1], plan[L.runs + 2 * t + 1] = total[1] + total[2];
+            return;
+        }
+    }
+    const int64_t block = SINGLE ? 0 : blockIdx.x - kTableBlocks;
+    unsigned* s_cnt32 = reinterpret_cast<unsigned*>(s_mem + stride);
     unsigned short* s_cnt = reinterpret_cast<unsigned short*>(s_cnt32);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
     for (int i = threadIdx.x; i < WAVES * stride / 2; i += THREADS) s_cnt32[i] = 0;
-    if (!SINGLE)
-        for (int k = threadIdx.x; k < keys; k += THREADS) s_off[k] = totals[k];
     __syncthreads();
 
-    const int64_t begin = blockIdx.x * chunk, end = begin + chunk < n ? begin + chunk : n;
+    const int64_t begin = block * chunk, end = begin + chunk < n ? begin + chunk : n;
     const int64_t per = ((end - begin + THREADS - 1) / THREADS) * 64;   // rows of a wavefront, whole 64s
     const int64_t w0 = begin + wave * per, w1 = w0 + per < end ? w0 + per : end;
     unsigned short* mine = s_cnt + wave * stride;
-    for (int64_t r = w0 + lane; r < w1; r += 64) {
-        const int slot = wave * stride + key_of(index, r, E);
-        atomicAdd(&s_cnt32[slot >> 1], (slot & 1) ? 0x10000u : 1u);
+    for (int64_t r = w0 + lane; r < w1; r += 64 * kAhead) {
+        int key[kAhead];
+        load_keys(index, r, 64, w1, E, key);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int slot = wave * stride + key[i];
+            if (key[i] >= 0) atomicAdd(&s_cnt32[slot >> 1], (slot & 1) ? 0x10000u : 1u);
+        }
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < keys; k += THREADS) {
-        int run = 0;
+    for (int p = threadIdx.x; p < stride / 2; p += THREADS) {   // two keys at a time: a chunk's counts stay under 2^16
+        unsigned run = 0;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-            const int v = s_cnt[w * stride + k];
-            s_cnt[w * stride + k] = (unsigned short)run;
+            const unsigned v = s_cnt32[w * (stride / 2) + p];
+            s_cnt32[w * (stride / 2) + p] = run;
             run += v;
         }
-        if (SINGLE) s_off[k] = run;
+        if (SINGLE) s_off[2 * p] = int(run & 0xffffu), s_off[2 * p + 1] = int(run >> 16);
     }
     __syncthreads();
-    block_exclusive<THREADS>(s_off, keys, s_part);
-
-    const PlanLayout L(n, E);
-    for (int k = blockIdx.x * THREADS + threadIdx.x; k < keys; k += gridDim.x * THREADS) {
-        plan[L.offsets + k] = s_off[k];
-        if (k < E) plan[k] = s_off[k + 1] - s_off[k];
-    }
-    // the tables: whole runs look their key up in the keys' sums, then every key with a rest has one run more
-    for (int t = 0; t < nrf::kTileTables; ++t) {
-        const int s = nrf::kTileShift0 + t;
-        int2* out = reinterpret_cast<int2*>(plan + L.tiles[t]);
-        for (int k = threadIdx.x; k < keys; k += THREADS) s_run[k] = (s_off[k + 1] - s_off[k]) >> s;
-        __syncthreads();
-        block_exclusive<THREADS>(s_run, keys, s_part);
-        const int whole = s_run[keys];
-        for (int run = blockIdx.x * THREADS + threadIdx.x; run < whole; run += gridDim.x * THREADS) {
-            int lo = 0, hi = E;   // the last key whose first run is not past this one: it has a run
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (s_run[mid] <= run) lo = mid;
-                else hi = mid - 1;
-            }
-            out[run] = make_int2(s_off[lo] + ((run - s_run[lo]) << s), 1 << (16 + s) | lo);
+    // where this chunk's rows of each key begin
+    if (SINGLE) {
+        int at[kSums], total[kSums];
+        key_sums<WAVES, kSums>(keys, s_part, [&](int k) { return s_off[k]; }, at, total);
+        for (int i = 0; i < each; ++i) {
+            const int k = threadIdx.x * each + i, rows = k < keys ? s_off[k] : 0;
+            if (k < keys) write_key(L, plan, E, k, rows, at[0]), s_off[k] = at[0];
+#pragma unroll
+            for (int t = 0; t < nrf::kTileTables; ++t)
+                fill_runs(reinterpret_cast<int2*>(plan + L.tiles[t]), nrf::kTileShift0 + t, k, at[0], rows, at[1 + 2 * t],
+                          total[1 + 2 * t] + at[2 + 2 * t], true, 0, 1);
+            pass_key(rows, at);
+        }
+        if (threadIdx.x == 0) write_lengths(L, plan, total);
+    } else {
+        int at[1], total[1];
+        key_sums<WAVES, 1>(keys, s_part, [&](int k) { return s_off[k]; }, at, total);
+        for (int k = threadIdx.x * each; k < int(threadIdx.x + 1) * each && k < keys; ++k) {
+            const int rows = s_off[k];
+            s_off[k] = at[0];
+            at[0] += rows;
         }
         __syncthreads();
-        for (int k = threadIdx.x; k < keys; k += THREADS) s_run[k] = ((s_off[k + 1] - s_off[k]) & ((1 << s) - 1)) != 0;
-        __syncthreads();
-        block_exclusive<THREADS>(s_run, keys, s_part);
-        for (int k = blockIdx.x * THREADS + threadIdx.x; k < keys; k += gridDim.x * THREADS) {
-            const int rest = (s_off[k + 1] - s_off[k]) & ((1 << s) - 1);
-            if (rest) out[whole + s_run[k]] = make_int2(s_off[k + 1] - rest, rest << 16 | k);
-        }
-        if (blockIdx.x == 0 && threadIdx.x == 0) plan[L.runs + 2 * t] = whole, plan[L.runs + 2 * t + 1] = whole + s_run[keys];
-        __syncthreads();
-    }
-    if (!SINGLE) {
-        __syncthreads();
-        for (int k = threadIdx.x; k < keys; k += THREADS) s_off[k] += hist[int64_t(blockIdx.x) * keys + k];
+#pragma unroll 8
+        for (int k = threadIdx.x; k < keys; k += THREADS) s_off[k] += hist[block * keys + k];
     }
     __syncthreads();
 
     int* order = plan + L.order;
     const int bits = 32 - __clz(E);                        // keys 0 .. E
     const unsigned long long below = (1ull << lane) - 1;
-    for (int64_t r0 = w0; r0 < w1; r0 += 64) {
-        const int64_t r = r0 + lane;
-        const bool there = r < w1;
-        const int key = there ? key_of(index, r, E) : 0;
-        unsigned long long same = __ballot(there);
-        for (int b = 0; b < bits; ++b) {
-            const bool one = (key >> b) & 1;
-            const unsigned long long m = __ballot(one);
-            same &= one ? m : ~m;
+    for (int64_t r0 = w0; r0 < w1; r0 += 64 * kAhead) {
+        int keys_ahead[kAhead];
+        load_keys(index, r0 + lane, 64, w1, E, keys_ahead);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int key = keys_ahead[i];
+            if (r0 + 64 * i >= w1) break;
+            const unsigned long long there = __ballot(key >= 0);
+            unsigned lo = unsigned(there), hi = unsigned(there >> 32);   // the lanes with this one's key
+#pragma unroll
+            for (int b = 0; b < 15; ++b) {                               // bits that no key has change nothing
+                if (b >= 8 && bits <= 8) continue;
+                const int one = (key << (31 - b)) >> 31;                 // all ones where bit b is set
+                const unsigned long long m = __ballot(one != 0);
+                lo &= ~(unsigned(m) ^ unsigned(one)), hi &= ~(unsigned(m >> 32) ^ unsigned(one));
+            }
+            const unsigned long long same = (unsigned long long)hi << 32 | lo;
+            if (key >= 0) {
+                const int start = mine[key];
+                order[s_off[key] + start + __popcll(same & below)] = int(r0) + 64 * i + lane;
+                if ((same >> lane) == 1) mine[key] = (unsigned short)(start + __popcll(same));   // the highest lane of the key
+            }
+            // the next 64 rows' lanes read what these lanes wrote: same wavefront, LDS in order, the compiler kept from moving it
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
-        if (there) {
-            const int start = mine[key];
-            order[s_off[key] + start + __popcll(same & below)] = int(r);
-            if ((same >> lane) == 1) mine[key] = (unsigned short)(start + __popcll(same));   // the highest lane of the key
-        }
-        // the next 64 rows' lanes read what these lanes wrote: same wavefront, LDS in order, the compiler kept from moving it
-        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-        __builtin_amdgcn_wave_barrier();
     }
 }
 
 int64_t plan_chunk(int64_t n) {
-    int64_t chunk = (n + 255) / 256;          // one workgroup per CU; a counter of a chunk has 16 bits
+    int64_t chunk = (n + 223) / 224;          // with the tables' 32, one workgroup per CU; a counter of a chunk has 16 bits
     if (chunk < 2048) chunk = 2048;
     return chunk > 32768 ? 32768 : chunk;
 }
 bool plan_single(int64_t n) { return n <= kSingleRows; }
 
 size_t place_lds(int E, int waves) {
-    return size_t((E + 3) & ~1) * 8 + size_t(waves) * ((E + 2) & ~1) * 2;
+    return size_t((E + 2) & ~1) * 4 + size_t(waves) * ((E + 2) & ~1) * 2;
 }
 
 template <int WAVES, bool SINGLE>
@@ -209,8 +289,8 @@ int launch_place(const int* index, int64_t n, int E, int64_t chunk, int64_t chun
         hipFuncSetAttribute(reinterpret_cast<const void*>(&plan_place_kernel<WAVES, SINGLE>), hipFuncAttributeMaxDynamicSharedMemorySize,
                             int(place_lds(E, WAVES))) != hipSuccess)
         return NRF_ERR_LAUNCH;
-    plan_place_kernel<WAVES, SINGLE><<<dim3(unsigned(chunks)), WAVES * 64, place_lds(E, WAVES), stream>>>(index, n, E, chunk, hist,
-                                                                                                         totals, plan);
+    const unsigned grid = unsigned(chunks) + (SINGLE ? 0 : kTableBlocks);
+    plan_place_kernel<WAVES, SINGLE><<<dim3(grid), WAVES * 64, place_lds(E, WAVES), stream>>>(index, n, E, chunk, hist, totals, plan);
     return NRF_OK;
 }
 
@@ -238,12 +318,12 @@ NRF_EXPORT int nrf_expert_plan(const int32_t* index, int64_t n_rows, int num_exp
     if (!nrf_aligned16(plan) || (work > 0 && !nrf_aligned16(workspace))) return NRF_ERR_ALIGN;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     const int E = num_experts;
-    const bool wide = E > 4096;               // eight wavefronts' counters fit in LDS up to 4096 experts, one's beyond
+    const bool wide = E > 4096;               // eight wavefronts' counters fit in LDS up to 4096 experts, two's beyond
     int* out = static_cast<int*>(plan);
     nrf_launch_begin();
     if (plan_single(n_rows)) {
         const int64_t chunk = n_rows > 0 ? n_rows : 1;
-        const int st = wide ? launch_place<1, true>(index, n_rows, E, chunk, 1, nullptr, nullptr, out, stream)
+        const int st = wide ? launch_place<2, true>(index, n_rows, E, chunk, 1, nullptr, nullptr, out, stream)
                             : launch_place<8, true>(index, n_rows, E, chunk, 1, nullptr, nullptr, out, stream);
         return st != NRF_OK ? st : nrf_launch_status();
     }
@@ -256,7 +336,7 @@ NRF_EXPORT int nrf_expert_plan(const int32_t* index, int64_t n_rows, int num_exp
         return NRF_ERR_LAUNCH;
     plan_hist_kernel<<<dim3(unsigned(chunks)), 512, hist_lds, stream>>>(index, n_rows, E, chunk, hist);
     plan_chunks_kernel<<<dim3(unsigned(E / 64 + 1)), 1024, 0, stream>>>(hist, int(chunks), E, totals);
-    const int st = wide ? launch_place<1, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream)
+    const int st = wide ? launch_place<2, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream)
                         : launch_place<8, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream);
     return st != NRF_OK ? st : nrf_launch_status();
 }

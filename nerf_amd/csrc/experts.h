@@ -15,7 +15,7 @@
 
 namespace nrf {
 
-constexpr int kMaxExperts = 16000;            // 15 bits of a tile word; the keys' counters of a workgroup fit in LDS
+constexpr int kMaxExperts = 16384;            // 15 bits of a tile word; the keys' counters of a workgroup fit in LDS
 constexpr int64_t kMaxExpertRows = 1ll << 28;
 constexpr int kTileShift0 = 5, kTileTables = 4;   // 32, 64, 128, 256 rows
 

@@ -3,7 +3,7 @@ expert, the product of every row with its expert's weights, and the gradients.  
 happens in libnerf_amd.so.
 
 The KiloNeRF kernels (``kilo_ops``) are the fused form for one fixed tiny network per cell; these take any layer size, fp32,
-bf16 or fp16, and up to 16000 experts."""
+bf16 or fp16, and up to 16384 experts."""
 from __future__ import annotations
 
 import ctypes as C
@@ -13,7 +13,7 @@ import torch
 from ._lib import NrfError, check, lib
 from .ops import _ptr, _stream
 
-MAX_EXPERTS = 16000
+MAX_EXPERTS = 16384
 MAX_ROWS = 1 << 28
 MAX_WIDTH = 65536
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # the C ABI's NRF_DTYPE_*

@@ -9,7 +9,7 @@ from nerf_amd import _lib, expert_ops
 
 def test_sizes_out_of_range():
     L = _lib.lib()
-    assert L.nrf_expert_plan_bytes(10, 0) == -1 and L.nrf_expert_plan_bytes(10, 16001) == -1
+    assert L.nrf_expert_plan_bytes(10, 0) == -1 and L.nrf_expert_plan_bytes(10, 16385) == -1
     assert L.nrf_expert_plan_bytes(-1, 4) == -1 and L.nrf_expert_plan_bytes((1 << 28) + 1, 4) == -1
     assert L.nrf_expert_plan_workspace_bytes(8192, 4) == 0 and L.nrf_expert_plan_workspace_bytes(8193, 4) > 0
     assert L.nrf_expert_linear_backward_workspace_bytes(10, 4, 0, 4, 0) == -1

@@ -45,7 +45,7 @@ def plan_by_definition(index, E):
 
 
 @pytest.mark.parametrize("n,E", [(0, 3), (1, 1), (2, 5), (63, 1), (64, 2), (65, 4096), (1000, 7), (8192, 64), (8193, 64),
-                                 (8193, 4096), (40000, 4097), (5000, 16000), (100003, 16000), (300001, 1), (1200007, 4096)])
+                                 (8193, 4096), (40000, 4097), (5000, 16384), (100003, 16384), (300001, 1), (1200007, 4096)])
 @pytest.mark.parametrize("kind", ["uniform", "skew", "outside"])
 def test_plan(n, E, kind):
     index = index_of(n, E, kind, n + E)
@@ -310,7 +310,7 @@ def test_refusals():
     for bad in (index.long(), index.view(2, 20), index.cpu()):
         with pytest.raises(E):
             expert_plan(bad, 2)
-    for experts in (0, -1, 16001):
+    for experts in (0, -1, 16385):
         with pytest.raises(E):
             expert_plan(index, experts)
     for args in ((x[:39], w, b, plan), (x, w[:1], b, plan), (x, w, b[:, :5], plan), (x, w[:, :, :7], b, plan),
