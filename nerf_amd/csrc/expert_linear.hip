@@ -486,6 +486,274 @@ bool wide(int64_t n, int E, int n_in, int n_out, int dtype) {
            n * (n_in > n_out ? n_in : n_out) < int64_t(1) << 31 && int64_t(n_out) * n_in < int64_t(1) << 31;
 }
 
+// ---- fp32, thousands of tiny layers (at most 64 x 64) -----------------------------------------------------------------------
+// v_mfma_f32_32x32x2_f32 on 32 rows per wavefront: memory bounds these (a 63 -> 32 layer moves 380 B and multiplies 2016 times
+// per row; the fp32 matrix pipe needs half of that time).  Rows of any length and alignment are loaded lanes along the row,
+// 4 B each (fragments straight from memory, 16 B per lane at row pitch, occupy the address unit for longer than the rest
+// takes: 47 us for 262 k rows, 63 -> 32; rows by 4 B LDS-DMA 59 us), and turned through LDS at an odd pitch.
+#define NRF_MFMA_F32(a, b, c) __builtin_amdgcn_mfma_f32_32x32x2f32((a), (b), (c), 0, 0, 0)
+
+// COUNT rows (row i at base + row_of(i) * width, uniform), one load of 64 lanes x 4 B each; zeros past the row's end.  Lanes past
+// it read its last element: loads under no condition are in flight together.
+template <int COUNT, class F>
+__device__ __forceinline__ void load_rows(float (&v)[COUNT], const float* base, int width, int lane, F row_of) {
+    const int at = lane < width ? lane : width - 1;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) v[i] = (base + int64_t(__builtin_amdgcn_readfirstlane(row_of(i))) * width)[at];
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) v[i] = lane < width ? v[i] : 0.f;
+}
+// a wavefront's own LDS: in order in the hardware, the compiler kept from moving accesses across
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+template <int COUNT>
+__device__ __forceinline__ void keep_rows(const float (&v)[COUNT], int padded, float* s_rows, int pitch, int lane) {
+    if (lane < padded)
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) s_rows[i * pitch + lane] = v[i];
+}
+
+// A workgroup takes a run of at most 128 rows of one expert, a wavefront 32 of them; the weights are shared.
+constexpr int kCellRows = 128, kCellRowsTable = 2;
+template <int NI, int NO>
+__global__ __launch_bounds__(256) void expert_cell_forward_kernel(ExpertArgs g) {
+    constexpr int kPitch = 32 * NI + 1;
+    __shared__ float s_w[NO * 32 * kPitch], s_all[4][32 * 33];
+    const PlanLayout L(g.n, g.E);
+    const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[kCellRowsTable])[blockIdx.x];   // inside the table's room
+    if (int(blockIdx.x) >= g.plan[L.runs + 2 * kCellRowsTable + 1]) return;
+    const int expert = tile.y & 0xffff, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
+    const int left = (tile.y >> 16) - wave * 32, rows = left < 0 ? 0 : left < 32 ? left : 32;
+    const bool none = expert == g.E;
+    float* s_x = s_all[wave];
+    const int mine = c < rows ? g.plan[L.order + tile.x + wave * 32 + c] : 0;
+    f32x16 acc[NO] = {};
+    if (!none) {
+        const float* w = static_cast<const float*>(g.w) + int64_t(expert) * g.n_out * g.n_in;
+        const int f0 = wave * 8 * NO;
+        float wv[8 * NO], xv[32];
+        load_rows<8 * NO>(wv, w, g.n_in, lane, [&](int i) { return f0 + i < g.n_out ? f0 + i : g.n_out - 1; });
+        load_rows<32>(xv, static_cast<const float*>(g.x), g.n_in, lane, [&](int i) { return __builtin_amdgcn_readlane(mine, i); });
+        if (g.bias) {
+            const float* b = static_cast<const float*>(g.bias) + int64_t(expert) * g.n_out;
+#pragma unroll
+            for (int o = 0; o < NO; ++o)
+#pragma unroll
+                for (int t = 0; t < 16; ++t) {
+                    const int f = 32 * o + nrf::acc_row(t, h);
+                    acc[o][t] = f < g.n_out ? b[f] : 0.f;
+                }
+        }
+        keep_rows(wv, 32 * NI, s_w + f0 * kPitch, kPitch, lane);
+        __syncthreads();
+        const float *px = s_x + c * 33 + h, *pw = s_w + c * kPitch + h;
+#pragma unroll
+        for (int half = 0; half < NI; ++half) {        // 32 inputs at a time through the wavefront's own piece of LDS
+            if (half) wave_order();
+            if (NI == 1 ? lane < 32 : lane >> 5 == half)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) s_x[i * 33 + c] = xv[i];
+            wave_order();
+#pragma unroll
+            for (int k = 0; k < 32; k += 2)
+#pragma unroll
+                for (int o = 0; o < NO; ++o) acc[o] = NRF_MFMA_F32(pw[32 * o * kPitch + 32 * half + k], px[k], acc[o]);
+        }
+    }
+    if (c >= rows) return;
+    float* y = static_cast<float*>(g.out) + int64_t(mine) * g.n_out;
+#pragma unroll
+    for (int o = 0; o < NO; ++o)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int f = 32 * o + 8 * j + 4 * h;
+            f32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = acc[o][4 * j + i];
+                if (g.relu) v[i] = v[i] < 0.f ? 0.f : v[i];
+            }
+            if (f < g.n_out) store4<Fp32>(y + f, v, g.n_out - f);
+        }
+}
+
+// Backward: a workgroup takes a run of at most 256 rows of one expert, each wavefront every fourth 32 of them: dx of those rows
+// and their part of dW and db, summed over the wavefronts in LDS.  An expert of one run is written at once; the parts of
+// longer ones go to slot (first place >> 8) + expert of the workspace (no two runs share one) and are summed in their order by
+// expert_cell_sum_kernel, which also zeroes the experts without rows.
+constexpr int kCellRun = 256, kCellTable = 3;
+__host__ __device__ constexpr int64_t cell_part(int n_in, int n_out) { return int64_t(n_out) * (n_in + 1); }   // dW, then db
+template <int NI, int NO>
+__global__ __launch_bounds__(256) void expert_cell_backward_kernel(ExpertArgs g, float* dx_out) {
+    __shared__ float s_turn[4][32 * 33], s_db[4][NO * 32];
+    const PlanLayout L(g.n, g.E);
+    const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[kCellTable])[blockIdx.x];   // inside the table's room
+    if (int(blockIdx.x) >= g.plan[L.runs + 2 * kCellTable + 1]) return;
+    const int rows = tile.y >> 16, expert = tile.y & 0xffff, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
+    const int* order = g.plan + L.order + tile.x;
+    const float *x = static_cast<const float*>(g.x), *dy = static_cast<const float*>(g.g), *ys = static_cast<const float*>(g.y);
+    if (expert == g.E) {                               // rows of no expert
+        if (dx_out)
+            for (int i = threadIdx.x; i < rows * g.n_in; i += 256) dx_out[int64_t(order[i / g.n_in]) * g.n_in + i % g.n_in] = 0.f;
+        return;
+    }
+    const bool with_w = g.out != nullptr;
+    float* s_dz = s_turn[wave];
+    const float* w = static_cast<const float*>(g.w) + int64_t(expert) * g.n_out * g.n_in;
+    constexpr bool kHoldW = NI * NO <= 2;              // the weights, lanes along a row: in registers where they fit beside the rest
+    float wv[kHoldW ? 16 * NO : 1][NI] = {};           // (a feature past the last repeats it: its dz is zero, its dx not stored)
+    if (kHoldW && dx_out)
+#pragma unroll
+        for (int i = 0; i < 16 * NO; ++i)
+#pragma unroll
+            for (int b = 0; b < NI; ++b) {
+                const int f = 2 * i + h < g.n_out ? 2 * i + h : g.n_out - 1, j = 32 * b + c < g.n_in ? 32 * b + c : g.n_in - 1;
+                wv[kHoldW ? i : 0][b] = w[int64_t(f) * g.n_in + j];
+            }
+    f32x16 dw[NO][NI] = {};
+    float db[NO] = {};
+    for (int r0 = wave * 32; r0 < rows; r0 += 128) {
+        const int count = rows - r0 < 32 ? rows - r0 : 32;
+        const int mine = order[r0 + (c < count ? c : 0)];
+        // two rows per load, lanes along the row: row 2 p + h (a row past the end is the first one again, its dz and x zeroed)
+        float xv[16][NI], dz[16][NO], yv[16][NO];
+        int64_t row[16];
+#pragma unroll
+        for (int p = 0; p < 16; ++p) {
+            row[p] = __shfl(mine, 2 * p + h);
+#pragma unroll
+            for (int o = 0; o < NO; ++o) dz[p][o] = dy[row[p] * g.n_out + (32 * o + c < g.n_out ? 32 * o + c : g.n_out - 1)];
+        }
+        if (g.relu)
+#pragma unroll
+            for (int p = 0; p < 16; ++p)
+#pragma unroll
+                for (int o = 0; o < NO; ++o) yv[p][o] = ys[row[p] * g.n_out + (32 * o + c < g.n_out ? 32 * o + c : g.n_out - 1)];
+        if (with_w)
+#pragma unroll
+            for (int p = 0; p < 16; ++p)
+#pragma unroll
+                for (int b = 0; b < NI; ++b) xv[p][b] = x[row[p] * g.n_in + (32 * b + c < g.n_in ? 32 * b + c : g.n_in - 1)];
+#pragma unroll
+        for (int p = 0; p < 16; ++p) {
+            const bool there = 2 * p + h < count;
+#pragma unroll
+            for (int o = 0; o < NO; ++o) {
+                const bool keep = there && 32 * o + c < g.n_out && (!g.relu || yv[p][o] > 0.f);
+                dz[p][o] = keep ? dz[p][o] : 0.f;
+            }
+#pragma unroll
+            for (int b = 0; b < NI; ++b) xv[p][b] = there ? xv[p][b] : 0.f;
+        }
+        if (dx_out) {
+            f32x16 acc[NI] = {};
+#pragma unroll
+            for (int o = 0; o < NO; ++o) {             // dz turned through the wavefront's own piece of LDS: lanes down the rows
+                wave_order();
+#pragma unroll
+                for (int p = 0; p < 16; ++p) s_dz[(2 * p + h) * 33 + c] = dz[p][o];
+                wave_order();
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    const int f = 32 * o + k + h;
+                    const float d = s_dz[c * 33 + k + h];
+#pragma unroll
+                    for (int b = 0; b < NI; ++b) {
+                        const int j = 32 * b + c;
+                        const float wk = kHoldW ? wv[kHoldW ? 16 * o + k / 2 : 0][b] : f < g.n_out && j < g.n_in ? w[int64_t(f) * g.n_in + j] : 0.f;
+                        acc[b] = NRF_MFMA_F32(wk, d, acc[b]);
+                    }
+                }
+            }
+            if (c < count)
+#pragma unroll
+                for (int b = 0; b < NI; ++b)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int at = 32 * b + 8 * j + 4 * h;
+                        if (at < g.n_in)
+                            store4<Fp32>(dx_out + int64_t(mine) * g.n_in + at,
+                                         (f32x4){acc[b][4 * j], acc[b][4 * j + 1], acc[b][4 * j + 2], acc[b][4 * j + 3]}, g.n_in - at);
+                    }
+        }
+        if (with_w)
+#pragma unroll
+            for (int p = 0; p < 16; ++p)
+#pragma unroll
+                for (int o = 0; o < NO; ++o) {
+                    db[o] += dz[p][o];
+#pragma unroll
+                    for (int b = 0; b < NI; ++b) dw[o][b] = NRF_MFMA_F32(xv[p][b], dz[p][o], dw[o][b]);
+                }
+    }
+    if (!with_w) return;
+    const bool whole = g.plan[expert] <= kCellRun;
+    float* to_w = whole ? static_cast<float*>(g.out) + int64_t(expert) * g.n_out * g.n_in
+                        : g.partial + ((tile.x >> 8) + expert) * cell_part(g.n_in, g.n_out);
+    float* to_b = !whole ? to_w + int64_t(g.n_out) * g.n_in : g.db ? static_cast<float*>(g.db) + int64_t(expert) * g.n_out : nullptr;
+    // the wavefronts' parts of each 32 x 32 block, summed in their order.  Lane (c, h) register t: dW[32 o + c][32 b + acc_row(t, h)]
+#pragma unroll
+    for (int o = 0; o < NO; ++o) {
+        const float both = nrf_add_halves(db[o]);
+        if (h == 0) s_db[wave][32 * o + c] = both;
+#pragma unroll
+        for (int b = 0; b < NI; ++b) {
+            if (o + b) __syncthreads();
+            else wave_order();
+#pragma unroll
+            for (int t = 0; t < 16; ++t) s_dz[c * 33 + nrf::acc_row(t, h)] = dw[o][b][t];
+            __syncthreads();
+            const int j = 32 * b + (threadIdx.x & 31);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int f = 32 * o + 8 * r + (threadIdx.x >> 5), at = (f & 31) * 33 + (threadIdx.x & 31);
+                if (f < g.n_out && j < g.n_in) to_w[int64_t(f) * g.n_in + j] = ((s_turn[0][at] + s_turn[1][at]) + s_turn[2][at]) + s_turn[3][at];
+            }
+        }
+    }
+    if (to_b && int(threadIdx.x) < g.n_out) {
+        const int f = threadIdx.x;
+        to_b[f] = ((s_db[0][f] + s_db[1][f]) + s_db[2][f]) + s_db[3][f];
+    }
+}
+__global__ __launch_bounds__(256) void expert_cell_sum_kernel(ExpertArgs g) {
+    const PlanLayout L(g.n, g.E);
+    const int expert = blockIdx.x, rows = g.plan[expert];
+    if (rows > 0 && rows <= kCellRun) return;
+    const int64_t part = cell_part(g.n_in, g.n_out), weights = int64_t(g.n_out) * g.n_in;
+    const int first = g.plan[L.offsets + expert];
+    for (int i = threadIdx.x; i < part; i += 256) {
+        float v = 0.f;
+        for (int r = 0; r < rows; r += kCellRun) v += g.partial[(((first + r) >> 8) + expert) * part + i];
+        if (i < weights) static_cast<float*>(g.out)[expert * weights + i] = v;
+        else if (g.db) static_cast<float*>(g.db)[int64_t(expert) * g.n_out + i - weights] = v;
+    }
+}
+
+int launch_cell_forward(const ExpertArgs& g, hipStream_t stream) {
+    const bool i2 = g.n_in > 32, o2 = g.n_out > 32;
+    const dim3 grid(unsigned(PlanLayout::slots(g.n, g.E, kCellRowsTable)));
+    if (i2 && o2) expert_cell_forward_kernel<2, 2><<<grid, 256, 0, stream>>>(g);
+    else if (i2) expert_cell_forward_kernel<2, 1><<<grid, 256, 0, stream>>>(g);
+    else if (o2) expert_cell_forward_kernel<1, 2><<<grid, 256, 0, stream>>>(g);
+    else expert_cell_forward_kernel<1, 1><<<grid, 256, 0, stream>>>(g);
+    return NRF_OK;
+}
+template <int NI, int NO>
+int launch_cell_backward(const ExpertArgs& g, float* dx, hipStream_t stream) {
+    expert_cell_backward_kernel<NI, NO><<<dim3(unsigned(PlanLayout::slots(g.n, g.E, kCellTable))), 256, 0, stream>>>(g, dx);
+    if (g.out) expert_cell_sum_kernel<<<dim3(unsigned(g.E)), 256, 0, stream>>>(g);
+    return NRF_OK;
+}
+int launch_cell_backward(const ExpertArgs& g, float* dx, hipStream_t stream) {
+    const bool i2 = g.n_in > 32, o2 = g.n_out > 32;
+    return i2 && o2 ? launch_cell_backward<2, 2>(g, dx, stream) : i2 ? launch_cell_backward<2, 1>(g, dx, stream)
+         : o2       ? launch_cell_backward<1, 2>(g, dx, stream) : launch_cell_backward<1, 1>(g, dx, stream);
+}
+bool cells(int n_in, int n_out, int dtype) { return dtype == NRF_DTYPE_FP32 && n_in <= 64 && n_out <= 64; }
+
 // out[i] = sum over the splits, in their order
 template <class T>
 __global__ __launch_bounds__(256) void expert_reduce_kernel(const float* __restrict__ partial, int64_t count, int splits, void* out) {
@@ -552,6 +820,10 @@ NRF_EXPORT int nrf_expert_linear(const void* x, const void* weight, const void* 
                                                : launch_wide_rows<Fp16, kForward>(g, static_cast<hipStream_t>(stream));
         return st != NRF_OK ? st : nrf_launch_status();
     }
+    if (cells(n_in, n_out, dtype)) {
+        const int st = launch_cell_forward(g, static_cast<hipStream_t>(stream));
+        return st != NRF_OK ? st : nrf_launch_status();
+    }
     launch_tile<kForward>(dtype, dim3(unsigned(PlanLayout::slots(n_rows, num_experts, 1)), (n_out + kT - 1) / kT), g,
                           static_cast<hipStream_t>(stream));
     return nrf_launch_status();
@@ -567,7 +839,9 @@ struct BackwardWork {
         const int tile_splits = dw_splits(n, E, n_in, n_out, false), wide_splits = is_wide ? dw_splits(n, E, n_in, n_out, true) : 1;
         splits = tile_splits > wide_splits ? tile_splits : wide_splits;   // either kernel may run: alignment is known at the call
         dz = is_wide ? (n * n_out * 2 + 255) & ~int64_t(255) : 0;
-        partial = splits > 1 ? int64_t(splits) * E * n_out * (n_in + 1) * 4 : 0;
+        partial = cells(n_in, n_out, dtype) ? PlanLayout::slots(n, E, kCellTable) * cell_part(n_in, n_out) * 4
+                  : splits > 1              ? int64_t(splits) * E * n_out * (n_in + 1) * 4
+                                            : 0;
     }
 };
 }  // namespace
@@ -602,6 +876,11 @@ NRF_EXPORT int nrf_expert_linear_backward(const void* grad_y, const void* x, con
     const int tiles_in = (n_in + kT - 1) / kT, tiles_out = (n_out + kT - 1) / kT;
     int st = NRF_OK;
     nrf_launch_begin();
+    if (cells(n_in, n_out, dtype) && n_rows > 0) {
+        g.out = grad_weight, g.db = grad_bias;
+        st = launch_cell_backward(g, static_cast<float*>(grad_x), stream);
+        return st != NRF_OK ? st : nrf_launch_status();
+    }
     if (is_wide && g.relu) {
         const int64_t octets = n_rows * n_out / 8, blocks = (octets + 255) / 256;
         const dim3 grid(unsigned(blocks < 8192 ? blocks : 8192));
