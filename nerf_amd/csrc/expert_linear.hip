@@ -36,14 +36,18 @@ typedef float f32x4_u4 __attribute__((ext_vector_type(4), aligned(4)));
 template <class T> struct Oct;
 template <> struct Oct<Fp32> {
     f32x4 lo, hi;
-    __device__ __forceinline__ void zero() { lo = hi = (f32x4){0.f, 0.f, 0.f, 0.f}; }
-    __device__ __forceinline__ void load(const float* p, int valid) {
-        if (valid >= 8) {
+    // the eight elements from p on, those before `end` (the tensor's) at least
+    __device__ __forceinline__ void load(const float* p, const float* end) {
+        if (p + 8 <= end) {
             lo = *reinterpret_cast<const f32x4_u4*>(p), hi = *reinterpret_cast<const f32x4_u4*>(p + 4);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) lo[j] = j < valid ? p[j] : 0.f, hi[j] = 4 + j < valid ? p[4 + j] : 0.f;
+            for (int j = 0; j < 4; ++j) lo[j] = p + j < end ? p[j] : 0.f, hi[j] = p + 4 + j < end ? p[4 + j] : 0.f;
         }
+    }
+    __device__ __forceinline__ void limit(int valid) {   // zeros from element `valid` on
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lo[j] = j < valid ? lo[j] : 0.f, hi[j] = 4 + j < valid ? hi[j] : 0.f;
     }
     __device__ __forceinline__ void keep_positive(const Oct& y) {
 #pragma unroll
@@ -62,15 +66,18 @@ template <> struct Oct<Fp32> {
 };
 template <class T, unsigned INF> struct Oct16 {
     u32x4 v;
-    __device__ __forceinline__ void zero() { v = (u32x4){0, 0, 0, 0}; }
-    __device__ __forceinline__ void load(const unsigned short* p, int valid) {
-        if (valid >= 8) {
+    __device__ __forceinline__ void load(const unsigned short* p, const unsigned short* end) {
+        if (p + 8 <= end) {
             v = *reinterpret_cast<const u32x4_u2*>(p);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                v[j] = (2 * j < valid ? unsigned(p[2 * j]) : 0u) | (2 * j + 1 < valid ? unsigned(p[2 * j + 1]) << 16 : 0u);
+                v[j] = (p + 2 * j < end ? unsigned(p[2 * j]) : 0u) | (p + 2 * j + 1 < end ? unsigned(p[2 * j + 1]) << 16 : 0u);
         }
+    }
+    __device__ __forceinline__ void limit(int valid) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] &= (2 * j < valid ? 0xffffu : 0u) | (2 * j + 1 < valid ? 0xffff0000u : 0u);
     }
     __device__ __forceinline__ void keep_positive(const Oct16& y) {   // positive: bits in 1 .. INF (NaN lies above)
 #pragma unroll
@@ -125,48 +132,83 @@ __device__ __forceinline__ void store4(typename Traits<T>::elem* p, const f32x4&
     }
 }
 
+// dW and db in parts (fp32, db behind dW): either of runs of at most kPartRows rows -- part (first place >> 8) + expert, no two
+// runs share one; experts of a single run are written at once -- or `splits` equal shares of every expert's rows, part
+// share * E + expert.  expert_sum_kernel adds an expert's parts in their order.
+constexpr int kPartRows = 256, kPartTable = 3;
+__host__ __device__ constexpr int64_t part_size(int n_in, int n_out) { return int64_t(n_out) * (n_in + 1); }
+
 struct ExpertArgs {
     const void *x, *w, *bias, *y, *g;     // y: the saved outputs whose sign is the relu's mask, or NULL
     const int* plan;
     void *out, *db;                       // the product's output; db: dW only, may be NULL
-    float* partial;                       // dW split over the rows: fp32 sums, reduced by a second kernel
+    float* partial;                       // dW's parts
     int64_t n;
-    int E, n_in, n_out, relu, splits;
+    int E, n_in, n_out, relu, splits;     // splits: 0 for parts by runs
 };
 
-// The general tile: 64 x 64 outputs, k in steps of 32, four wavefronts of 32 x 32 each, the next step's loads in registers
-// while this step is multiplied.  Any size, any alignment.
-constexpr int kT = 64, kK = 32, kPitch = kK + 8;   // LDS row pitch: 80 B, so that 16 rows' 16 B reads spread over the banks
+// four consecutive outputs of a product, after bias and relu
+template <class T>
+__device__ __forceinline__ void finish_row(typename Traits<T>::elem* out, f32x4 v, int valid, const typename Traits<T>::elem* bias, int relu) {
+    if (bias)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < valid) v[j] += to_float(bias[j], T{});
+    if (relu)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];   // NaN stays
+    store4<T>(out, v, valid);
+}
 
-template <class T, int FORM>
+// The general tile: TT x TT outputs (64 or 128), k in steps of 32, four wavefronts of a quarter each, the next step's loads in
+// registers while this step is multiplied.  Any size, any alignment.  The larger tile splits fp32 operands half as often per
+// product (splitting 32 elements per thread and step takes about half as long as the step's 96 MFMAs; at 64 x 64 as long as its
+// 24); the smaller one fills the chip with small problems.
+constexpr int kK = 32, kPitch = kK + 8;   // LDS row pitch: 80 B, so that 16 rows' 16 B reads spread over the banks
+
+template <class T, int FORM, int TT>
 __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
     typedef typename Traits<T>::elem elem;
-    constexpr int P = Traits<T>::planes;
-    __shared__ __align__(16) unsigned short s_a[P][kT][kPitch], s_b[P][kT][kPitch];
-    __shared__ int s_rows[kT];            // forward / dx: the tile's batch rows
+    constexpr int P = Traits<T>::planes, kTable = TT == 64 ? 1 : 2, N = TT / 64, M = TT / 32;   // octets per thread, 16-row blocks per wave
+    constexpr bool a_cols = FORM != kForward, b_cols = FORM == kDw;
+    typedef DmaSide<kCols, TT, kK, 1, 4> Cols;
+    __shared__ __align__(16) unsigned short s_a[P][TT * (a_cols ? kK : kPitch)], s_b[P][TT * (b_cols ? kK : kPitch)];
+    __shared__ int s_rows[TT];            // forward / dx: the tile's batch rows
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, q = lane >> 4;
-    const int wa = (wave & 1) * 32, wb = (wave >> 1) * 32;
-    const int a0 = blockIdx.y * kT;       // first A row = first output column
+    const int wa = (wave & 1) * (TT / 2), wb = (wave >> 1) * (TT / 2);
+    const int a0 = blockIdx.y * TT;       // first A row = first output column
     const PlanLayout L(g.n, g.E);
     const int* order = g.plan + L.order;
 
     int expert, b0 = 0, b_count, k_begin = 0, k_end;
     const int n_a = FORM == kForward ? g.n_out : g.n_in;
+    int64_t part = 0;                     // dW in parts: which
+    bool in_parts = false;
     if (FORM == kDw) {
-        expert = blockIdx.x / g.splits;
-        const int split = blockIdx.x % g.splits;
-        const int first = g.plan[L.offsets + expert], rows = g.plan[expert];
-        const int per = (((rows + g.splits - 1) / g.splits) + kK - 1) / kK * kK;   // whole k steps
-        k_begin = first + (split * per < rows ? split * per : rows);
-        k_end = first + (split * per + per < rows ? split * per + per : rows);
-        b0 = blockIdx.z * kT;
-        b_count = g.n_out - b0 < kT ? g.n_out - b0 : kT;
+        if (g.splits == 0) {              // a run of at most kPartRows rows
+            const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[kPartTable])[blockIdx.x];   // inside the table's room
+            if (int(blockIdx.x) >= g.plan[L.runs + 2 * kPartTable + 1]) return;
+            expert = tile.y & 0xffff;
+            if (expert == g.E) return;
+            k_begin = tile.x, k_end = tile.x + (tile.y >> 16);
+            part = (tile.x >> 8) + expert, in_parts = g.plan[expert] > kPartRows;
+        } else {
+            expert = blockIdx.x / g.splits;
+            const int split = blockIdx.x % g.splits;
+            const int first = g.plan[L.offsets + expert], rows = g.plan[expert];
+            const int per = (((rows + g.splits - 1) / g.splits) + kK - 1) / kK * kK;   // whole k steps
+            k_begin = first + (split * per < rows ? split * per : rows);
+            k_end = first + (split * per + per < rows ? split * per + per : rows);
+            part = int64_t(split) * g.E + expert, in_parts = g.splits > 1;
+        }
+        b0 = blockIdx.z * TT;
+        b_count = g.n_out - b0 < TT ? g.n_out - b0 : TT;
     } else {
-        if (int(blockIdx.x) >= g.plan[L.runs + 2 * 1 + 1]) return;
-        const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[1])[blockIdx.x];
+        const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[kTable])[blockIdx.x];   // inside the table's room
+        if (int(blockIdx.x) >= g.plan[L.runs + 2 * kTable + 1]) return;
         b_count = tile.y >> 16;
         expert = tile.y & 0xffff;
-        if (t < kT) s_rows[t] = t < b_count ? order[tile.x + t] : -1;
+        if (t < TT) s_rows[t] = t < b_count ? order[tile.x + t] : -1;
         __syncthreads();
         k_end = FORM == kForward ? g.n_in : g.n_out;
     }
@@ -178,87 +220,96 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
     const elem* ys = static_cast<const elem*>(g.y);
     const SplitSel sel = SplitSel::make();
 
-    // This thread's eight elements of a step: along k for an operand whose k is contiguous, along the tile's rows otherwise.
-    const int kr = t >> 2, kc = (t & 3) * 8;          // [64 rows][4 octets of k]
-    const int ck = t >> 3, cr = (t & 7) * 8;          // [32 k][8 octets of rows]
-    constexpr bool a_cols = FORM != kForward, b_cols = FORM == kDw;
-    const int my_row = FORM == kDw ? 0 : s_rows[kr];
-
-    auto load_a = [&](Oct<T>& v, int k0) {
-        v.zero();
-        if (!a_cols) {
-            if (a0 + kr < n_a && k0 + kc < k_end) v.load(w + int64_t(a0 + kr) * g.n_in + k0 + kc, k_end - k0 - kc);
-        } else if (k0 + ck < k_end && a0 + cr < n_a) {
-            if (FORM == kDx) v.load(w + int64_t(k0 + ck) * g.n_in + a0 + cr, n_a - a0 - cr);
-            else v.load(x + int64_t(order[k0 + ck]) * g.n_in + a0 + cr, n_a - a0 - cr);
-        }
+    // This thread's eight elements of a step, N times: along k for an operand whose k is contiguous, along the tile's rows
+    // otherwise.  Rows past the operand's last one read a row that is there (their outputs are not stored), octets may run on
+    // into the next row, and what lies past the end of k is zeroed on its way into LDS: no load stands under a condition but
+    // at the very end of a tensor.
+    const elem *w_end = w + int64_t(g.n_out) * g.n_in, *x_end = x + g.n * g.n_in, *dy_end = dy + g.n * g.n_out, *ys_end = ys + g.n * g.n_out;
+    int kr[N], ck[N], cr[N], my_row[N], k_row[N];
+    const int kc = (t & 3) * 8;                       // [TT rows][4 octets of k]
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        kr[i] = (t >> 2) + 64 * i;
+        ck[i] = (t + 256 * i) / (TT / 8), cr[i] = (t + 256 * i) % (TT / 8) * 8;   // [32 k][TT / 8 octets of rows]
+        my_row[i] = FORM == kDw ? 0 : s_rows[kr[i]] < 0 ? s_rows[0] : s_rows[kr[i]];
+        k_row[i] = 0;
+    }
+    // dW: the batch rows of a step, looked up a step before its loads
+    auto look_up = [&](int k0) {
+        if (FORM == kDw)
+#pragma unroll
+            for (int i = 0; i < N; ++i) k_row[i] = order[k0 + ck[i] < k_end ? k0 + ck[i] : k_end - 1];
     };
-    auto load_b = [&](Oct<T>& v, int k0) {
-        v.zero();
-        int64_t at = 0;
-        int valid = 0;
+    auto load_a = [&](Oct<T>& v, int i, int k0) {
+        const int col = a0 + cr[i] < n_a ? a0 + cr[i] : 0;
+        if (FORM == kForward) v.load(w + int64_t(a0 + kr[i] < n_a ? a0 + kr[i] : n_a - 1) * g.n_in + (k0 + kc < k_end ? k0 + kc : 0), w_end);
+        else if (FORM == kDx) v.load(w + int64_t(k0 + ck[i] < k_end ? k0 + ck[i] : 0) * g.n_in + col, w_end);
+        else v.load(x + int64_t(k_row[i]) * g.n_in + col, x_end);
+    };
+    auto load_b = [&](Oct<T>& v, Oct<T>& s, int i, int k0) {
         if (FORM == kForward) {
-            if (my_row >= 0 && k0 + kc < k_end) v.load(x + int64_t(my_row) * g.n_in + k0 + kc, k_end - k0 - kc);
+            v.load(x + int64_t(my_row[i]) * g.n_in + (k0 + kc < k_end ? k0 + kc : 0), x_end);
             return;
         }
-        if (FORM == kDx) {
-            if (my_row >= 0 && k0 + kc < k_end) at = int64_t(my_row) * g.n_out + k0 + kc, valid = k_end - k0 - kc;
-        } else if (k0 + ck < k_end && cr < b_count) {
-            at = int64_t(order[k0 + ck]) * g.n_out + b0 + cr, valid = b_count - cr;
-        }
-        if (valid > 0) {
-            v.load(dy + at, valid);
-            if (g.relu) {
-                Oct<T> s;
-                s.load(ys + at, valid);
-                v.keep_positive(s);
-            }
-        }
+        const int64_t at = FORM == kDx ? int64_t(my_row[i]) * g.n_out + (k0 + kc < k_end ? k0 + kc : 0)
+                                       : int64_t(k_row[i]) * g.n_out + (cr[i] < b_count ? b0 + cr[i] : 0);
+        v.load(dy + at, dy_end);
+        if (g.relu) s.load(ys + at, ys_end);
     };
-    auto stage = [&](unsigned short (&s)[P][kT][kPitch], const Oct<T>& v, bool cols) {
+    // LDS holds [row][k] (pitch kPitch) of an operand whose k is contiguous, [k][row] of the others, read back transposed
+    auto stage = [&](unsigned short* s, int plane, Oct<T> v, int i, int k0, bool cols) {
+        if (k0 + kK > k_end) v.limit(cols ? (k0 + ck[i] < k_end ? 8 : 0) : k_end - k0 - kc);
         u32x4 p[P];
         v.terms(sel, p);
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            if (!cols) {
-                *reinterpret_cast<u32x4*>(&s[i][kr][kc]) = p[i];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[i][cr + 2 * j][ck] = (unsigned short)p[i][j];
-                    s[i][cr + 2 * j + 1][ck] = (unsigned short)(p[i][j] >> 16);
-                }
-            }
-        }
+        for (int j = 0; j < P; ++j)
+            *reinterpret_cast<u32x4*>(s + j * plane + (cols ? ck[i] * TT + ((cr[i] / 8) ^ Cols::swizzle(ck[i])) * 8 : kr[i] * kPitch + kc)) = p[j];
+    };
+    auto fragment = [&](const unsigned short* s, int first, int m, bool cols) {
+        return cols ? __builtin_bit_cast(u32x4, Cols::frag(reinterpret_cast<const char*>(s), first, m, 0, c, q))
+                    : *reinterpret_cast<const u32x4*>(&s[(first + 16 * m + c) * kPitch + 8 * q]);
     };
 
-    f32x4 acc[2][2] = {};
-    f32x4 sum[2] = {};                                // dW: db of this wavefront's 32 outputs
+    f32x4 acc[M][M] = {};
+    f32x4 sum[M] = {};                                // dW: db of this wavefront's outputs
     const bool with_db = FORM == kDw && g.db && blockIdx.y == 0 && wa == 0;
     const unsigned one = __is_same(T, Fp16) ? 0x3c003c00u : 0x3f803f80u;
     const u32x4 ones = {one, one, one, one};
     if (!none && k_begin < k_end) {
-        Oct<T> ra, rb;
-        load_a(ra, k_begin), load_b(rb, k_begin);
+        Oct<T> ra[N], rb[N], rs[N];
+        look_up(k_begin);
+#pragma unroll
+        for (int i = 0; i < N; ++i) load_a(ra[i], i, k_begin), load_b(rb[i], rs[i], i, k_begin);
+        look_up(k_begin + kK);
         for (int k0 = k_begin; k0 < k_end; k0 += kK) {
-            stage(s_a, ra, a_cols), stage(s_b, rb, b_cols);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                stage(s_a[0], sizeof(s_a[0]) / 2, ra[i], i, k0, a_cols);
+                if (FORM != kForward && g.relu) rb[i].keep_positive(rs[i]);
+                stage(s_b[0], sizeof(s_b[0]) / 2, rb[i], i, k0, b_cols);
+            }
             __syncthreads();
-            if (k0 + kK < k_end) load_a(ra, k0 + kK), load_b(rb, k0 + kK);
-            u32x4 fa[2][P], fb[2][P];
+            if (k0 + kK < k_end) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+                for (int i = 0; i < N; ++i) load_a(ra[i], i, k0 + kK), load_b(rb[i], rs[i], i, k0 + kK);
+                look_up(k0 + 2 * kK);
+            }
+            u32x4 fb[M][P];
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    fa[m][i] = *reinterpret_cast<const u32x4*>(&s_a[i][wa + 16 * m + c][8 * q]);
-                    fb[m][i] = *reinterpret_cast<const u32x4*>(&s_b[i][wb + 16 * m + c][8 * q]);
-                }
+            for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int ma = 0; ma < 2; ++ma)
+                for (int i = 0; i < P; ++i) fb[m][i] = fragment(s_b[i], wb, m, b_cols);
 #pragma unroll
-                for (int mb = 0; mb < 2; ++mb) acc[ma][mb] = mfma_terms<T>(fa[ma], fb[mb], acc[ma][mb]);
+            for (int ma = 0; ma < M; ++ma) {
+                u32x4 fa[P];
+#pragma unroll
+                for (int i = 0; i < P; ++i) fa[i] = fragment(s_a[i], wa, ma, a_cols);
+#pragma unroll
+                for (int mb = 0; mb < M; ++mb) acc[ma][mb] = mfma_terms<T>(fa, fb[mb], acc[ma][mb]);
+            }
             if (with_db)
 #pragma unroll
-                for (int mb = 0; mb < 2; ++mb)
+                for (int mb = 0; mb < M; ++mb)
 #pragma unroll
                     for (int i = P - 1; i >= 0; --i) sum[mb] = mfma16<T>(ones, fb[mb][i], sum[mb]);
             __syncthreads();
@@ -267,39 +318,26 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
 
     // lane (c, q) holds outputs a0 + wa + 16 ma + 4 q .. + 3 of b row wb + 16 mb + c
 #pragma unroll
-    for (int mb = 0; mb < 2; ++mb) {
+    for (int mb = 0; mb < M; ++mb) {
         const int br = wb + 16 * mb + c;
         if (br >= b_count) continue;
 #pragma unroll
-        for (int ma = 0; ma < 2; ++ma) {
+        for (int ma = 0; ma < M; ++ma) {
             const int a = a0 + wa + 16 * ma + 4 * q, valid = n_a - a;
             if (valid <= 0) continue;
-            f32x4 v = acc[ma][mb];
-            if (FORM == kForward) {
-                if (g.bias && !none) {
-                    const elem* b = static_cast<const elem*>(g.bias) + int64_t(expert) * g.n_out + a;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (j < valid) v[j] += to_float(b[j], T{});
-                }
-                if (g.relu)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];   // NaN stays
-            }
             if (FORM == kDw) {
-                const int64_t at = (int64_t(expert) * g.n_out + b0 + br) * g.n_in + a;
-                if (g.splits > 1) store4<Fp32>(g.partial + int64_t(blockIdx.x % g.splits) * g.E * g.n_out * g.n_in + at, v, valid);
-                else store4<T>(static_cast<elem*>(g.out) + at, v, valid);
+                const int64_t at = int64_t(b0 + br) * g.n_in + a, size = int64_t(g.n_out) * g.n_in;
+                if (in_parts) store4<Fp32>(g.partial + part * (size + g.n_out) + at, acc[ma][mb], valid);
+                else store4<T>(static_cast<elem*>(g.out) + expert * size + at, acc[ma][mb], valid);
             } else {
-                store4<T>(static_cast<elem*>(g.out) + int64_t(s_rows[br]) * n_a + a, v, valid);
+                const elem* bias = FORM == kForward && g.bias && !none ? static_cast<const elem*>(g.bias) + int64_t(expert) * g.n_out + a : nullptr;
+                finish_row<T>(static_cast<elem*>(g.out) + int64_t(s_rows[br]) * n_a + a, acc[ma][mb], valid, bias, FORM == kForward ? g.relu : 0);
             }
         }
         if (with_db && q == 0) {
-            const int64_t at = int64_t(expert) * g.n_out + b0 + br;
-            if (g.splits > 1)
-                g.partial[int64_t(g.splits) * g.E * g.n_out * g.n_in + int64_t(blockIdx.x % g.splits) * g.E * g.n_out + at] = sum[mb][0];
-            else
-                static_cast<elem*>(g.db)[at] = from_float(sum[mb][0], T{});
+            const int64_t size = int64_t(g.n_out) * g.n_in;
+            if (in_parts) g.partial[part * (size + g.n_out) + size + b0 + br] = sum[mb][0];
+            else static_cast<elem*>(g.db)[int64_t(expert) * g.n_out + b0 + br] = from_float(sum[mb][0], T{});
         }
     }
 }
@@ -317,37 +355,25 @@ __device__ __forceinline__ int xcd_run(const int* runs, int xcd, int local) {
 }
 __host__ __device__ constexpr int64_t xcd_blocks(int64_t slots, int a_tiles) { return (slots / 8 + 2) * 8 * a_tiles; }
 
-// four consecutive outputs of a product, after bias and relu
-template <class T>
-__device__ __forceinline__ void finish_row(typename Traits<T>::elem* out, f32x4 v, int valid, const typename Traits<T>::elem* bias, int relu) {
-    if (bias)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < valid) v[j] += to_float(bias[j], T{});
-    if (relu)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];   // NaN stays
-    store4<T>(out, v, valid);
-}
-
-// Forward and dx: 256 output columns x 256 batch rows, eight wavefronts of 128 x 64 (12 KiB of LDS reads to 32 MFMAs), two
-// steps of 64 k in LDS (128 KiB).  dx reads the weights' columns (DmaGemm: kCols); g.g holds dz.
-template <class T, int FORM> struct WideRows {
-    static constexpr int kA = 256, kB = 256, kTable = 3;
-    typedef DmaGemm<__is_same(T, Bf16), FORM == kForward ? kRows : kCols, kRows, kA, kB, 2, 4, 1, 64, 2> Gemm;
+// Forward and dx: 256 output columns by a run of batch rows, eight wavefronts.  Runs of more than 128 rows: 256 x 256, 128 x 64
+// per wavefront (12 KiB of LDS reads to 32 MFMAs), two steps of 64 k in LDS (128 KiB).  Shorter runs wait for data, not for the
+// matrix cores: 256 x 128 with three steps in LDS, 256 x 64 with four, so that more of the weights is on its way (a run of 64
+// rows through the 256 x 256 form takes three quarters of a whole run's time).  dx reads the weights' columns (DmaGemm: kCols),
+// whose transposing reads need registers that the 256 x 256 form has not left: its runs are of 128 rows; so are the forward's
+// where 256 would leave the chip less than two workgroups per CU (dx of 16 k rows, 16 experts, 1536 -> 1024: 92 us, 116 in runs
+// of 256).  g.g holds dz.
+constexpr int kWideA = 256;
+template <class T, int FORM, int ROWS> struct WideRows {
+    static constexpr int kWA = ROWS == 256 ? 2 : 4, kST = ROWS == 256 ? 2 : ROWS == 128 ? 3 : 4;
+    typedef DmaGemm<__is_same(T, Bf16), FORM == kForward ? kRows : kCols, kRows, kWideA, ROWS, kWA, 8 / kWA, 1, 64, kST, kST> Gemm;
 };
-template <class T, int FORM>
-__global__ __launch_bounds__(512) void expert_wide_rows_kernel(ExpertArgs g, int a_tiles) {
-    typedef WideRows<T, FORM> W;
-    typedef typename W::Gemm Gemm;
+constexpr int kWideLds = 4 * (256 + 64) * 128;   // of the 256 x 64 form, the largest
+
+template <class T, int FORM, int ROWS>
+__device__ __forceinline__ void wide_rows_tile(const ExpertArgs& g, char* smem, int a0, int b_count, int expert, const int* order) {
+    typedef typename WideRows<T, FORM, ROWS>::Gemm Gemm;
     typedef unsigned short elem;
-    extern __shared__ __align__(16) char smem[];
-    const PlanLayout L(g.n, g.E);
-    const int local = blockIdx.x / 8, at = xcd_run(g.plan + L.runs + 2 * W::kTable, blockIdx.x % 8, local / a_tiles);
-    if (at < 0) return;
-    const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[W::kTable])[at];
-    const int b_count = tile.y >> 16, expert = tile.y & 0xffff, a0 = local % a_tiles * W::kA;
-    const int* order = g.plan + L.order + tile.x;
+    static_assert(Gemm::kLds <= kWideLds && Gemm::kThreads == 512, "one launch for all forms");
     const bool none = expert == g.E;
     const int n_a = FORM == kForward ? g.n_out : g.n_in, n_k = FORM == kForward ? g.n_in : g.n_out;
     const elem* w = static_cast<const elem*>(g.w) + int64_t(none ? 0 : expert) * g.n_out * g.n_in;
@@ -380,15 +406,26 @@ __global__ __launch_bounds__(512) void expert_wide_rows_kernel(ExpertArgs g, int
         }
     }
 }
+template <class T, int FORM, int ROWS>   // runs of at most ROWS rows
+__global__ __launch_bounds__(512) void expert_wide_rows_kernel(ExpertArgs g, int a_tiles) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr int table = ROWS == 256 ? 3 : 2;
+    const PlanLayout L(g.n, g.E);
+    const int local = blockIdx.x / 8, at = xcd_run(g.plan + L.runs + 2 * table, blockIdx.x % 8, local / a_tiles);
+    if (at < 0) return;
+    const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[table])[at];
+    const int b_count = tile.y >> 16, expert = tile.y & 0xffff, a0 = local % a_tiles * kWideA;
+    const int* order = g.plan + L.order + tile.x;
+    if (ROWS == 256 && b_count > 128) wide_rows_tile<T, FORM, ROWS>(g, smem, a0, b_count, expert, order);
+    else if (b_count > 64) wide_rows_tile<T, FORM, 128>(g, smem, a0, b_count, expert, order);
+    else wide_rows_tile<T, FORM, 64>(g, smem, a0, b_count, expert, order);
+}
 
-// dW: 256 input columns x DWB output columns, k the expert's rows through the list of them in LDS, kListRows at a time.
-#ifndef DWB
-#define DWB 128
-#endif
+// dW: 256 input columns x 128 output columns, k the expert's rows through the list of them in LDS, kListRows at a time.
 constexpr int kListRows = 4096;
 template <class T> struct WideDw {
-    static constexpr int kA = 256, kB = DWB;
-    typedef DmaGemm<__is_same(T, Bf16), kGather, kGather, kA, kB, DWB == 256 ? 2 : 4, DWB == 256 ? 4 : 2, 1, 64, 2, true> Gemm;
+    static constexpr int kA = 256, kB = 128;
+    typedef DmaGemm<__is_same(T, Bf16), kGather, kGather, kA, kB, 4, 2, 1, 64, 2, 2, true> Gemm;
     static constexpr int kLds = Gemm::kLds + kListRows * 4;
 };
 template <class T>
@@ -399,10 +436,19 @@ __global__ __launch_bounds__(512) void expert_wide_dw_kernel(ExpertArgs g, int a
     extern __shared__ __align__(16) char smem[];
     int* s_list = reinterpret_cast<int*>(smem + Gemm::kLds);
     const PlanLayout L(g.n, g.E);
-    // an expert's tiles stay on one XCD, which keeps the expert's rows in its L2
-    const int tiles = a_tiles * b_tiles * g.splits, local = blockIdx.x / 8, expert = local / tiles * 8 + blockIdx.x % 8;
+    // Every XCD takes a contiguous eighth of each expert's tiles (whole experts per XCD leave the XCD of the two most popular
+    // of sixteen with twice the average: 172 us where this takes 99); fewer than eight go round.
+    const int tiles = a_tiles * b_tiles * g.splits, local = blockIdx.x / 8, xcd = blockIdx.x % 8;
+    int expert, at;
+    if (tiles >= 8) {
+        const int per = (tiles + 7) / 8;
+        expert = local / per, at = tiles * xcd / 8 + local % per;
+        if (at >= tiles * (xcd + 1) / 8) return;
+    } else {
+        expert = (local * 8 + xcd) / tiles, at = (local * 8 + xcd) % tiles;
+    }
     if (expert >= g.E) return;
-    const int split = local % tiles / (a_tiles * b_tiles), tile = local % (a_tiles * b_tiles);
+    const int split = at / (a_tiles * b_tiles), tile = at % (a_tiles * b_tiles);
     const int a0 = tile % a_tiles * W::kA, b0 = tile / a_tiles * W::kB;
     const int rows = g.plan[expert], per = ((rows + g.splits - 1) / g.splits + 63) / 64 * 64;
     const int begin = split * per < rows ? split * per : rows, end = begin + per < rows ? begin + per : rows;
@@ -422,22 +468,23 @@ __global__ __launch_bounds__(512) void expert_wide_dw_kernel(ExpertArgs g, int a
         gemm.run(smem, count, acc, s_list, &sum, with_db);
     }
     const int c = gemm.lane & 15, q = gemm.lane >> 4;
-    const int64_t weights = int64_t(g.E) * g.n_out * g.n_in;
+    const int64_t size = int64_t(g.n_out) * g.n_in;
+    float* part = g.partial + (int64_t(split) * g.E + expert) * part_size(g.n_in, g.n_out);
 #pragma unroll
     for (int mb = 0; mb < Gemm::kMB; ++mb) {
         const int br = b0 + gemm.wave_b() + 16 * mb + c;
         if (br >= g.n_out) continue;
-        const int64_t row = int64_t(expert) * g.n_out + br;
 #pragma unroll
         for (int ma = 0; ma < Gemm::kMA; ++ma) {
             const int a = a0 + gemm.wave_a() + 16 * ma + 4 * q, valid = g.n_in - a;
             if (valid <= 0) continue;
-            if (g.splits > 1) store4<Fp32>(g.partial + split * weights + row * g.n_in + a, acc[ma][mb], valid);
-            else store4<T>(static_cast<elem*>(g.out) + row * g.n_in + a, acc[ma][mb], valid);
+            const int64_t at = int64_t(br) * g.n_in + a;
+            if (g.splits > 1) store4<Fp32>(part + at, acc[ma][mb], valid);
+            else store4<T>(static_cast<elem*>(g.out) + expert * size + at, acc[ma][mb], valid);
         }
         if (with_db && q == 0) {
-            if (g.splits > 1) g.partial[g.splits * weights + split * int64_t(g.E) * g.n_out + row] = sum[mb][0];
-            else static_cast<elem*>(g.db)[row] = from_float(sum[mb][0], T{});
+            if (g.splits > 1) part[size + br] = sum[mb][0];
+            else static_cast<elem*>(g.db)[int64_t(expert) * g.n_out + br] = from_float(sum[mb][0], T{});
         }
     }
 }
@@ -458,15 +505,20 @@ int allow_lds(const void* kernel, int bytes) {
     return bytes <= 65536 || hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? NRF_OK : NRF_ERR_LAUNCH;
 }
 
-template <class T, int FORM>
+template <class T, int FORM, int ROWS>
 int launch_wide_rows(const ExpertArgs& g, hipStream_t stream) {
-    typedef WideRows<T, FORM> W;
-    const int a_tiles = ((FORM == kForward ? g.n_out : g.n_in) + W::kA - 1) / W::kA;
-    auto kernel = &expert_wide_rows_kernel<T, FORM>;
-    const int st = allow_lds(reinterpret_cast<const void*>(kernel), W::Gemm::kLds);
+    const int a_tiles = ((FORM == kForward ? g.n_out : g.n_in) + kWideA - 1) / kWideA;
+    auto kernel = &expert_wide_rows_kernel<T, FORM, ROWS>;
+    const int st = allow_lds(reinterpret_cast<const void*>(kernel), kWideLds);
     if (st != NRF_OK) return st;
-    kernel<<<dim3(unsigned(xcd_blocks(PlanLayout::slots(g.n, g.E, W::kTable), a_tiles))), 512, W::Gemm::kLds, stream>>>(g, a_tiles);
+    const int64_t blocks = xcd_blocks(PlanLayout::slots(g.n, g.E, ROWS == 256 ? 3 : 2), a_tiles);
+    kernel<<<dim3(unsigned(blocks)), 512, kWideLds, stream>>>(g, a_tiles);
     return NRF_OK;
+}
+template <class T>
+int launch_wide_forward(const ExpertArgs& g, hipStream_t stream) {
+    const int64_t tiles = (g.n / 256 + (g.E < g.n ? g.E : g.n) / 2) * ((g.n_out + kWideA - 1) / kWideA);
+    return tiles < 512 ? launch_wide_rows<T, kForward, 128>(g, stream) : launch_wide_rows<T, kForward, 256>(g, stream);
 }
 template <class T>
 int launch_wide_dw(const ExpertArgs& g, hipStream_t stream) {
@@ -475,14 +527,16 @@ int launch_wide_dw(const ExpertArgs& g, hipStream_t stream) {
     auto kernel = &expert_wide_dw_kernel<T>;
     const int st = allow_lds(reinterpret_cast<const void*>(kernel), W::kLds);
     if (st != NRF_OK) return st;
-    kernel<<<dim3(unsigned((g.E + 7) / 8 * 8) * unsigned(a_tiles * b_tiles * g.splits)), 512, W::kLds, stream>>>(g, a_tiles, b_tiles);
+    const int64_t tiles = int64_t(a_tiles) * b_tiles * g.splits, blocks = tiles >= 8 ? g.E * ((tiles + 7) / 8) * 8 : (g.E * tiles + 7) / 8 * 8;
+    kernel<<<dim3(unsigned(blocks)), 512, W::kLds, stream>>>(g, a_tiles, b_tiles);
     return NRF_OK;
 }
 
-// Whether the wide kernels take a product: octets that do not straddle rows, operands under 4 GiB, at least half a tile's
-// rows per expert and half a tile's columns.
+// Whether the wide kernels take a product: octets that do not straddle rows, operands under 4 GiB and at least half a tile's
+// columns.  Any number of rows: single tokens through 32 experts of 1024 -> 2048 take 17 us (7.3 TB/s of weights), the general
+// tile 25.
 bool wide(int64_t n, int E, int n_in, int n_out, int dtype) {
-    return dtype != NRF_DTYPE_FP32 && n_in % 8 == 0 && n_out % 8 == 0 && n_in >= 128 && n_out >= 128 && n / E >= 64 &&
+    return dtype != NRF_DTYPE_FP32 && n_in % 8 == 0 && n_out % 8 == 0 && n_in >= 128 && n_out >= 128 &&
            n * (n_in > n_out ? n_in : n_out) < int64_t(1) << 31 && int64_t(n_out) * n_in < int64_t(1) << 31;
 }
 
@@ -580,17 +634,13 @@ __global__ __launch_bounds__(256) void expert_cell_forward_kernel(ExpertArgs g) 
 }
 
 // Backward: a workgroup takes a run of at most 256 rows of one expert, each wavefront every fourth 32 of them: dx of those rows
-// and their part of dW and db, summed over the wavefronts in LDS.  An expert of one run is written at once; the parts of
-// longer ones go to slot (first place >> 8) + expert of the workspace (no two runs share one) and are summed in their order by
-// expert_cell_sum_kernel, which also zeroes the experts without rows.
-constexpr int kCellRun = 256, kCellTable = 3;
-__host__ __device__ constexpr int64_t cell_part(int n_in, int n_out) { return int64_t(n_out) * (n_in + 1); }   // dW, then db
+// and their part of dW and db, summed over the wavefronts in LDS (parts by runs: see ExpertArgs).
 template <int NI, int NO>
 __global__ __launch_bounds__(256) void expert_cell_backward_kernel(ExpertArgs g, float* dx_out) {
     __shared__ float s_turn[4][32 * 33], s_db[4][NO * 32];
     const PlanLayout L(g.n, g.E);
-    const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[kCellTable])[blockIdx.x];   // inside the table's room
-    if (int(blockIdx.x) >= g.plan[L.runs + 2 * kCellTable + 1]) return;
+    const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[kPartTable])[blockIdx.x];   // inside the table's room
+    if (int(blockIdx.x) >= g.plan[L.runs + 2 * kPartTable + 1]) return;
     const int rows = tile.y >> 16, expert = tile.y & 0xffff, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 31, h = lane >> 5;
     const int* order = g.plan + L.order + tile.x;
     const float *x = static_cast<const float*>(g.x), *dy = static_cast<const float*>(g.g), *ys = static_cast<const float*>(g.y);
@@ -689,9 +739,9 @@ __global__ __launch_bounds__(256) void expert_cell_backward_kernel(ExpertArgs g,
                 }
     }
     if (!with_w) return;
-    const bool whole = g.plan[expert] <= kCellRun;
+    const bool whole = g.plan[expert] <= kPartRows;
     float* to_w = whole ? static_cast<float*>(g.out) + int64_t(expert) * g.n_out * g.n_in
-                        : g.partial + ((tile.x >> 8) + expert) * cell_part(g.n_in, g.n_out);
+                        : g.partial + ((tile.x >> 8) + expert) * part_size(g.n_in, g.n_out);
     float* to_b = !whole ? to_w + int64_t(g.n_out) * g.n_in : g.db ? static_cast<float*>(g.db) + int64_t(expert) * g.n_out : nullptr;
     // the wavefronts' parts of each 32 x 32 block, summed in their order.  Lane (c, h) register t: dW[32 o + c][32 b + acc_row(t, h)]
 #pragma unroll
@@ -718,20 +768,6 @@ __global__ __launch_bounds__(256) void expert_cell_backward_kernel(ExpertArgs g,
         to_b[f] = ((s_db[0][f] + s_db[1][f]) + s_db[2][f]) + s_db[3][f];
     }
 }
-__global__ __launch_bounds__(256) void expert_cell_sum_kernel(ExpertArgs g) {
-    const PlanLayout L(g.n, g.E);
-    const int expert = blockIdx.x, rows = g.plan[expert];
-    if (rows > 0 && rows <= kCellRun) return;
-    const int64_t part = cell_part(g.n_in, g.n_out), weights = int64_t(g.n_out) * g.n_in;
-    const int first = g.plan[L.offsets + expert];
-    for (int i = threadIdx.x; i < part; i += 256) {
-        float v = 0.f;
-        for (int r = 0; r < rows; r += kCellRun) v += g.partial[(((first + r) >> 8) + expert) * part + i];
-        if (i < weights) static_cast<float*>(g.out)[expert * weights + i] = v;
-        else if (g.db) static_cast<float*>(g.db)[int64_t(expert) * g.n_out + i - weights] = v;
-    }
-}
-
 int launch_cell_forward(const ExpertArgs& g, hipStream_t stream) {
     const bool i2 = g.n_in > 32, o2 = g.n_out > 32;
     const dim3 grid(unsigned(PlanLayout::slots(g.n, g.E, kCellRowsTable)));
@@ -743,8 +779,7 @@ int launch_cell_forward(const ExpertArgs& g, hipStream_t stream) {
 }
 template <int NI, int NO>
 int launch_cell_backward(const ExpertArgs& g, float* dx, hipStream_t stream) {
-    expert_cell_backward_kernel<NI, NO><<<dim3(unsigned(PlanLayout::slots(g.n, g.E, kCellTable))), 256, 0, stream>>>(g, dx);
-    if (g.out) expert_cell_sum_kernel<<<dim3(unsigned(g.E)), 256, 0, stream>>>(g);
+    expert_cell_backward_kernel<NI, NO><<<dim3(unsigned(PlanLayout::slots(g.n, g.E, kPartTable))), 256, 0, stream>>>(g, dx);
     return NRF_OK;
 }
 int launch_cell_backward(const ExpertArgs& g, float* dx, hipStream_t stream) {
@@ -754,44 +789,80 @@ int launch_cell_backward(const ExpertArgs& g, float* dx, hipStream_t stream) {
 }
 bool cells(int n_in, int n_out, int dtype) { return dtype == NRF_DTYPE_FP32 && n_in <= 64 && n_out <= 64; }
 
-// out[i] = sum over the splits, in their order
+// An expert's parts, added in their order; zeros for an expert without rows.
 template <class T>
-__global__ __launch_bounds__(256) void expert_reduce_kernel(const float* __restrict__ partial, int64_t count, int splits, void* out) {
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count; i += int64_t(gridDim.x) * 256) {
+__global__ __launch_bounds__(256) void expert_sum_kernel(ExpertArgs g) {
+    typedef typename Traits<T>::elem elem;
+    const PlanLayout L(g.n, g.E);
+    const int expert = blockIdx.y, rows = g.plan[expert];
+    const bool by_runs = g.splits == 0;
+    if (by_runs && rows > 0 && rows <= kPartRows) return;              // written at once
+    const int64_t size = part_size(g.n_in, g.n_out), weights = int64_t(g.n_out) * g.n_in;
+    const int64_t first = by_runs ? (g.plan[L.offsets + expert] >> 8) + expert : expert, step = by_runs ? 1 : g.E;
+    const int parts = by_runs ? (rows + kPartRows - 1) / kPartRows : g.splits;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < size; i += int64_t(gridDim.x) * 256) {
+        const float* p = g.partial + first * size + i;
         float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += partial[s * count + i];
-        static_cast<typename Traits<T>::elem*>(out)[i] = from_float(v, T{});
+#pragma unroll 4
+        for (int r = 0; r < parts; ++r) v += p[r * step * size];
+        if (i < weights) static_cast<elem*>(g.out)[expert * weights + i] = from_float(v, T{});
+        else if (g.db) static_cast<elem*>(g.db)[int64_t(expert) * g.n_out + i - weights] = from_float(v, T{});
     }
 }
 
-// How many parts the sum over an expert's rows is cut into: enough workgroups for the chip where the outputs alone give too
-// few, none shorter than 256 rows of the average expert.
+// The general tile's size for a product: 128 where that leaves at least one and a half workgroups per CU.
+int64_t tile_count(int form, int64_t n, int E, int n_in, int n_out, int tile) {
+    const int64_t in = (n_in + tile - 1) / tile, out = (n_out + tile - 1) / tile, rows = n / tile + (E < n ? E : n) / 2;
+    return form == kForward ? rows * out : form == kDx ? rows * in : in * out * E;
+}
+int tile_size(int form, int64_t n, int E, int n_in, int n_out, int splits) {
+    return n / E > 64 && n_in > 64 && n_out > 64 && tile_count(form, n, E, n_in, n_out, 128) * splits >= 384 ? 128 : 64;
+}
+// How dW's sum over an expert's rows is cut (see ExpertArgs): not at all where the outputs alone give 512 workgroups; else by
+// runs, which balances uneven experts, while the parts stay under 1 GiB; else into equal shares.  Wide kernels: equal shares of
+// at least 512 rows of the average expert, enough for a workgroup per CU.
 int dw_splits(int64_t n, int E, int n_in, int n_out, bool is_wide) {
+    int64_t want, most;
     if (is_wide) {
         typedef WideDw<Bf16> W;
         const int64_t tiles = int64_t(E) * ((n_in + W::kA - 1) / W::kA) * ((n_out + W::kB - 1) / W::kB);
-        const int64_t want = (256 + tiles - 1) / tiles, most = n / E / 512;
-        return int(want < most ? want : most < 1 ? 1 : most);
+        want = (256 + tiles - 1) / tiles, most = n / E / 512;
+    } else {
+        const int64_t tiles = tile_count(kDw, n, E, n_in, n_out, n_in > 64 && n_out > 64 ? 128 : 64);
+        if (tiles >= 512 || n / E < 2 * kPartRows) return 1;
+        if (PlanLayout::slots(n, E, kPartTable) * part_size(n_in, n_out) * 4 <= int64_t(1) << 30) return 0;
+        want = (512 + tiles - 1) / tiles, most = n / E / 256;
     }
-    const int64_t tiles = int64_t(E) * ((n_in + kT - 1) / kT) * ((n_out + kT - 1) / kT);
-    const int64_t want = (1024 + tiles - 1) / tiles, most = n / E / 256;
     const int64_t s = want < most ? want : most;
     return s < 1 ? 1 : s > 64 ? 64 : int(s);
 }
-
-template <int FORM>
-void launch_tile(int dtype, dim3 grid, const ExpertArgs& g, hipStream_t stream) {
-    if (dtype == NRF_DTYPE_FP32) expert_tile_kernel<Fp32, FORM><<<grid, 256, 0, stream>>>(g);
-    else if (dtype == NRF_DTYPE_BF16) expert_tile_kernel<Bf16, FORM><<<grid, 256, 0, stream>>>(g);
-    else expert_tile_kernel<Fp16, FORM><<<grid, 256, 0, stream>>>(g);
+int64_t part_bytes(int64_t n, int E, int n_in, int n_out, int splits) {
+    const int64_t parts = splits == 0 ? PlanLayout::slots(n, E, kPartTable) : splits > 1 ? int64_t(splits) * E : 0;
+    return parts * part_size(n_in, n_out) * 4;
 }
 
-void launch_reduce(int dtype, const float* partial, int64_t count, int splits, void* out, hipStream_t stream) {
-    const int64_t blocks = (count + 255) / 256;
-    const dim3 grid(unsigned(blocks < 4096 ? blocks : 4096));
-    if (dtype == NRF_DTYPE_FP32) expert_reduce_kernel<Fp32><<<grid, 256, 0, stream>>>(partial, count, splits, out);
-    else if (dtype == NRF_DTYPE_BF16) expert_reduce_kernel<Bf16><<<grid, 256, 0, stream>>>(partial, count, splits, out);
-    else expert_reduce_kernel<Fp16><<<grid, 256, 0, stream>>>(partial, count, splits, out);
+template <int FORM, int TT>
+void launch_tile(int dtype, const ExpertArgs& g, hipStream_t stream) {
+    const unsigned in = (g.n_in + TT - 1) / TT, out = (g.n_out + TT - 1) / TT, slots = unsigned(PlanLayout::slots(g.n, g.E, TT == 64 ? 1 : 2));
+    const dim3 grid = FORM == kForward ? dim3(slots, out) : FORM == kDx ? dim3(slots, in) 
+                      : g.splits == 0 ? dim3(unsigned(PlanLayout::slots(g.n, g.E, kPartTable)), in, out)
+                                      : dim3(unsigned(g.E) * unsigned(g.splits), in, out);
+    if (dtype == NRF_DTYPE_FP32) expert_tile_kernel<Fp32, FORM, TT><<<grid, 256, 0, stream>>>(g);
+    else if (dtype == NRF_DTYPE_BF16) expert_tile_kernel<Bf16, FORM, TT><<<grid, 256, 0, stream>>>(g);
+    else expert_tile_kernel<Fp16, FORM, TT><<<grid, 256, 0, stream>>>(g);
+}
+template <int FORM>
+void launch_tile(int dtype, const ExpertArgs& g, hipStream_t stream) {
+    if (tile_size(FORM, g.n, g.E, g.n_in, g.n_out, g.splits == 0 ? int(g.n / g.E / kPartRows) : g.splits) == 128) launch_tile<FORM, 128>(dtype, g, stream);
+    else launch_tile<FORM, 64>(dtype, g, stream);
+}
+
+void launch_sum(int dtype, const ExpertArgs& g, hipStream_t stream) {
+    const int64_t size = part_size(g.n_in, g.n_out), blocks = size > 8192 ? (size + 255) / 256 : (size + 2047) / 2048;   // (tiny layers: many experts)
+    const dim3 grid(unsigned(blocks < 1024 ? blocks : 1024), unsigned(g.E));
+    if (dtype == NRF_DTYPE_FP32) expert_sum_kernel<Fp32><<<grid, 256, 0, stream>>>(g);
+    else if (dtype == NRF_DTYPE_BF16) expert_sum_kernel<Bf16><<<grid, 256, 0, stream>>>(g);
+    else expert_sum_kernel<Fp16><<<grid, 256, 0, stream>>>(g);
 }
 
 bool shapes_ok(int64_t n, int E, int n_in, int n_out, int dtype, int act) {
@@ -816,32 +887,30 @@ NRF_EXPORT int nrf_expert_linear(const void* x, const void* weight, const void* 
     g.n = n_rows, g.E = num_experts, g.n_in = n_in, g.n_out = n_out, g.relu = act == NRF_ACT_RELU, g.splits = 1;
     nrf_launch_begin();
     if (wide(n_rows, num_experts, n_in, n_out, dtype) && nrf_aligned16(x) && nrf_aligned16(weight)) {
-        const int st = dtype == NRF_DTYPE_BF16 ? launch_wide_rows<Bf16, kForward>(g, static_cast<hipStream_t>(stream))
-                                               : launch_wide_rows<Fp16, kForward>(g, static_cast<hipStream_t>(stream));
+        const int st = dtype == NRF_DTYPE_BF16 ? launch_wide_forward<Bf16>(g, static_cast<hipStream_t>(stream))
+                                               : launch_wide_forward<Fp16>(g, static_cast<hipStream_t>(stream));
         return st != NRF_OK ? st : nrf_launch_status();
     }
     if (cells(n_in, n_out, dtype)) {
         const int st = launch_cell_forward(g, static_cast<hipStream_t>(stream));
         return st != NRF_OK ? st : nrf_launch_status();
     }
-    launch_tile<kForward>(dtype, dim3(unsigned(PlanLayout::slots(n_rows, num_experts, 1)), (n_out + kT - 1) / kT), g,
-                          static_cast<hipStream_t>(stream));
+    launch_tile<kForward>(dtype, g, static_cast<hipStream_t>(stream));
     return nrf_launch_status();
 }
 
 namespace {
 // the backward's workspace: the masked gradient (wide kernels behind a relu), then the partial sums of dW and db
 struct BackwardWork {
-    int splits;
     int64_t dz, partial;
     BackwardWork(int64_t n, int E, int n_in, int n_out, int dtype) {
         const bool is_wide = wide(n, E, n_in, n_out, dtype);
-        const int tile_splits = dw_splits(n, E, n_in, n_out, false), wide_splits = is_wide ? dw_splits(n, E, n_in, n_out, true) : 1;
-        splits = tile_splits > wide_splits ? tile_splits : wide_splits;   // either kernel may run: alignment is known at the call
         dz = is_wide ? (n * n_out * 2 + 255) & ~int64_t(255) : 0;
-        partial = cells(n_in, n_out, dtype) ? PlanLayout::slots(n, E, kCellTable) * cell_part(n_in, n_out) * 4
-                  : splits > 1              ? int64_t(splits) * E * n_out * (n_in + 1) * 4
-                                            : 0;
+        partial = part_bytes(n, E, n_in, n_out, cells(n_in, n_out, dtype) ? 0 : dw_splits(n, E, n_in, n_out, false));
+        if (is_wide) {   // either kernel may run: alignment is known at the call
+            const int64_t p = part_bytes(n, E, n_in, n_out, dw_splits(n, E, n_in, n_out, true));
+            if (p > partial) partial = p;
+        }
     }
 };
 }  // namespace
@@ -873,12 +942,13 @@ NRF_EXPORT int nrf_expert_linear_backward(const void* grad_y, const void* x, con
     g.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + work.dz);
     const bool is_wide = work.dz > 0 && n_rows > 0 && nrf_aligned16(grad_y) && nrf_aligned16(x) && nrf_aligned16(weight) &&
                          nrf_aligned16(y);
-    const int tiles_in = (n_in + kT - 1) / kT, tiles_out = (n_out + kT - 1) / kT;
     int st = NRF_OK;
     nrf_launch_begin();
     if (cells(n_in, n_out, dtype) && n_rows > 0) {
         g.out = grad_weight, g.db = grad_bias;
+        g.splits = 0;
         st = launch_cell_backward(g, static_cast<float*>(grad_x), stream);
+        if (st == NRF_OK && grad_weight) launch_sum(dtype, g, stream);
         return st != NRF_OK ? st : nrf_launch_status();
     }
     if (is_wide && g.relu) {
@@ -892,20 +962,15 @@ NRF_EXPORT int nrf_expert_linear_backward(const void* grad_y, const void* x, con
     }
     if (grad_x && n_rows > 0) {
         g.out = grad_x, g.splits = 1;
-        if (!is_wide) launch_tile<kDx>(dtype, dim3(unsigned(PlanLayout::slots(n_rows, num_experts, 1)), tiles_in), g, stream);
-        else st = dtype == NRF_DTYPE_BF16 ? launch_wide_rows<Bf16, kDx>(g, stream) : launch_wide_rows<Fp16, kDx>(g, stream);
+        if (!is_wide) launch_tile<kDx>(dtype, g, stream);
+        else st = dtype == NRF_DTYPE_BF16 ? launch_wide_rows<Bf16, kDx, 128>(g, stream) : launch_wide_rows<Fp16, kDx, 128>(g, stream);
     }
     if (grad_weight && st == NRF_OK) {
-        const int64_t count = int64_t(num_experts) * n_out * n_in;
         g.splits = dw_splits(n_rows, num_experts, n_in, n_out, is_wide);
         g.out = grad_weight, g.db = grad_bias;
-        if (!is_wide) launch_tile<kDw>(dtype, dim3(unsigned(num_experts) * unsigned(g.splits), tiles_in, tiles_out), g, stream);
+        if (!is_wide) launch_tile<kDw>(dtype, g, stream);
         else st = dtype == NRF_DTYPE_BF16 ? launch_wide_dw<Bf16>(g, stream) : launch_wide_dw<Fp16>(g, stream);
-        if (g.splits > 1) {
-            launch_reduce(dtype, g.partial, count, g.splits, grad_weight, stream);
-            if (grad_bias)
-                launch_reduce(dtype, g.partial + g.splits * count, int64_t(num_experts) * n_out, g.splits, grad_bias, stream);
-        }
+        if (g.splits != 1 && st == NRF_OK) launch_sum(dtype, g, stream);
     }
     return st != NRF_OK ? st : nrf_launch_status();
 }

@@ -328,7 +328,7 @@ __device__ __forceinline__ void store_terms_down(_Float16* dst, int64_t plane, i
 // both places), X' = Q X (to X' and X'^T; the last step: to the output).
 template <class T, int WHAT, int TT>
 __global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, LargeShape L, _Float16* __restrict__ work, int which) {
-    typedef DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2> Gemm;
+    typedef DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2, 2> Gemm;
     extern __shared__ __align__(16) char smem[];
     const int64_t m = blockIdx.y;
     _Float16* w = work + m * L.per_matrix();
@@ -429,7 +429,7 @@ void launch_small(const SchulzArgs& s, hipStream_t stream) {
 
 template <class T, int WHAT, int TT>
 int launch_product(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream) {
-    typedef DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2> Gemm;
+    typedef DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2, 2> Gemm;
     const int m = L.Mp / TT, n = L.Np / TT;
     const int64_t tiles = WHAT == kGram || WHAT == kPoly ? int64_t(m) * (m + 1) / 2 : int64_t(m) * n;
     auto kernel = &schulz_product_kernel<T, WHAT, TT>;
