@@ -59,13 +59,14 @@ struct DmaSide {
     }
     static __device__ __forceinline__ int octet(int j, int wave, int lane) { return (lane % kSlots) ^ swizzle(line(j, wave, lane)); }
 
-    // row_offset(plane, row): bytes from `base` to k = 0 of that row
+    // row_offset(row): bytes from `base` to k = 0 of that row; plane_bytes: from one plane to the next, which is another
+    // wavefront's, so that only a plane's rows have to lie within 4 GiB
     template <class F>
-    __device__ __forceinline__ void start_rows(int wave, int lane, const void* base_, F row_offset) {
-        base = static_cast<const char*>(base_);
+    __device__ __forceinline__ void start_rows(int wave, int lane, const void* base_, int64_t plane_bytes, F row_offset) {
+        static_assert(WAVES % P == 0, "a wavefront moves pieces of one plane");
+        base = static_cast<const char*>(base_) + (wave * kPieces) / (kPlane / 1024) * plane_bytes;
 #pragma unroll
-        for (int j = 0; j < kPieces; ++j)
-            src[j] = row_offset((wave * kPieces + j) / (kPlane / 1024), line(j, wave, lane)) + octet(j, wave, lane) * 16;
+        for (int j = 0; j < kPieces; ++j) src[j] = row_offset(line(j, wave, lane)) + octet(j, wave, lane) * 16;
     }
     // base: k = 0 of row 0; pitch: bytes from one k to the next (kGather: of one list entry); `octets` whole octets are in a row
     __device__ __forceinline__ void start_cols(int wave, int lane, const void* base_, unsigned pitch, int octets) {

@@ -382,12 +382,12 @@ __device__ __forceinline__ void wide_rows_tile(const ExpertArgs& g, char* smem, 
     if (!none) {
         const unsigned pitch = unsigned(n_k) * 2u;
         if constexpr (FORM == kForward) {
-            gemm.a.start_rows(gemm.wave, gemm.lane, w, [&](int, int row) { return unsigned(a0 + row < n_a ? a0 + row : n_a - 1) * pitch; });
+            gemm.a.start_rows(gemm.wave, gemm.lane, w, 0, [&](int row) { return unsigned(a0 + row < n_a ? a0 + row : n_a - 1) * pitch; });
         } else {
             gemm.pitch_a = unsigned(n_a) * 2u, gemm.step_a = int64_t(n_a) * 128;
             gemm.a.start_cols(gemm.wave, gemm.lane, w + a0, gemm.pitch_a, (n_a - a0) / 8);
         }
-        gemm.b.start_rows(gemm.wave, gemm.lane, FORM == kForward ? g.x : g.g, [&](int, int row) { return unsigned(order[row < b_count ? row : 0]) * pitch; });
+        gemm.b.start_rows(gemm.wave, gemm.lane, FORM == kForward ? g.x : g.g, 0, [&](int row) { return unsigned(order[row < b_count ? row : 0]) * pitch; });
         gemm.idle = gemm.wave_b() >= b_count || a0 + gemm.wave_a() >= n_a;
         gemm.run(smem, n_k, acc);
     }

@@ -47,26 +47,27 @@ __device__ __forceinline__ float clamp_grad(float g, const SchulzArgs& s) {
     g *= s.grad_scale;
     return g > s.clip ? s.clip : g < -s.clip ? -s.clip : g;   // NaN stays
 }
-// the matrix to orthogonalise, at element i of tensor t; Muon: from the gradient and the momentum before (NEW: after) its update
+// the matrix to orthogonalise, at element base + i of tensor t; Muon: from the gradient and the momentum before (NEW: after)
+// its update.  With a uniform base and 32 bits of i an address costs one register.
 template <class T, bool NEW>
-__device__ __forceinline__ float element(const SchulzArgs& s, int t, int64_t i, float* momentum) {
+__device__ __forceinline__ float element(const SchulzArgs& s, int t, int64_t base, unsigned i, float* momentum) {
     if constexpr (__is_same(T, OutMuon)) {
-        const float g = clamp_grad(static_cast<const float*>(s.g[t])[i], s);
-        const float old = s.mom[t][i];
+        const float g = clamp_grad((static_cast<const float*>(s.g[t]) + base)[i], s);
+        const float old = (s.mom[t] + base)[i];
         const float m = NEW ? old : __fmaf_rn(s.mu, old, g);
         if (momentum) *momentum = m;
         return s.nesterov ? __fmaf_rn(s.mu, m, g) : m;
     } else {
-        return float(static_cast<const typename Elem<T>::type*>(s.g[t])[i]);
+        return float((static_cast<const typename Elem<T>::type*>(s.g[t]) + base)[i]);
     }
 }
 template <class T>
-__device__ __forceinline__ void emit(const SchulzArgs& s, int t, int64_t i, float v) {
+__device__ __forceinline__ void emit(const SchulzArgs& s, int t, int64_t base, unsigned i, float v) {
     if constexpr (__is_same(T, OutMuon)) {
-        float* p = static_cast<float*>(s.out[t]) + i;
-        *p = __fmaf_rn(-s.rate, v, s.decay * *p);
+        float* p = static_cast<float*>(s.out[t]) + base;
+        p[i] = __fmaf_rn(-s.rate, v, s.decay * p[i]);
     } else {
-        static_cast<typename Elem<T>::type*>(s.out[t])[i] = (typename Elem<T>::type)v;
+        (static_cast<typename Elem<T>::type*>(s.out[t]) + base)[i] = (typename Elem<T>::type)v;
     }
 }
 // 4096 / max(norm, eps); a norm that is not a number stays one
@@ -119,6 +120,24 @@ __device__ __forceinline__ f32x16 product(const Frag& a, const Frag& b, f32x16 c
     for (int s = 0; s < 2; ++s) c = mfma32(a.hi[s], b.hi[s], c);
     return c;
 }
+// A A with what the two terms of A leave out: rest = A - hi - lo as a third term, lo lo, hi rest and rest hi.  A is where
+// rounding starts to be multiplied by b and c; with 22 bits in A's square a batch of 32 x 63 matrices was 1.1e-6 off float64,
+// with these products it is as far off as the iteration in fp32.
+__device__ __forceinline__ f32x16 square(const f32x16& v, const Frag& f) {
+    u32x4 rest[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = f16_residual_lo(f16_residual_lo(v[8 * s + 2 * i], f.hi[s][i]), f.lo[s][i]);
+            const float b = f16_residual_hi(f16_residual_hi(v[8 * s + 2 * i + 1], f.hi[s][i]), f.lo[s][i]);
+            rest[s][i] = pk_f16(a, b);
+        }
+    f32x16 c = {};
+#pragma unroll
+    for (int s = 0; s < 2; ++s) c = mfma32(f.hi[s], rest[s], c), c = mfma32(rest[s], f.hi[s], c), c = mfma32(f.lo[s], f.lo[s], c);
+    return product(f, f, c);
+}
 
 constexpr int kTurnPitch = 36;
 // the fragments of V^T from those of V: element pairs {hi, lo} as words through this wavefront's piece of LDS
@@ -148,16 +167,18 @@ __device__ __forceinline__ Frag turn_block(const Frag& f, unsigned* s_turn, int 
 }
 
 template <class T, int NB, bool TALL>
-__global__ __launch_bounds__(256) void schulz_small_kernel(SchulzArgs s) {
+__global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 2 ? 3 : 4) void schulz_small_kernel(SchulzArgs s) {
     __shared__ __align__(16) unsigned s_all[4][32 * kTurnPitch];
-    const int64_t m = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t m = int64_t(blockIdx.x) * 4 + wave;
     if (m >= s.batch) return;                      // no barrier below: every wavefront works alone
-    unsigned* s_turn = s_all[threadIdx.x >> 6];
+    unsigned* s_turn = s_all[wave];
     const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
     const int t0 = int(m / s.per);
     const int64_t base = (m % s.per) * int64_t(s.rows) * s.cols;
 
-    // G in blocks along its longer side, lanes along its rows: X_j of a wide matrix, Y_j of a tall one (X = G^T)
+    // G in blocks along its longer side, lanes along its rows: X_j of a wide matrix, Y_j of a tall one (X = G^T).  Every load
+    // is made, at the nearest element there is: a load under a condition of its lanes would wait for the one before it
     f32x16 v[NB];
     double sum = 0.0;
 #pragma unroll
@@ -165,15 +186,16 @@ __global__ __launch_bounds__(256) void schulz_small_kernel(SchulzArgs s) {
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
             const int r = (TALL ? 32 * j : 0) + nrf::acc_row(t, h), q = TALL ? c : 32 * j + c;
-            v[j][t] = 0.f;
-            if (r < s.rows && q < s.cols) {
-                const int64_t i = base + int64_t(r) * s.cols + q;
-                float mom = 0.f;
-                v[j][t] = element<T, false>(s, t0, i, &mom);
-                if constexpr (__is_same(T, OutMuon)) s.mom[t0][i] = mom;
-            }
-            sum = __builtin_fma(double(v[j][t]), double(v[j][t]), sum);
+            const int rc = r < s.rows ? r : s.rows - 1, qc = q < s.cols ? q : s.cols - 1;
+            float mom = 0.f;
+            v[j][t] = element<T, false>(s, t0, base, rc * s.cols + qc, &mom);
+            if (r != rc || q != qc) v[j][t] = 0.f;
+            else if constexpr (__is_same(T, OutMuon)) (s.mom[t0] + base)[unsigned(r * s.cols + q)] = mom;
         }
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int t = 0; t < 16; ++t) sum = __builtin_fma(double(v[j][t]), double(v[j][t]), sum);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
     const float scale = start_scale(sum, s.eps);
@@ -183,34 +205,35 @@ __global__ __launch_bounds__(256) void schulz_small_kernel(SchulzArgs s) {
         v[j] = v[j] * scale;
         here[j] = split_block(v[j]);
         turned[j] = turn_block(here[j], s_turn, c, h);
-        v[j] = v[j] * kScale;                      // no step at all: the scaled matrix
     }
     for (int k = 0; k < s.steps; ++k) {
         f32x16 acc = {};
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc = TALL ? product(here[j], here[j], acc) : product(turned[j], turned[j], acc);
         const f32x16 gram = acc * kUnscale;
-        const Frag fg = split_block(gram);
-        acc = product(fg, fg, (f32x16){});
-        f32x16 poly = s.b * gram + (s.c * kUnscale) * acc;
+        acc = square(gram, split_block(gram));
+        // Q without the scale (the matrix cores read subnormal terms: 2^-25 off at most), so that Q X has X's
+        f32x16 poly = (s.b * kUnscale) * gram + (s.c * kUnscale * kUnscale) * acc;
 #pragma unroll
-        for (int t = 0; t < 16; ++t) poly[t] += nrf::acc_row(t, h) == c ? s.a * kScale : 0.f;
+        for (int t = 0; t < 16; ++t) poly[t] += nrf::acc_row(t, h) == c ? s.a : 0.f;
         const Frag fq = split_block(poly);
 #pragma unroll
         for (int j = 0; j < NB; ++j) v[j] = TALL ? product(turned[j], fq, (f32x16){}) : product(fq, here[j], (f32x16){});
         if (k + 1 < s.steps)
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
-                here[j] = split_block(v[j] * kUnscale);
+                here[j] = split_block(v[j]);
                 turned[j] = turn_block(here[j], s_turn, c, h);
             }
     }
+    const bool whole = TALL ? s.cols == 32 : s.rows == 32;   // every lane (row) of the shorter side is there
 #pragma unroll
     for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
             const int r = (TALL ? 32 * j : 0) + nrf::acc_row(t, h), q = TALL ? c : 32 * j + c;
-            if (r < s.rows && q < s.cols) emit<T>(s, t0, base + int64_t(r) * s.cols + q, v[j][t] * (kUnscale * kUnscale));
+            if ((whole || (TALL ? q < s.cols : r < s.rows)) && (TALL ? r < s.rows : q < s.cols))
+                emit<T>(s, t0, base, r * s.cols + q, v[j][t] * kUnscale);
         }
 }
 
@@ -218,7 +241,7 @@ __global__ __launch_bounds__(256) void schulz_small_kernel(SchulzArgs s) {
 // The workspace of a matrix, in fp16 elements, M and N padded with zeros (which every product keeps) to the tile: X [2 terms]
 // [M][N] and X^T [2][N][M], both twice (a step reads one and writes the other), A and Q [2][M][M].
 struct LargeShape {
-    int M, N, Mp, Np, tile, chunks;
+    int M, N, Mp, Np, tile, chunks, chunk;   // chunks: of the norm's sum, `chunk` elements each
     __host__ __device__ int64_t x_size() const { return int64_t(2) * Mp * Np; }
     __host__ __device__ int64_t s_size() const { return int64_t(2) * Mp * Mp; }
     __host__ __device__ int64_t per_matrix() const { return 4 * x_size() + 2 * s_size(); }
@@ -227,21 +250,31 @@ struct LargeShape {
     __host__ __device__ int64_t gram_at() const { return 4 * x_size(); }
     __host__ __device__ int64_t poly_at() const { return 4 * x_size() + s_size(); }
 };
-constexpr int kNormChunk = 16384;   // elements a workgroup sums
+constexpr int kNormBatch = 8;       // elements of a thread at a time, all loaded before the first is used
 
-// |G|_F^2 in parts; Muon: the momentum's update
+// |G|_F^2 in L.chunks parts; Muon: the momentum's update
 template <class T>
 __global__ __launch_bounds__(256) void schulz_norm_kernel(SchulzArgs s, LargeShape L, double* __restrict__ parts) {
     const int64_t m = blockIdx.y, count = int64_t(s.rows) * s.cols;
     const int t = int(m / s.per);
     const int64_t base = (m % s.per) * count;
-    const int64_t begin = int64_t(blockIdx.x) * kNormChunk, end = begin + kNormChunk < count ? begin + kNormChunk : count;
+    const int64_t begin = int64_t(blockIdx.x) * L.chunk, end = begin + L.chunk < count ? begin + L.chunk : count;
     double sum = 0.0;
-    for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
-        float mom = 0.f;
-        const float v = element<T, false>(s, t, base + i, &mom);
-        if constexpr (__is_same(T, OutMuon)) s.mom[t][base + i] = mom;
-        sum = __builtin_fma(double(v), double(v), sum);
+    for (int64_t i0 = begin; i0 < end; i0 += 256 * kNormBatch) {
+        const unsigned left = unsigned(end - i0 < 256 * kNormBatch ? end - i0 : 256 * kNormBatch);
+        float v[kNormBatch], mom[kNormBatch];
+#pragma unroll
+        for (int u = 0; u < kNormBatch; ++u) {
+            const unsigned i = 256 * u + threadIdx.x;
+            v[u] = element<T, false>(s, t, base + i0, i < left ? i : left - 1, mom + u);
+        }
+#pragma unroll
+        for (int u = 0; u < kNormBatch; ++u) {
+            const unsigned i = 256 * u + threadIdx.x;
+            if (i >= left) continue;
+            if constexpr (__is_same(T, OutMuon)) (s.mom[t] + base + i0)[i] = mom[u];
+            sum = __builtin_fma(double(v[u]), double(v[u]), sum);
+        }
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
@@ -256,42 +289,51 @@ template <class T>
 __global__ __launch_bounds__(256) void schulz_start_kernel(SchulzArgs s, LargeShape L, const double* __restrict__ parts,
                                                            _Float16* __restrict__ work) {
     __shared__ float s_tile[64][65];
-    __shared__ float s_scale;
     const int64_t m = blockIdx.z, count = int64_t(s.rows) * s.cols;
-    if (threadIdx.x < 64) {
-        double sum = 0.0;
-        for (int i = threadIdx.x; i < L.chunks; i += 64) sum += parts[m * L.chunks + i];
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
-        if (threadIdx.x == 0) s_scale = start_scale(sum, s.eps);
-    }
-    __syncthreads();
-    const float scale = s_scale;
     const bool tall = s.rows > s.cols;
     const int t = int(m / s.per), r0 = blockIdx.y * 64, q0 = blockIdx.x * 64;
-    const int64_t base = (m % s.per) * count;
+    const int64_t base = (m % s.per) * count + int64_t(r0 < s.rows ? r0 : 0) * s.cols;
+    const int lane = threadIdx.x & 63;
+    double sum = 0.0;                                                // every wavefront for itself
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int i = 64 * u + lane;
+        const double part = parts[m * L.chunks + (i < L.chunks ? i : 0)];
+        sum += i < L.chunks ? part : 0.0;
+    }
+    const int q = (threadIdx.x & 31) * 2;                            // a pair of columns
+    float v[8][2];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = r0 + (threadIdx.x >> 5) + 8 * u, col = q0 + q + i;
+            const bool in = r < s.rows && col < s.cols;
+            const float x = element<T, true>(s, t, base, in ? unsigned(r - r0) * s.cols + col : 0u, nullptr);
+            v[u][i] = in ? x : 0.f;
+        }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+    const float scale = start_scale(sum, s.eps);
     const int rp = tall ? L.Np : L.Mp, cp = tall ? L.Mp : L.Np;      // padded rows and columns of G
     _Float16* w = work + m * L.per_matrix();
     _Float16* straight = w + (tall ? L.xt_at(0) : L.x_at(0));        // [rp][cp]
     _Float16* turned = w + (tall ? L.x_at(0) : L.xt_at(0));          // [cp][rp]
     unsigned *straight32 = reinterpret_cast<unsigned*>(straight), *turned32 = reinterpret_cast<unsigned*>(turned);
-    const int q = (threadIdx.x & 31) * 2;                            // a pair of columns
-    for (int r = threadIdx.x >> 5; r < 64; r += 8) {
-        float v[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            v[i] = 0.f;
-            if (r0 + r < s.rows && q0 + q + i < s.cols)
-                v[i] = element<T, true>(s, t, base + int64_t(r0 + r) * s.cols + q0 + q + i, nullptr) * scale;
-            s_tile[r][q + i] = v[i];
-        }
+    for (int u = 0; u < 8; ++u) {
+        const int r = (threadIdx.x >> 5) + 8 * u;
+        v[u][0] *= scale, v[u][1] *= scale;
+        s_tile[r][q] = v[u][0], s_tile[r][q + 1] = v[u][1];
         unsigned hi, lo;
-        split_pair_h2(v[0], v[1], hi, lo);
+        split_pair_h2(v[u][0], v[u][1], hi, lo);
         const int64_t at = int64_t(r0 + r) * cp + q0 + q;
         straight32[at >> 1] = hi, straight32[(int64_t(rp) * cp + at) >> 1] = lo;
     }
     __syncthreads();
-    for (int r = threadIdx.x >> 5; r < 64; r += 8) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int r = (threadIdx.x >> 5) + 8 * u;
         unsigned hi, lo;
         split_pair_h2(s_tile[q][r], s_tile[q + 1][r], hi, lo);
         const int64_t at = int64_t(q0 + r) * rp + r0 + q;
@@ -347,8 +389,9 @@ __global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, Large
     const _Float16* pb = w + (WHAT == kGram ? L.x_at(which) : WHAT == kPoly ? L.gram_at() : L.xt_at(which));
     const int64_t plane_a = int64_t(L.Mp) * K, plane_b = int64_t(WHAT == kGram || WHAT == kPoly ? L.Mp : L.Np) * K;
     Gemm gemm;
-    gemm.a.start_rows(gemm.wave, gemm.lane, pa, [&](int plane, int row) { return unsigned(plane * plane_a + int64_t(a0 + row) * K) * 2u; });
-    gemm.b.start_rows(gemm.wave, gemm.lane, pb, [&](int plane, int row) { return unsigned(plane * plane_b + int64_t(b0 + row) * K) * 2u; });
+    // offsets inside a tile: at most 128 rows of 65536 terms
+    gemm.a.start_rows(gemm.wave, gemm.lane, pa + int64_t(a0) * K, plane_a * 2, [&](int row) { return unsigned(row * K) * 2u; });
+    gemm.b.start_rows(gemm.wave, gemm.lane, pb + int64_t(b0) * K, plane_b * 2, [&](int row) { return unsigned(row * K) * 2u; });
     f32x4 acc[Gemm::kMA][Gemm::kMB] = {};
     gemm.run(smem, K, acc);
 
@@ -386,7 +429,7 @@ __global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, Large
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (a + r < L.M)
-                        emit<T>(s, t, base + (tall ? int64_t(b) * s.cols + a + r : int64_t(a + r) * s.cols + b), v[r] * kUnscale);
+                        emit<T>(s, t, base, tall ? unsigned(b) * s.cols + a + r : unsigned(a + r) * s.cols + b, v[r] * kUnscale);
             }
         }
 }
@@ -401,7 +444,7 @@ __global__ __launch_bounds__(256) void schulz_copy_kernel(SchulzArgs s, LargeSha
     const int t = int(m / s.per);
     const int64_t base = (m % s.per) * count;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count; i += int64_t(gridDim.x) * 256)
-        emit<T>(s, t, base + i, element<T, true>(s, t, base + i, nullptr) * scale);
+        emit<T>(s, t, base + i, 0, element<T, true>(s, t, base + i, 0, nullptr) * scale);
 }
 
 bool small_path(int rows, int cols) {
@@ -414,7 +457,11 @@ LargeShape large_shape(int rows, int cols) {
     L.M = rows < cols ? rows : cols, L.N = rows < cols ? cols : rows;
     L.tile = L.M > 512 ? 128 : 64;
     L.Mp = (L.M + L.tile - 1) / L.tile * L.tile, L.Np = (L.N + L.tile - 1) / L.tile * L.tile;
-    L.chunks = int((int64_t(rows) * cols + kNormChunk - 1) / kNormChunk);
+    // at most 512 parts, which every workgroup of schulz_start_kernel adds up again
+    const int64_t count = int64_t(rows) * cols, least = 256 * kNormBatch;
+    const int64_t times = (count + 512 * least - 1) / (512 * least);
+    L.chunk = int(times * least);
+    L.chunks = int((count + L.chunk - 1) / L.chunk);
     return L;
 }
 
@@ -428,7 +475,7 @@ void launch_small(const SchulzArgs& s, hipStream_t stream) {
 }
 
 template <class T, int WHAT, int TT>
-int launch_product(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream) {
+int launch_tiles(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream) {
     typedef DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2, 2> Gemm;
     const int m = L.Mp / TT, n = L.Np / TT;
     const int64_t tiles = WHAT == kGram || WHAT == kPoly ? int64_t(m) * (m + 1) / 2 : int64_t(m) * n;
@@ -440,7 +487,16 @@ int launch_product(const SchulzArgs& s, const LargeShape& L, _Float16* work, int
     return NRF_OK;
 }
 
-template <class T, int TT>
+// Tiles of 128 x 128 read half as much as tiles of 64 x 64, but one of them holds a CU by itself (128 KiB of LDS): they are
+// for products that have enough of them.
+template <class T, int WHAT>
+int launch_product(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream) {
+    const int64_t m = L.Mp / 128, n = L.Np / 128;
+    const int64_t tiles = (WHAT == kGram || WHAT == kPoly ? m * (m + 1) / 2 : m * n) * s.batch;
+    return L.tile == 128 && tiles >= 192 ? launch_tiles<T, WHAT, 128>(s, L, work, which, stream) : launch_tiles<T, WHAT, 64>(s, L, work, which, stream);
+}
+
+template <class T>
 int run_large(const SchulzArgs& s, const LargeShape& L, double* parts, _Float16* work, hipStream_t stream) {
     const dim3 cover(unsigned((s.rows > s.cols ? L.Mp : L.Np) / 64), unsigned((s.rows > s.cols ? L.Np : L.Mp) / 64), unsigned(s.batch));
     schulz_norm_kernel<T><<<dim3(unsigned(L.chunks), unsigned(s.batch)), 256, 0, stream>>>(s, L, parts);
@@ -450,11 +506,11 @@ int run_large(const SchulzArgs& s, const LargeShape& L, double* parts, _Float16*
     }
     schulz_start_kernel<T><<<cover, 256, 0, stream>>>(s, L, parts, work);
     for (int k = 0; k < s.steps; ++k) {
-        int st = launch_product<Out32, kGram, TT>(s, L, work, k & 1, stream);   // the output's type matters to kLast alone
-        if (st == NRF_OK) st = launch_product<Out32, kPoly, TT>(s, L, work, k & 1, stream);
+        int st = launch_product<Out32, kGram>(s, L, work, k & 1, stream);   // the output's type matters to kLast alone
+        if (st == NRF_OK) st = launch_product<Out32, kPoly>(s, L, work, k & 1, stream);
         if (st == NRF_OK)
-            st = k + 1 < s.steps ? launch_product<Out32, kApply, TT>(s, L, work, k & 1, stream)
-                                 : launch_product<T, kLast, TT>(s, L, work, k & 1, stream);
+            st = k + 1 < s.steps ? launch_product<Out32, kApply>(s, L, work, k & 1, stream)
+                                 : launch_product<T, kLast>(s, L, work, k & 1, stream);
         if (st != NRF_OK) return st;
     }
     return NRF_OK;
@@ -471,7 +527,7 @@ int run(const SchulzArgs& s, void* workspace, hipStream_t stream) {
     const LargeShape L = large_shape(s.rows, s.cols);
     double* parts = static_cast<double*>(workspace);
     _Float16* work = reinterpret_cast<_Float16*>(parts + ((s.batch * L.chunks + 31) & ~int64_t(31)));
-    const int st = L.tile == 128 ? run_large<T, 128>(s, L, parts, work, stream) : run_large<T, 64>(s, L, parts, work, stream);
+    const int st = run_large<T>(s, L, parts, work, stream);
     return st != NRF_OK ? st : nrf_launch_status();
 }
 
