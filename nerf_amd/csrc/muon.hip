@@ -343,45 +343,43 @@ __global__ __launch_bounds__(256) void schulz_start_kernel(SchulzArgs s, LargeSh
 
 enum Product { kGram, kPoly, kApply, kLast };
 
-// four values of consecutive a as their two terms: at dst (plane stride `plane`), or down a column of rows of `pitch`
-struct Terms {
-    u32x2 hi, lo;
-};
-__device__ __forceinline__ Terms terms_of(const f32x4& v) {
-    unsigned h0, l0, h1, l1;
-    split_pair_h2(v[0], v[1], h0, l0);
-    split_pair_h2(v[2], v[3], h1, l1);
-    return {{h0, h1}, {l0, l1}};
-}
-__device__ __forceinline__ void store_terms(_Float16* dst, int64_t plane, const Terms& v) {
-    *reinterpret_cast<u32x2*>(dst) = v.hi;
-    *reinterpret_cast<u32x2*>(dst + plane) = v.lo;
-}
-__device__ __forceinline__ void store_terms_down(_Float16* dst, int64_t plane, int64_t pitch, const Terms& v) {
-    unsigned short* d = reinterpret_cast<unsigned short*>(dst);
+// 64 x 64 or 128 x 128 outputs by four wavefronts
+template <int TT> using SchulzGemm = DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2, 2>;
+
+// words[i] = {hi, lo} of eight consecutive elements -> 16 B of each plane
+__device__ __forceinline__ void store_octet(_Float16* dst, int64_t plane, const unsigned (&w)[8]) {
+    u32x4 hi, lo;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        d[r * pitch] = (unsigned short)(v.hi[r >> 1] >> (16 * (r & 1)));
-        d[plane + r * pitch] = (unsigned short)(v.lo[r >> 1] >> (16 * (r & 1)));
+    for (int i = 0; i < 4; ++i) {
+        hi[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
+        lo[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
     }
+    *reinterpret_cast<u32x4*>(dst) = hi;
+    *reinterpret_cast<u32x4*>(dst + plane) = lo;
 }
 
 // One product of a step: A = X X^T and Q = a I + b A + c A A (symmetric: the tiles on and over the diagonal, each written to
-// both places), X' = Q X (to X' and X'^T; the last step: to the output).
+// both places), X' = Q X (to X' and X'^T; the last step: to the output).  Workgroups are dealt out to the XCDs in turn, so each
+// XCD takes consecutive tiles, which share their operands' rows in its L2.  A finished tile goes through LDS (rows of TT + 1
+// words), so that both orientations are written 16 B per lane: as the accumulators lie, a lane has 4 elements of one
+// orientation and 1 of the other.
 template <class T, int WHAT, int TT>
-__global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, LargeShape L, _Float16* __restrict__ work, int which) {
-    typedef DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2, 2> Gemm;
+__global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, LargeShape L, _Float16* __restrict__ work, int which, int tiles) {
+    typedef SchulzGemm<TT> Gemm;
     extern __shared__ __align__(16) char smem[];
-    const int64_t m = blockIdx.y;
+    const int total = int(s.batch) * tiles, share = (total + 7) / 8;
+    const int unit = int(blockIdx.x & 7) * share + int(blockIdx.x >> 3);
+    if (unit >= total) return;
+    const int64_t m = unit / tiles;
     _Float16* w = work + m * L.per_matrix();
     const int tiles_m = L.Mp / TT;
     int ta, tb;
     if (WHAT == kGram || WHAT == kPoly) {   // tile pairs (ta <= tb), tb-th row has tb + 1
-        int left = blockIdx.x;
+        int left = unit % tiles;
         for (tb = 0; left > tb; ++tb) left -= tb + 1;
         ta = left;
     } else {
-        ta = blockIdx.x % tiles_m, tb = blockIdx.x / tiles_m;
+        ta = unit % tiles % tiles_m, tb = unit % tiles / tiles_m;
     }
     const int a0 = ta * TT, b0 = tb * TT;
     const int K = WHAT == kGram ? L.Np : L.Mp;
@@ -395,43 +393,75 @@ __global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, Large
     f32x4 acc[Gemm::kMA][Gemm::kMB] = {};
     gemm.run(smem, K, acc);
 
+    constexpr int kPitch = TT + 1;
+    static_assert(TT * kPitch * 4 <= Gemm::kLds, "the tile in LDS");
+    unsigned* s_out = reinterpret_cast<unsigned*>(smem);              // [a][b]
     const int c = gemm.lane & 15, q = gemm.lane >> 4, t = int(m / s.per);
-    const int64_t base = (m % s.per) * int64_t(s.rows) * s.cols;
-    const bool tall = s.rows > s.cols;
-    _Float16* sym = w + (WHAT == kGram ? L.gram_at() : L.poly_at());
-    _Float16 *xn = w + L.x_at(which ^ 1), *xtn = w + L.xt_at(which ^ 1);
+    const int64_t plane = int64_t(L.Mp) * (WHAT == kGram || WHAT == kPoly ? L.Mp : L.Np);
+    __syncthreads();
 #pragma unroll
     for (int ma = 0; ma < Gemm::kMA; ++ma)
 #pragma unroll
         for (int mb = 0; mb < Gemm::kMB; ++mb) {
-            const int a = a0 + gemm.wave_a() + 16 * ma + 4 * q, b = b0 + gemm.wave_b() + 16 * mb + c;
+            const int a = gemm.wave_a() + 16 * ma + 4 * q, b = gemm.wave_b() + 16 * mb + c;
             f32x4 v = acc[ma][mb] * kUnscale;
-            if (WHAT == kGram || WHAT == kPoly) {
-                const int64_t plane = int64_t(L.Mp) * L.Mp, at = int64_t(b) * L.Mp + a;
-                if (WHAT == kPoly) {
-                    const u32x2 hi = *reinterpret_cast<const u32x2*>(w + L.gram_at() + at);
-                    const u32x2 lo = *reinterpret_cast<const u32x2*>(w + L.gram_at() + plane + at);
+            if (WHAT == kPoly) {
+                const int64_t at = int64_t(b0 + b) * L.Mp + a0 + a;
+                const u32x2 hi = *reinterpret_cast<const u32x2*>(w + L.gram_at() + at);
+                const u32x2 lo = *reinterpret_cast<const u32x2*>(w + L.gram_at() + plane + at);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float g = r & 1 ? pair_hi(hi[r >> 1]) + pair_hi(lo[r >> 1]) : pair_lo(hi[r >> 1]) + pair_lo(lo[r >> 1]);
-                        v[r] = s.b * g + s.c * v[r] + (a + r == b ? s.a * kScale : 0.f);
-                    }
+                for (int r = 0; r < 4; ++r) {
+                    const float g = r & 1 ? pair_hi(hi[r >> 1]) + pair_hi(lo[r >> 1]) : pair_lo(hi[r >> 1]) + pair_lo(lo[r >> 1]);
+                    v[r] = s.b * g + s.c * v[r] + (a0 + a + r == b0 + b ? s.a * kScale : 0.f);
                 }
-                const Terms o = terms_of(v);
-                store_terms(sym + at, plane, o);
-                if (ta != tb) store_terms_down(sym + int64_t(a) * L.Mp + b, plane, L.Mp, o);
-            } else if (WHAT == kApply) {   // a: row of X', b: column
-                const int64_t plane = int64_t(L.Mp) * L.Np;
-                const Terms o = terms_of(v);
-                store_terms(xtn + int64_t(b) * L.Mp + a, plane, o);
-                store_terms_down(xn + int64_t(a) * L.Np + b, plane, L.Np, o);
-            } else if (b < L.N) {
+            }
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (a + r < L.M)
-                        emit<T>(s, t, base, tall ? unsigned(b) * s.cols + a + r : unsigned(a + r) * s.cols + b, v[r] * kUnscale);
+            for (int r = 0; r < 4; r += 2) {
+                unsigned w0, w1;
+                if (WHAT == kLast) {
+                    w0 = __builtin_bit_cast(unsigned, v[r] * kUnscale), w1 = __builtin_bit_cast(unsigned, v[r + 1] * kUnscale);
+                } else {
+                    unsigned hi, lo;
+                    split_pair_h2(v[r], v[r + 1], hi, lo);
+                    w0 = __builtin_amdgcn_perm(lo, hi, 0x05040100u), w1 = __builtin_amdgcn_perm(lo, hi, 0x07060302u);
+                }
+                s_out[(a + r) * kPitch + b] = w0, s_out[(a + r + 1) * kPitch + b] = w1;
             }
         }
+    __syncthreads();
+    if constexpr (WHAT == kLast) {
+        // lanes along the output's rows; what a Muon step reads of the parameters is loaded four ahead
+        const bool tall = s.rows > s.cols;
+        const int64_t base = (m % s.per) * int64_t(s.rows) * s.cols;
+        const int r0 = tall ? b0 : a0, q0 = tall ? a0 : b0;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < TT * TT; i += 256) {
+            const int r = i / TT, col = i % TT;
+            if (r0 + r < s.rows && q0 + col < s.cols)
+                emit<T>(s, t, base, unsigned(r0 + r) * s.cols + q0 + col, __builtin_bit_cast(float, s_out[tall ? col * kPitch + r : r * kPitch + col]));
+        }
+    } else {
+        _Float16* straight = w + (WHAT == kGram ? L.gram_at() : WHAT == kPoly ? L.poly_at() : L.xt_at(which ^ 1));   // rows b
+        _Float16* turned = WHAT == kApply ? w + L.x_at(which ^ 1) : straight;                                        // rows a
+        const int pitch_turned = WHAT == kApply ? L.Np : L.Mp;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < TT * TT / 8; i += 256) {
+            const int b = i / (TT / 8), a = i % (TT / 8) * 8;
+            unsigned v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = s_out[(a + j) * kPitch + b];
+            store_octet(straight + int64_t(b0 + b) * L.Mp + a0 + a, plane, v);
+        }
+        if (WHAT == kApply || ta != tb)
+#pragma unroll 4
+            for (int i = threadIdx.x; i < TT * TT / 8; i += 256) {
+                const int a = i / (TT / 8), b = i % (TT / 8) * 8;
+                unsigned v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = s_out[a * kPitch + b + j];
+                store_octet(turned + int64_t(a0 + a) * pitch_turned + b0 + b, plane, v);
+            }
+    }
 }
 
 // no step at all: the scaled matrix itself
@@ -476,14 +506,15 @@ void launch_small(const SchulzArgs& s, hipStream_t stream) {
 
 template <class T, int WHAT, int TT>
 int launch_tiles(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream) {
-    typedef DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2, 2> Gemm;
+    typedef SchulzGemm<TT> Gemm;
     const int m = L.Mp / TT, n = L.Np / TT;
-    const int64_t tiles = WHAT == kGram || WHAT == kPoly ? int64_t(m) * (m + 1) / 2 : int64_t(m) * n;
+    const int tiles = WHAT == kGram || WHAT == kPoly ? m * (m + 1) / 2 : m * n;
     auto kernel = &schulz_product_kernel<T, WHAT, TT>;
     if (Gemm::kLds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                   Gemm::kLds) != hipSuccess)
         return NRF_ERR_LAUNCH;
-    kernel<<<dim3(unsigned(tiles), unsigned(s.batch)), 256, Gemm::kLds, stream>>>(s, L, work, which);
+    const unsigned groups = unsigned((int(s.batch) * tiles + 7) / 8 * 8);
+    kernel<<<groups, 256, Gemm::kLds, stream>>>(s, L, work, which, tiles);
     return NRF_OK;
 }
 
@@ -534,7 +565,8 @@ int run(const SchulzArgs& s, void* workspace, hipStream_t stream) {
 bool schulz_shape_ok(int64_t batch, int rows, int cols) {
     if (batch < 0 || rows < 1 || cols < 1 || rows > 65536 || cols > 65536) return false;
     if (small_path(rows, cols)) return batch <= int64_t(1) << 24;
-    return batch <= 65535;
+    const LargeShape L = large_shape(rows, cols);
+    return batch <= 65535 && batch * (int64_t(L.Mp / 64) * (L.Np / 64)) <= int64_t(1) << 24;
 }
 // the iteration on the singular values, which start in [0, 1]: entries of X, A and Q must stay inside fp16 at scale 2^12
 bool coefficients_ok(int steps, float a, float b, float c) {
