@@ -343,15 +343,15 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
 }
 
 // ---- bf16 / fp16, wide layers ----------------------------------------------------------------------------------------------
-// Consecutive workgroups go to different XCDs: each XCD takes a contiguous eighth of the whole row runs and of the rests (an
-// expert's runs share its weights in that XCD's L2).  -> the `local`-th run of this one, -1 past its last.
+// Consecutive workgroups go to different XCDs: each XCD takes a contiguous eighth of the long row runs and of the short
+// ones (an expert's runs share its weights in that XCD's L2).  -> the `local`-th run of this one, -1 past its last.
 __device__ __forceinline__ int xcd_run(const int* runs, int xcd, int local) {
-    const int whole = runs[0], rests = runs[1] - whole;
-    int begin = int(int64_t(whole) * xcd / 8), end = int(int64_t(whole) * (xcd + 1) / 8);
+    const int longs = runs[0], shorts = runs[1] - longs;
+    int begin = int(int64_t(longs) * xcd / 8), end = int(int64_t(longs) * (xcd + 1) / 8);
     if (local < end - begin) return begin + local;
     local -= end - begin;
-    begin = int(int64_t(rests) * xcd / 8), end = int(int64_t(rests) * (xcd + 1) / 8);
-    return local < end - begin ? whole + begin + local : -1;
+    begin = int(int64_t(shorts) * xcd / 8), end = int(int64_t(shorts) * (xcd + 1) / 8);
+    return local < end - begin ? longs + begin + local : -1;
 }
 __host__ __device__ constexpr int64_t xcd_blocks(int64_t slots, int a_tiles) { return (slots / 8 + 2) * 8 * a_tiles; }
 

@@ -36,7 +36,11 @@ __device__ __forceinline__ void load_keys(const int* __restrict__ index, int64_t
     }
 }
 
-// Exclusive sums over the keys' rows (and, TABLES, over their whole runs and rests of the four run lengths): thread i owns the
+// A key's rows as runs of 2^s: the long ones, and whether half a run or less is left
+__device__ __forceinline__ int long_runs(int rows, int s) { return int((unsigned(rows) + (1u << (s - 1)) - 1u) >> s); }
+__device__ __forceinline__ int short_run(int rows, int s) { return rows > long_runs(rows, s) << s; }
+
+// Exclusive sums over the keys' rows (and over their long and short runs of (Q - 1) / 2 run lengths from table0 on): thread i owns the
 // keys [i per, (i + 1) per).  before[]: the sums over all keys before this thread's; total[]: over all.  `part`: Q per wavefront.
 template <int WAVES, int Q, class F>
 __device__ __forceinline__ void key_sums(int keys, int* part, F rows_of, int (&before)[Q], int (&total)[Q], int table0 = 0) {
@@ -48,7 +52,7 @@ __device__ __forceinline__ void key_sums(int keys, int* part, F rows_of, int (&b
 #pragma unroll
         for (int t = 0; t < (Q - 1) / 2; ++t) {
             const int s = nrf::kTileShift0 + table0 + t;
-            sum[1 + 2 * t] += c >> s, sum[2 + 2 * t] += (c & ((1 << s) - 1)) != 0;
+            sum[1 + 2 * t] += long_runs(c, s), sum[2 + 2 * t] += short_run(c, s);
         }
     }
 #pragma unroll
@@ -69,18 +73,22 @@ __device__ __forceinline__ void key_sums(int keys, int* part, F rows_of, int (&b
     __syncthreads();
 }
 
-// Key k's runs of 2^s rows in table `out` (whole ones from `first`, the rest at `last`): a key's first runs and its rest by its
-// own lane, where `mine`; further ones by the wavefront, share `share` of `shares`.  All 64 lanes call it; rows = 0 has none.
+// Key k's runs of 2^s rows in table `out` (long ones from `first`, a short one at `last`): a key's first runs and its short one by
+// its own lane, where `mine`; further ones by the wavefront, share `share` of `shares`.  All 64 lanes call it; rows = 0 has none.
+__device__ __forceinline__ int2 run_of(int s, int k, int off, int rows, int r) {
+    const int left = rows - (r << s);
+    return make_int2(off + (r << s), (left < 1 << s ? left : 1 << s) << 16 | k);
+}
 __device__ __forceinline__ void fill_runs(int2* out, int s, int k, int off, int rows, int first, int last, bool mine, int share, int shares) {
-    const int whole = rows >> s, rest = rows & ((1 << s) - 1), direct = !mine ? 0 : whole < 16 ? whole : 16;
-    for (int r = 0; r < direct; ++r) out[first + r] = make_int2(off + (r << s), 1 << (16 + s) | k);
-    for (unsigned long long many = __ballot(whole > 16); many; many &= many - 1) {
+    const int runs = long_runs(rows, s), direct = !mine ? 0 : runs < 16 ? runs : 16;
+    for (int r = 0; r < direct; ++r) out[first + r] = run_of(s, k, off, rows, r);
+    for (unsigned long long many = __ballot(runs > 16); many; many &= many - 1) {
         const int l = __ffsll((long long)many) - 1;
-        const int w = __builtin_amdgcn_readlane(whole, l), f = __builtin_amdgcn_readlane(first, l),
+        const int w = __builtin_amdgcn_readlane(runs, l), f = __builtin_amdgcn_readlane(first, l), c = __builtin_amdgcn_readlane(rows, l),
                   o = __builtin_amdgcn_readlane(off, l), key = __builtin_amdgcn_readlane(k, l);
-        for (int r = 16 + 64 * share + int(threadIdx.x & 63); r < w; r += 64 * shares) out[f + r] = make_int2(o + (r << s), 1 << (16 + s) | key);
+        for (int r = 16 + 64 * share + int(threadIdx.x & 63); r < w; r += 64 * shares) out[f + r] = run_of(s, key, o, c, r);
     }
-    if (mine && rest) out[last] = make_int2(off + rows - rest, rest << 16 | k);
+    if (mine && short_run(rows, s)) out[last] = run_of(s, k, off, rows, runs);
 }
 constexpr int kSums = 1 + 2 * nrf::kTileTables;
 // counts, offsets and the run tables' lengths; at: this thread's sums before its key k, total: over all keys
@@ -98,7 +106,7 @@ __device__ __forceinline__ void pass_key(int rows, int (&at)[kSums]) {
 #pragma unroll
     for (int t = 0; t < nrf::kTileTables; ++t) {
         const int s = nrf::kTileShift0 + t;
-        at[1 + 2 * t] += rows >> s, at[2 + 2 * t] += (rows & ((1 << s) - 1)) != 0;
+        at[1 + 2 * t] += long_runs(rows, s), at[2 + 2 * t] += short_run(rows, s);
     }
 }
 
@@ -172,7 +180,7 @@ __global__ __launch_bounds__(WAVES * 64) void plan_place_kernel(const int* __res
                 const bool mine = i % kTableShares == share;
                 if (t == 0 && mine && k < keys) write_key(L, plan, E, k, rows, at[0]);
                 fill_runs(out, s, k, at[0], rows, at[1], total[1] + at[2], mine, share, kTableShares);
-                at[0] += rows, at[1] += rows >> s, at[2] += (rows & ((1 << s) - 1)) != 0;
+                at[0] += rows, at[1] += long_runs(rows, s), at[2] += short_run(rows, s);
             }
             if (share == 0 && threadIdx.x == 0) plan[L.runs + 2 * t] = total[1], plan[L.runs + 2 * t + 1] = total[1] + total[2];
             return;

@@ -54,19 +54,19 @@ def test_plan(n, E, kind):
     assert np.array_equal(plan.counts.cpu().numpy(), counts)
     assert np.array_equal(plan.offsets.cpu().numpy(), offsets)
     assert np.array_equal(plan.order.cpu().numpy(), order)
-    # the tile tables: every grouped place, the rows of no expert among them, in exactly one run of one expert, whole runs first
+    # the tile tables: every grouped place, the rows of no expert among them, in exactly one run of one expert; runs of half
+    # the length and less last
     at = expert_ops._up4(E) + expert_ops._up4(E + 1) + expert_ops._up4(n)
     runs = plan.buffer[at:at + 8].view(4, 2).tolist()
     at += 8
     ends = np.concatenate([offsets, [n]])
-    for shift, (whole, count) in zip((5, 6, 7, 8), runs):
-        assert whole == (np.diff(ends) >> shift).sum()
+    for shift, (longs, count) in zip((5, 6, 7, 8), runs):
         assert count == (-(-np.diff(ends) // (1 << shift))).sum() <= (n >> shift) + E + 1
         table = plan.buffer[at:at + 2 * count].view(-1, 2).cpu().numpy().astype(np.int64)
         at += expert_ops._up4(2 * ((n >> shift) + E + 1))
         first, rows, expert = table[:, 0], table[:, 1] >> 16, table[:, 1] & 0xffff
-        assert (rows[:whole] == 1 << shift).all() and (rows > 0).all() and (rows[whole:] < 1 << shift).all()
-        assert (np.diff(first[:whole]) > 0).all() and (np.diff(first[whole:]) > 0).all()
+        assert (rows > 0).all() and (rows <= 1 << shift).all() and (2 * rows[:longs] > 1 << shift).all() and (2 * rows[longs:] <= 1 << shift).all()
+        assert (np.diff(first[:longs]) > 0).all() and (np.diff(first[longs:]) > 0).all()
         grouped = np.argsort(first)
         assert rows.sum() == n and np.array_equal(first[grouped], np.cumsum(rows[grouped]) - rows[grouped])
         assert (first >= ends[expert]).all() and (first + rows <= ends[expert + 1]).all()
