@@ -8,8 +8,8 @@ import ctypes as C
 import torch
 
 from ._lib import NrfError, check, lib
-from .expert_ops import DTYPES
-from .ops import _ptr, _stream
+from .expert_ops import DTYPES, _on, _stream
+from .ops import _ptr
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # steep at 0 (weak directions catch up in five steps), within 0.7 .. 1.2 near 1
 MAX_TENSORS = 32                           # of one nrf_muon_update call
@@ -42,7 +42,7 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, ep
     work, need = _workspace(batch, rows, cols, g.device)
     g = g.contiguous()
     a, b, c = coefficients
-    with torch.cuda.device(g.device):
+    with _on(g.device):
         check(lib().nrf_newton_schulz(_ptr(g), _ptr(out), batch, rows, cols, DTYPES[g.dtype], int(steps), a, b, c, eps,
                                       _ptr(work), need, _stream(g)), "nrf_newton_schulz")
     return out
@@ -80,7 +80,7 @@ def muon_update(params, grads, momentum_buffers, lr: float = 0.02, momentum: flo
         n = len(part[0])
         work, need = _workspace(batch * n, rows, cols, dev)
         arrays = [(C.c_void_p * n)(*[t.data_ptr() for t in ts]) for ts in part]
-        with torch.cuda.device(dev):
+        with _on(dev):
             check(lib().nrf_muon_update(*arrays, n, batch, rows, cols, grad_scale, clip_value, momentum, int(nesterov), lr,
                                         weight_decay, int(steps), a, b, c, eps, _ptr(work), need, _stream(params[0])),
                   "nrf_muon_update")
