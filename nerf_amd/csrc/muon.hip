@@ -62,13 +62,17 @@ __device__ __forceinline__ float element(const SchulzArgs& s, int t, int64_t bas
     }
 }
 template <class T>
-__device__ __forceinline__ void emit(const SchulzArgs& s, int t, int64_t base, unsigned i, float v) {
+__device__ __forceinline__ void emit(const SchulzArgs& s, int t, int64_t base, unsigned i, float v, float old) {   // old: before<T>() of the element
     if constexpr (__is_same(T, OutMuon)) {
-        float* p = static_cast<float*>(s.out[t]) + base;
-        p[i] = __fmaf_rn(-s.rate, v, s.decay * p[i]);
+        (static_cast<float*>(s.out[t]) + base)[i] = __fmaf_rn(-s.rate, v, s.decay * old);
     } else {
         (static_cast<typename Elem<T>::type*>(s.out[t]) + base)[i] = (typename Elem<T>::type)v;
     }
+}
+template <class T>
+__device__ __forceinline__ float before(const SchulzArgs& s, int t, int64_t base, unsigned i) {   // Muon: the parameter
+    if constexpr (__is_same(T, OutMuon)) return (static_cast<const float*>(s.out[t]) + base)[i];
+    else return 0.f;
 }
 // 4096 / max(norm, eps); a norm that is not a number stays one
 __device__ __forceinline__ float start_scale(double sum, float eps) {
@@ -227,14 +231,23 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 2 ? 3 : 4) void schulz_sma
             }
     }
     const bool whole = TALL ? s.cols == 32 : s.rows == 32;   // every lane (row) of the shorter side is there
+    int cols = s.cols;
+    asm volatile("" : "+s"(cols) : : "memory");   // the offsets are computed again, not kept since the loads (Muon: 91 spills)
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
+    for (int j = 0; j < NB; ++j) {
+        float old[16];
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
             const int r = (TALL ? 32 * j : 0) + nrf::acc_row(t, h), q = TALL ? c : 32 * j + c;
-            if ((whole || (TALL ? q < s.cols : r < s.rows)) && (TALL ? r < s.rows : q < s.cols))
-                emit<T>(s, t0, base, r * s.cols + q, v[j][t] * kUnscale);
+            old[t] = before<T>(s, t0, base, (r < s.rows ? r : s.rows - 1) * cols + (q < cols ? q : cols - 1));
         }
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            const int r = (TALL ? 32 * j : 0) + nrf::acc_row(t, h), q = TALL ? c : 32 * j + c;
+            if ((whole || (TALL ? q < cols : r < s.rows)) && (TALL ? r < s.rows : q < cols))
+                emit<T>(s, t0, base, r * cols + q, v[j][t] * kUnscale, old[t]);
+        }
+    }
 }
 
 // ---- larger matrices ----------------------------------------------------------------------------------------------------
@@ -248,6 +261,7 @@ struct LargeShape {
     __host__ __device__ int64_t x_at(int which) const { return which * 2 * x_size(); }
     __host__ __device__ int64_t xt_at(int which) const { return which * 2 * x_size() + x_size(); }
     __host__ __device__ int64_t gram_at() const { return 4 * x_size(); }
+    __device__ float* parts(_Float16* w, int which) const { return reinterpret_cast<float*>(w + x_at(which ^ 1)); }
     __host__ __device__ int64_t poly_at() const { return 4 * x_size() + s_size(); }
 };
 constexpr int kNormBatch = 8;       // elements of a thread at a time, all loaded before the first is used
@@ -341,7 +355,7 @@ __global__ __launch_bounds__(256) void schulz_start_kernel(SchulzArgs s, LargeSh
     }
 }
 
-enum Product { kGram, kPoly, kApply, kLast };
+enum Product { kGram, kPoly, kApply, kLast, kGramPart };
 
 // 64 x 64 or 128 x 128 outputs by four wavefronts
 template <int TT> using SchulzGemm = DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2, 2>;
@@ -358,23 +372,38 @@ __device__ __forceinline__ void store_octet(_Float16* dst, int64_t plane, const 
     *reinterpret_cast<u32x4*>(dst + plane) = lo;
 }
 
+// A TT x TT tile of words {hi, lo} in LDS ([a][b], rows of TT + 1) to rows `row0 ..` and columns `col0 ..` of a matrix of
+// `pitch`: its rows b (TURN) or its rows a, 16 B per lane and plane
+template <int TT, bool TURN>
+__device__ __forceinline__ void write_terms(const unsigned* s_out, _Float16* dst, int64_t plane, int pitch, int row0, int col0) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < TT * TT / 8; i += 256) {
+        const int row = i / (TT / 8), col = i % (TT / 8) * 8;
+        unsigned v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = s_out[TURN ? (col + j) * (TT + 1) + row : row * (TT + 1) + col + j];
+        store_octet(dst + int64_t(row0 + row) * pitch + col0 + col, plane, v);
+    }
+}
+
 // One product of a step: A = X X^T and Q = a I + b A + c A A (symmetric: the tiles on and over the diagonal, each written to
 // both places), X' = Q X (to X' and X'^T; the last step: to the output).  Workgroups are dealt out to the XCDs in turn, so each
 // XCD takes consecutive tiles, which share their operands' rows in its L2.  A finished tile goes through LDS (rows of TT + 1
 // words), so that both orientations are written 16 B per lane: as the accumulators lie, a lane has 4 elements of one
 // orientation and 1 of the other.
 template <class T, int WHAT, int TT>
-__global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, LargeShape L, _Float16* __restrict__ work, int which, int tiles) {
+__global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, LargeShape L, _Float16* __restrict__ work, int which, int tiles, int share, int splits) {
     typedef SchulzGemm<TT> Gemm;
+    constexpr bool kSym = WHAT == kGram || WHAT == kGramPart || WHAT == kPoly, kX = WHAT == kGram || WHAT == kGramPart;   // A or Q; of X X^T
     extern __shared__ __align__(16) char smem[];
-    const int total = int(s.batch) * tiles, share = (total + 7) / 8;
-    const int unit = int(blockIdx.x & 7) * share + int(blockIdx.x >> 3);
-    if (unit >= total) return;
-    const int64_t m = unit / tiles;
+    int unit = int(blockIdx.x & 7) * share + int(blockIdx.x >> 3);
+    if (unit >= int(s.batch) * tiles * splits) return;
+    const int split = unit / tiles % splits;          // of kGramPart: an XCD's units share a stretch of k
+    const int64_t m = unit / (tiles * splits);
     _Float16* w = work + m * L.per_matrix();
     const int tiles_m = L.Mp / TT;
     int ta, tb;
-    if (WHAT == kGram || WHAT == kPoly) {   // tile pairs (ta <= tb), tb-th row has tb + 1
+    if (kSym) {   // tile pairs (ta <= tb), tb-th row has tb + 1
         int left = unit % tiles;
         for (tb = 0; left > tb; ++tb) left -= tb + 1;
         ta = left;
@@ -382,22 +411,32 @@ __global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, Large
         ta = unit % tiles % tiles_m, tb = unit % tiles / tiles_m;
     }
     const int a0 = ta * TT, b0 = tb * TT;
-    const int K = WHAT == kGram ? L.Np : L.Mp;
-    const _Float16* pa = w + (WHAT == kGram ? L.x_at(which) : WHAT == kPoly ? L.gram_at() : L.poly_at());
-    const _Float16* pb = w + (WHAT == kGram ? L.x_at(which) : WHAT == kPoly ? L.gram_at() : L.xt_at(which));
-    const int64_t plane_a = int64_t(L.Mp) * K, plane_b = int64_t(WHAT == kGram || WHAT == kPoly ? L.Mp : L.Np) * K;
+    const int K = kX ? L.Np : L.Mp;
+    const int per = ((K / 64 + splits - 1) / splits) * 64, k0 = split * per < K ? split * per : K, count = K - k0 < per ? K - k0 : per;
+    const _Float16* pa = w + (kX ? L.x_at(which) : WHAT == kPoly ? L.gram_at() : L.poly_at()) + k0;
+    const _Float16* pb = w + (kX ? L.x_at(which) : WHAT == kPoly ? L.gram_at() : L.xt_at(which)) + k0;
+    const int64_t plane_a = int64_t(L.Mp) * K, plane_b = int64_t(kSym ? L.Mp : L.Np) * K;
     Gemm gemm;
     // offsets inside a tile: at most 128 rows of 65536 terms
     gemm.a.start_rows(gemm.wave, gemm.lane, pa + int64_t(a0) * K, plane_a * 2, [&](int row) { return unsigned(row * K) * 2u; });
     gemm.b.start_rows(gemm.wave, gemm.lane, pb + int64_t(b0) * K, plane_b * 2, [&](int row) { return unsigned(row * K) * 2u; });
     f32x4 acc[Gemm::kMA][Gemm::kMB] = {};
-    gemm.run(smem, K, acc);
+    gemm.run(smem, count, acc);
 
     constexpr int kPitch = TT + 1;
     static_assert(TT * kPitch * 4 <= Gemm::kLds, "the tile in LDS");
     unsigned* s_out = reinterpret_cast<unsigned*>(smem);              // [a][b]
     const int c = gemm.lane & 15, q = gemm.lane >> 4, t = int(m / s.per);
-    const int64_t plane = int64_t(L.Mp) * (WHAT == kGram || WHAT == kPoly ? L.Mp : L.Np);
+    const int64_t plane = int64_t(L.Mp) * (kSym ? L.Mp : L.Np);
+    if constexpr (WHAT == kGramPart) {   // a tile [b][a], in place of the next X (see gram_splits)
+        float* part = L.parts(w, which) + (int64_t(split) * tiles + unit % tiles) * (TT * TT);
+#pragma unroll
+        for (int ma = 0; ma < Gemm::kMA; ++ma)
+#pragma unroll
+            for (int mb = 0; mb < Gemm::kMB; ++mb)
+                *reinterpret_cast<f32x4*>(part + (gemm.wave_b() + 16 * mb + c) * TT + gemm.wave_a() + 16 * ma + 4 * q) = acc[ma][mb];
+        return;
+    }
     __syncthreads();
 #pragma unroll
     for (int ma = 0; ma < Gemm::kMA; ++ma)
@@ -430,38 +469,64 @@ __global__ __launch_bounds__(256) void schulz_product_kernel(SchulzArgs s, Large
         }
     __syncthreads();
     if constexpr (WHAT == kLast) {
-        // lanes along the output's rows; what a Muon step reads of the parameters is loaded four ahead
+        // lanes along the output's rows; a Muon step's parameters are loaded sixteen ahead, under no condition
         const bool tall = s.rows > s.cols;
         const int64_t base = (m % s.per) * int64_t(s.rows) * s.cols;
         const int r0 = tall ? b0 : a0, q0 = tall ? a0 : b0;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < TT * TT; i += 256) {
-            const int r = i / TT, col = i % TT;
-            if (r0 + r < s.rows && q0 + col < s.cols)
-                emit<T>(s, t, base, unsigned(r0 + r) * s.cols + q0 + col, __builtin_bit_cast(float, s_out[tall ? col * kPitch + r : r * kPitch + col]));
+        constexpr int kAhead = 16;
+        for (int i0 = 0; i0 < TT * TT; i0 += 256 * kAhead) {
+            float old[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int i = i0 + 256 * u + int(threadIdx.x), r = r0 + i / TT, col = q0 + i % TT;
+                old[u] = before<T>(s, t, base, unsigned(r < s.rows ? r : s.rows - 1) * s.cols + (col < s.cols ? col : s.cols - 1));
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int i = i0 + 256 * u + int(threadIdx.x), r = i / TT, col = i % TT;
+                const float v = __builtin_bit_cast(float, s_out[tall ? col * kPitch + r : r * kPitch + col]);
+                if (r0 + r < s.rows && q0 + col < s.cols) emit<T>(s, t, base, unsigned(r0 + r) * s.cols + q0 + col, v, old[u]);
+            }
         }
     } else {
         _Float16* straight = w + (WHAT == kGram ? L.gram_at() : WHAT == kPoly ? L.poly_at() : L.xt_at(which ^ 1));   // rows b
         _Float16* turned = WHAT == kApply ? w + L.x_at(which ^ 1) : straight;                                        // rows a
         const int pitch_turned = WHAT == kApply ? L.Np : L.Mp;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < TT * TT / 8; i += 256) {
-            const int b = i / (TT / 8), a = i % (TT / 8) * 8;
-            unsigned v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = s_out[(a + j) * kPitch + b];
-            store_octet(straight + int64_t(b0 + b) * L.Mp + a0 + a, plane, v);
-        }
-        if (WHAT == kApply || ta != tb)
-#pragma unroll 4
-            for (int i = threadIdx.x; i < TT * TT / 8; i += 256) {
-                const int a = i / (TT / 8), b = i % (TT / 8) * 8;
-                unsigned v[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = s_out[a * kPitch + b + j];
-                store_octet(turned + int64_t(a0 + a) * pitch_turned + b0 + b, plane, v);
-            }
+        write_terms<TT, true>(s_out, straight, plane, L.Mp, b0, a0);
+        if (WHAT == kApply || ta != tb) write_terms<TT, false>(s_out, turned, plane, pitch_turned, a0, b0);
     }
+}
+
+// A from its parts: one 64 x 64 block of a tile per workgroup
+template <int TT>
+__global__ __launch_bounds__(256) void schulz_join_kernel(int64_t batch, LargeShape L, _Float16* __restrict__ work, int which, int tiles, int splits) {
+    constexpr int kBlocks = TT / 64 * (TT / 64), kPitch = 65;
+    __shared__ unsigned s_out[64 * kPitch];
+    const int tile = blockIdx.x / kBlocks % tiles, block = blockIdx.x % kBlocks;
+    const int64_t m = blockIdx.x / kBlocks / tiles;
+    _Float16* w = work + m * L.per_matrix();
+    int tb = 0, ta = tile;
+    for (; ta > tb; ++tb) ta -= tb + 1;
+    const int a_in = block % (TT / 64) * 64, b_in = block / (TT / 64) * 64, a = a_in + int(threadIdx.x & 15) * 4, row = threadIdx.x >> 4;
+    const float* part = L.parts(w, which) + int64_t(tile) * (TT * TT) + a;
+    f32x4 v[4] = {};
+    for (int i = 0; i < splits; ++i, part += int64_t(tiles) * (TT * TT))
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] += *reinterpret_cast<const f32x4*>(part + (b_in + row + 16 * u) * TT);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        v[u] = v[u] * kUnscale;
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+            unsigned hi, lo;
+            split_pair_h2(v[u][r], v[u][r + 1], hi, lo);
+            unsigned* to = s_out + (a - a_in + r) * kPitch + row + 16 * u;
+            to[0] = __builtin_amdgcn_perm(lo, hi, 0x05040100u), to[kPitch] = __builtin_amdgcn_perm(lo, hi, 0x07060302u);
+        }
+    }
+    __syncthreads();
+    write_terms<64, true>(s_out, w + L.gram_at(), int64_t(L.Mp) * L.Mp, L.Mp, tb * TT + b_in, ta * TT + a_in);
+    if (ta != tb) write_terms<64, false>(s_out, w + L.gram_at(), int64_t(L.Mp) * L.Mp, L.Mp, ta * TT + a_in, tb * TT + b_in);
 }
 
 // no step at all: the scaled matrix itself
@@ -474,7 +539,7 @@ __global__ __launch_bounds__(256) void schulz_copy_kernel(SchulzArgs s, LargeSha
     const int t = int(m / s.per);
     const int64_t base = (m % s.per) * count;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count; i += int64_t(gridDim.x) * 256)
-        emit<T>(s, t, base + i, 0, element<T, true>(s, t, base + i, 0, nullptr) * scale);
+        emit<T>(s, t, base + i, 0, element<T, true>(s, t, base + i, 0, nullptr) * scale, before<T>(s, t, base + i, 0));
 }
 
 bool small_path(int rows, int cols) {
@@ -505,16 +570,18 @@ void launch_small(const SchulzArgs& s, hipStream_t stream) {
 }
 
 template <class T, int WHAT, int TT>
-int launch_tiles(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream) {
+int launch_tiles(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream, int splits = 1) {
     typedef SchulzGemm<TT> Gemm;
     const int m = L.Mp / TT, n = L.Np / TT;
-    const int tiles = WHAT == kGram || WHAT == kPoly ? m * (m + 1) / 2 : m * n;
+    const int tiles = WHAT == kGram || WHAT == kGramPart || WHAT == kPoly ? m * (m + 1) / 2 : m * n;
     auto kernel = &schulz_product_kernel<T, WHAT, TT>;
     if (Gemm::kLds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                   Gemm::kLds) != hipSuccess)
         return NRF_ERR_LAUNCH;
-    const unsigned groups = unsigned((int(s.batch) * tiles + 7) / 8 * 8);
-    kernel<<<groups, 256, Gemm::kLds, stream>>>(s, L, work, which, tiles);
+    // tiles of an XCD: whole matrices, the same for every product, while its 32 CUs have one tile each at most
+    const int64_t whole = (s.batch + 7) / 8 * tiles;
+    const int share = whole <= 32 && splits == 1 ? int(whole) : (int(s.batch) * tiles * splits + 7) / 8;
+    kernel<<<8 * share, 256, Gemm::kLds, stream>>>(s, L, work, which, tiles, share, splits);
     return NRF_OK;
 }
 
@@ -523,8 +590,33 @@ int launch_tiles(const SchulzArgs& s, const LargeShape& L, _Float16* work, int w
 template <class T, int WHAT>
 int launch_product(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream) {
     const int64_t m = L.Mp / 128, n = L.Np / 128;
-    const int64_t tiles = (WHAT == kGram || WHAT == kPoly ? m * (m + 1) / 2 : m * n) * s.batch;
+    const int64_t tiles = (WHAT == kPoly ? m * (m + 1) / 2 : m * n) * s.batch;
     return L.tile == 128 && tiles >= 192 ? launch_tiles<T, WHAT, 128>(s, L, work, which, stream) : launch_tiles<T, WHAT, 64>(s, L, work, which, stream);
+}
+// A long k with few tiles is split, in shares of at least eight steps, until the tiles fill the chip.  The parts lie where the
+// step's new X will: splits m (m + 1) / 2 tiles of fp32 within 8 Mp Np bytes.
+int gram_splits(const SchulzArgs& s, const LargeShape& L) {
+    const int64_t m = L.Mp / L.tile, tiles = m * (m + 1) / 2;
+    int64_t splits = 256 / (tiles * s.batch);
+    if (splits > L.Np / 512) splits = L.Np / 512;
+    const int64_t room = 8 * int64_t(L.Mp) * L.Np / (tiles * L.tile * L.tile * 4);
+    if (splits > room) splits = room;
+    return splits < 2 ? 1 : int(splits);
+}
+template <int TT>
+int launch_gram_parts(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, int splits, hipStream_t stream) {
+    const int st = launch_tiles<Out32, kGramPart, TT>(s, L, work, which, stream, splits);
+    if (st != NRF_OK) return st;
+    const int tiles = L.Mp / TT * (L.Mp / TT + 1) / 2;
+    schulz_join_kernel<TT><<<unsigned(s.batch * tiles * (TT / 64) * (TT / 64)), 256, 0, stream>>>(s.batch, L, work, which, tiles, splits);
+    return NRF_OK;
+}
+int launch_gram(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream) {
+    const int splits = gram_splits(s, L);
+    const int64_t m = L.Mp / 128;
+    if (splits > 1) return L.tile == 128 ? launch_gram_parts<128>(s, L, work, which, splits, stream) : launch_gram_parts<64>(s, L, work, which, splits, stream);
+    return L.tile == 128 && m * (m + 1) / 2 * s.batch >= 192 ? launch_tiles<Out32, kGram, 128>(s, L, work, which, stream)
+                                                             : launch_tiles<Out32, kGram, 64>(s, L, work, which, stream);
 }
 
 template <class T>
@@ -537,7 +629,7 @@ int run_large(const SchulzArgs& s, const LargeShape& L, double* parts, _Float16*
     }
     schulz_start_kernel<T><<<cover, 256, 0, stream>>>(s, L, parts, work);
     for (int k = 0; k < s.steps; ++k) {
-        int st = launch_product<Out32, kGram>(s, L, work, k & 1, stream);   // the output's type matters to kLast alone
+        int st = launch_gram(s, L, work, k & 1, stream);   // the output's type matters to kLast alone
         if (st == NRF_OK) st = launch_product<Out32, kPoly>(s, L, work, k & 1, stream);
         if (st == NRF_OK)
             st = k + 1 < s.steps ? launch_product<Out32, kApply>(s, L, work, k & 1, stream)
