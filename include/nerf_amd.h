@@ -545,8 +545,9 @@ int nrf_expert_linear_backward(const void* grad_y, const void* x, const void* we
  * singular vectors stay.  g, out: (batch, rows, cols) of `dtype`; out may be g.  Arithmetic is fp32-class whatever the type
  * (two fp16 terms per operand, 22 significand bits, fp32 sums; the norm in float64), one rounding at the end.  A matrix with
  * a value that is not finite gives NaN, the others of the batch are untouched by it; a zero matrix gives zeros.
- * eps >= 1e-30, steps <= 16; the iteration over the singular values in [0, 1] must stay within 1.5 (checked on the host).  batch <= 65535
- * (2^24 where the shorter side is <= 32 and the longer <= 128).  The reference has no counterpart: its optimisers are
+ * eps >= 1e-30, steps <= 16; the iteration over the singular values in [0, 1] must stay within 1.5 (checked on the host).
+ * Sides up to 65536; batch up to 2^24 where the shorter side is <= 32 and the longer <= 128, else 65535 and 2^24 / (the
+ * matrix's tiles of 64 x 64, its sides rounded up to 128 each).  Apart from out = g nothing may overlap.  The reference has no counterpart: its optimisers are
  * torch.optim's (src/train/optimizer.py:9-29). */
 int64_t nrf_newton_schulz_workspace_bytes(int64_t batch, int rows, int cols);
 int nrf_newton_schulz(const void* g, void* out, int64_t batch, int rows, int cols, int dtype, int steps, float a, float b, float c,
@@ -555,8 +556,8 @@ int nrf_newton_schulz(const void* g, void* out, int64_t batch, int rows, int col
 /* One Muon step beside nrf_clip_adam, for weight matrices: g = clamp(grad * grad_scale, +-clip_value); momentum = mu momentum + g;
  * u = nesterov ? g + mu momentum : momentum; O = the Newton-Schulz products of u (nrf_newton_schulz);
  * p = (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) O.  params / grads / momentum: HOST arrays of n_tensors <= 32
- * DEVICE pointers, each a contiguous fp32 (batch, rows, cols); params and momentum are updated in place and must not
- * overlap.  workspace: nrf_newton_schulz_workspace_bytes(n_tensors * batch, rows, cols). */
+ * DEVICE pointers, each a contiguous fp32 (batch, rows, cols); params and momentum are updated in place: none of them may
+ * overlap another or a gradient (equal pointers give NRF_ERR_SHAPE).  workspace: nrf_newton_schulz_workspace_bytes(n_tensors * batch, rows, cols). */
 int nrf_muon_update(float* const* params, const float* const* grads, float* const* momentum, int n_tensors, int64_t batch, int rows,
                     int cols, float grad_scale, float clip_value, float mu, int nesterov, float lr, float weight_decay, int steps,
                     float a, float b, float c, float eps, void* workspace, int64_t workspace_bytes, nrf_stream_t stream);

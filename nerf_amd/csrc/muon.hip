@@ -171,7 +171,7 @@ __device__ __forceinline__ Frag turn_block(const Frag& f, unsigned* s_turn, int 
 }
 
 template <class T, int NB, bool TALL>
-__global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 2 ? 3 : 4) void schulz_small_kernel(SchulzArgs s) {
+__global__ __launch_bounds__(256, NB == 1 ? 4 : (NB == 2 ? 4 : 3) - __is_same(T, OutMuon)) void schulz_small_kernel(SchulzArgs s) {
     __shared__ __align__(16) unsigned s_all[4][32 * kTurnPitch];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t m = int64_t(blockIdx.x) * 4 + wave;
@@ -203,38 +203,11 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 2 ? 3 : 4) void schulz_sma
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
     const float scale = start_scale(sum, s.eps);
-    Frag here[NB], turned[NB];                     // of X_j and Y_j for a wide matrix, of Y_j and X_j for a tall one
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        v[j] = v[j] * scale;
-        here[j] = split_block(v[j]);
-        turned[j] = turn_block(here[j], s_turn, c, h);
-    }
-    for (int k = 0; k < s.steps; ++k) {
-        f32x16 acc = {};
-#pragma unroll
-        for (int j = 0; j < NB; ++j) acc = TALL ? product(here[j], here[j], acc) : product(turned[j], turned[j], acc);
-        const f32x16 gram = acc * kUnscale;
-        acc = square(gram, split_block(gram));
-        // Q without the scale (the matrix cores read subnormal terms: 2^-25 off at most), so that Q X has X's
-        f32x16 poly = (s.b * kUnscale) * gram + (s.c * kUnscale * kUnscale) * acc;
-#pragma unroll
-        for (int t = 0; t < 16; ++t) poly[t] += nrf::acc_row(t, h) == c ? s.a : 0.f;
-        const Frag fq = split_block(poly);
-#pragma unroll
-        for (int j = 0; j < NB; ++j) v[j] = TALL ? product(turned[j], fq, (f32x16){}) : product(fq, here[j], (f32x16){});
-        if (k + 1 < s.steps)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                here[j] = split_block(v[j]);
-                turned[j] = turn_block(here[j], s_turn, c, h);
-            }
-    }
-    const bool whole = TALL ? s.cols == 32 : s.rows == 32;   // every lane (row) of the shorter side is there
-    int cols = s.cols;
-    asm volatile("" : "+s"(cols) : : "memory");   // the offsets are computed again, not kept since the loads (Muon: 91 spills)
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
+
+    auto write = [&](int j, const f32x16& o) {     // the block's values, still at the scale
+        int cols = s.cols;
+        asm volatile("" : "+s"(cols) : : "memory");   // the offsets are computed again, not kept since the loads (Muon: 91 spills)
+        const bool whole = TALL ? cols == 32 : s.rows == 32;   // every lane (row) of the shorter side is there
         float old[16];
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
@@ -245,7 +218,38 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : NB == 2 ? 3 : 4) void schulz_sma
         for (int t = 0; t < 16; ++t) {
             const int r = (TALL ? 32 * j : 0) + nrf::acc_row(t, h), q = TALL ? c : 32 * j + c;
             if ((whole || (TALL ? q < cols : r < s.rows)) && (TALL ? r < s.rows : q < cols))
-                emit<T>(s, t0, base, r * cols + q, v[j][t] * kUnscale, old[t]);
+                emit<T>(s, t0, base, r * cols + q, o[t] * kUnscale, old[t]);
+        }
+    };
+    Frag here[NB];                                 // of X_j for a wide matrix, of Y_j for a tall one: all that a step keeps
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        if (s.steps == 0) write(j, v[j] * scale);
+        else here[j] = split_block(v[j] * scale);
+    }
+    auto apply = [&](int j, const Frag& fq) {
+        return TALL ? product(turn_block(here[j], s_turn, c, h), fq, (f32x16){}) : product(fq, here[j], (f32x16){});
+    };
+    for (int k = 1; k <= s.steps; ++k) {
+        f32x16 acc = {};
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const Frag f = TALL ? here[j] : turn_block(here[j], s_turn, c, h);
+            acc = product(f, f, acc);
+        }
+        const f32x16 gram = acc * kUnscale;
+        acc = square(gram, split_block(gram));
+        // Q without the scale (the matrix cores read subnormal terms: 2^-25 off at most), so that Q X has X's
+        f32x16 poly = (s.b * kUnscale) * gram + (s.c * kUnscale * kUnscale) * acc;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) poly[t] += nrf::acc_row(t, h) == c ? s.a : 0.f;
+        const Frag fq = split_block(poly);
+        if (k < s.steps) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) here[j] = split_block(apply(j, fq));
+        } else {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) write(j, apply(j, fq));
         }
     }
 }
@@ -721,6 +725,11 @@ NRF_EXPORT int nrf_muon_update(float* const* params, const float* const* grads, 
             return NRF_ERR_ALIGN;
         s.g[i] = grads[i], s.out[i] = params[i], s.mom[i] = momentum[i];
     }
+    for (int i = 0; i < n_tensors; ++i)      // the same tensor twice, or as gradient and momentum: read while it is written
+        for (int j = 0; j < n_tensors; ++j)
+            if (params[i] == momentum[j] || params[i] == grads[j] || momentum[i] == grads[j] ||
+                (i != j && (params[i] == params[j] || momentum[i] == momentum[j])))
+                return NRF_ERR_SHAPE;
     s.batch = batch * n_tensors, s.per = int(batch), s.rows = rows, s.cols = cols, s.steps = steps, s.nesterov = nesterov != 0;
     s.a = a, s.b = b, s.c = c, s.eps = eps, s.grad_scale = grad_scale, s.clip = clip_value, s.mu = mu;
     s.decay = float(1.0 - double(lr) * double(weight_decay));

@@ -19,7 +19,7 @@ def _workspace(batch: int, rows: int, cols: int, device):
     need = lib().nrf_newton_schulz_workspace_bytes(batch, rows, cols)
     if need < 0:
         raise NrfError(f"{batch} matrices of {rows} x {cols}: sides of 1 to 65536 and up to 65535 matrices are supported "
-                       "(2^24 up to 32 x 128)")
+                       "(2^24 up to 32 x 128), 2^24 tiles of 64 x 64 in all")
     return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
 
 
@@ -71,6 +71,9 @@ def muon_update(params, grads, momentum_buffers, lr: float = 0.02, momentum: flo
                 raise NrfError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}, want float32 {tuple(shape)} on {dev}")
             if name != "grad" and not t.is_contiguous():
                 raise NrfError(f"{name}: expected a contiguous tensor (it is updated in place)")
+    written = [t.data_ptr() for t in (*params, *momentum_buffers)]
+    if shape.numel() and len({*written, *(g.data_ptr() for g in grads)}) < len(written) + len({g.data_ptr() for g in grads}):
+        raise NrfError("muon_update: a tensor is given twice (each parameter and momentum buffer is updated in place)")
     grads = [g.contiguous() for g in grads]
     rows, cols = shape[-2:]
     batch = shape[0] if len(shape) == 3 else 1

@@ -214,6 +214,37 @@ def test_muon_on_a_side_stream_and_in_a_graph(shape):
     assert torch.equal(p, want_p) and torch.equal(m, want_m)
 
 
+@pytest.mark.parametrize("shape", [(1, 256, 8192), (3, 64, 4096), (2, 1000, 70), (1, 4500, 129), (1, 640, 1152), (1, 33, 40000)], ids=str)
+def test_long_sums_are_split(shape):
+    """few tiles and a long k: A = X X^T from parts"""
+    g = gradient(*shape, seed=sum(shape))
+    got, want = newton_schulz(g.to(DEV)), definition(g)
+    off, most = norm(got.double().cpu() - want), bound(g, want, torch.float32)
+    assert (off <= most).all(), (off / most).max()
+    assert torch.equal(got, newton_schulz(g.to(DEV)))
+
+
+def test_planes_of_more_than_2_gib():
+    """One non-zero per row, in columns of their own: every singular value goes its own way, x -> a x + b x^3 + c x^5.  A plane of
+    X takes 2.2 GiB, both 4.3: offsets past 32 bits.  Off by the output's rounding and the floor of the terms (no sums: each
+    has one addend)."""
+    m, n = 16450, 65500
+    at = (torch.arange(m) * 65123 + 77) % n
+    assert at.unique().numel() == m
+    s = torch.rand(m, generator=torch.Generator().manual_seed(1)) + 0.5
+    g = torch.zeros(m, n, dtype=torch.bfloat16, device=DEV)
+    rows = torch.arange(m, device=DEV)
+    g[rows, at.to(DEV)] = s.bfloat16().to(DEV)
+    x = s.bfloat16().double()
+    x = x / x.square().sum().sqrt()
+    want = ABC[0] * x + ABC[1] * x ** 3 + ABC[2] * x ** 5
+    newton_schulz(g, steps=1, out=g)
+    got = g[rows, at.to(DEV)].double().cpu()
+    assert ((got - want).abs() <= 2.0 ** -8 * want + 2.0 ** -20 * want + 4 * 2.0 ** -37).all()
+    g[rows, at.to(DEV)] = 0
+    assert not bool(g.any())
+
+
 def test_refusals():
     E = muon_ops.NrfError
     g = torch.zeros(2, 8, 8, device=DEV)
@@ -225,6 +256,10 @@ def test_refusals():
         with pytest.raises(E):
             newton_schulz(g, **kw)
     for args in ((g, g[0], g), (g, g.bfloat16(), g), (g.cpu(), g, g), (g.transpose(1, 2), g, g), ([g], [g, g], [g]), (g[0, 0], g[0, 0], g[0, 0])):
+        with pytest.raises(E):
+            muon_update(*args)
+    h, k = torch.zeros_like(g), torch.zeros_like(g)
+    for args in ((g, h, g), (g, g, h), (g, h, h), ([g, g], [h, h], [k, k.clone()]), ([g, k], [h, h], [k, h.clone()])):
         with pytest.raises(E):
             muon_update(*args)
     for kw in (dict(clip_value=0.0), dict(momentum=1.0), dict(steps=99)):

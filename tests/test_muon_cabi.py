@@ -15,6 +15,9 @@ def test_sizes():
     assert f(4096, 32, 63) == 0 and f(4096, 128, 32) == 0 and f(1, 33, 33) > 0 and f(1, 32, 129) > 0
     assert f(1, 0, 4) == -1 and f(1, 4, 65537) == -1 and f(-1, 4, 4) == -1 and f(65536, 64, 64) == -1
     assert f((1 << 24) + 1, 4, 4) == -1
+    assert f(16, 65536, 65536) > 0 and f(17, 65536, 65536) == -1         # 2^24 tiles
+    # two terms of 16 bits for X, X^T, both twice, and for A and Q: no size that 32 bits would cut
+    assert f(1, 16512, 65536) >= 16 * 16512 * 65536 + 8 * 16512 ** 2
 
 
 def test_newton_schulz_refuses_on_the_host():
@@ -43,6 +46,10 @@ def test_muon_update_refuses_on_the_host():
     assert call(params=None) == -1 and call(grads=null) == -1 and call(work=None) == -1
     assert call(size=100) == -4 and call(mom=bad) == -5
     assert call(n=0) == 0 and call(batch=0) == 0
+    a, b, c = ((C.c_void_p * 2)(x, y) for x, y in ((64, 128), (192, 256), (320, 384)))
+    for params, grads, mom in ((a, b, a), (a, a, c), (a, b, b), ((C.c_void_p * 2)(64, 64), b, c), (a, b, (C.c_void_p * 2)(320, 320)),
+                               (a, b, (C.c_void_p * 2)(320, 64))):
+        assert call(params=params, grads=grads, mom=mom, n=2) == -2      # a tensor twice
 
 
 def test_cpu_tensors_are_refused():
