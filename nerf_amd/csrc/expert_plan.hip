@@ -73,20 +73,23 @@ __device__ __forceinline__ void key_sums(int keys, int* part, F rows_of, int (&b
     __syncthreads();
 }
 
-// Key k's runs of 2^s rows in table `out` (long ones from `first`, a short one at `last`): a key's first runs and its short one by
-// its own lane, where `mine`; further ones by the wavefront, share `share` of `shares`.  All 64 lanes call it; rows = 0 has none.
+// Key k's runs of 2^s rows in table `out` (long ones from `first`, a short one at `last`), where `mine`: the first runs and the
+// short one by the key's own lane, further ones by the wavefront; of a key of more than kShared runs, where it is not alone,
+// share `share` of `shares`.  All 64 lanes call it; rows = 0 has none.
 __device__ __forceinline__ int2 run_of(int s, int k, int off, int rows, int r) {
     const int left = rows - (r << s);
     return make_int2(off + (r << s), (left < 1 << s ? left : 1 << s) << 16 | k);
 }
+constexpr int kShared = 1024;
 __device__ __forceinline__ void fill_runs(int2* out, int s, int k, int off, int rows, int first, int last, bool mine, int share, int shares) {
     const int runs = long_runs(rows, s), direct = !mine ? 0 : runs < 16 ? runs : 16;
     for (int r = 0; r < direct; ++r) out[first + r] = run_of(s, k, off, rows, r);
-    for (unsigned long long many = __ballot(runs > 16); many; many &= many - 1) {
+    for (unsigned long long many = __ballot(runs > 16 && (mine || runs > kShared)); many; many &= many - 1) {
         const int l = __ffsll((long long)many) - 1;
         const int w = __builtin_amdgcn_readlane(runs, l), f = __builtin_amdgcn_readlane(first, l), c = __builtin_amdgcn_readlane(rows, l),
                   o = __builtin_amdgcn_readlane(off, l), key = __builtin_amdgcn_readlane(k, l);
-        for (int r = 16 + 64 * share + int(threadIdx.x & 63); r < w; r += 64 * shares) out[f + r] = run_of(s, key, o, c, r);
+        const int from = w > kShared ? share : 0, step = w > kShared ? shares : 1;
+        for (int r = 16 + 64 * from + int(threadIdx.x & 63); r < w; r += 64 * step) out[f + r] = run_of(s, key, o, c, r);
     }
     if (mine && short_run(rows, s)) out[last] = run_of(s, k, off, rows, runs);
 }
@@ -153,7 +156,7 @@ __global__ __launch_bounds__(1024) void plan_chunks_kernel(int* __restrict__ his
 
 // Workgroups 0 .. kTableBlocks - 1: the run tables, kTableShares for each table; table 0's also write counts and offsets.  Those
 // behind them: the walk.  SINGLE: one workgroup does it all.
-constexpr int kTableShares = 8, kTableBlocks = nrf::kTileTables * kTableShares;
+constexpr int kTableShares = 2, kTableBlocks = nrf::kTileTables * kTableShares;
 template <int WAVES, bool SINGLE>
 __global__ __launch_bounds__(WAVES * 64) void plan_place_kernel(const int* __restrict__ index, int64_t n, int E, int64_t chunk,
                                                                 const int* __restrict__ hist, const int* __restrict__ totals,
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(WAVES * 64) void plan_place_kernel(const int* __res
 }
 
 int64_t plan_chunk(int64_t n) {
-    int64_t chunk = (n + 223) / 224;          // with the tables' 32, one workgroup per CU; a counter of a chunk has 16 bits
+    int64_t chunk = (n + 247) / 248;          // with the tables' 8, one workgroup per CU; a counter of a chunk has 16 bits
     if (chunk < 2048) chunk = 2048;
     return chunk > 32768 ? 32768 : chunk;
 }
@@ -344,7 +347,10 @@ NRF_EXPORT int nrf_expert_plan(const int32_t* index, int64_t n_rows, int num_exp
         return NRF_ERR_LAUNCH;
     plan_hist_kernel<<<dim3(unsigned(chunks)), 512, hist_lds, stream>>>(index, n_rows, E, chunk, hist);
     plan_chunks_kernel<<<dim3(unsigned(E / 64 + 1)), 1024, 0, stream>>>(hist, int(chunks), E, totals);
-    const int st = wide ? launch_place<2, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream)
-                        : launch_place<8, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream);
+    // sixteen wavefronts hide more of a long chunk's latency than their counters cost (2 M rows, 4096 experts: 22.7 us for 24.5;
+    // 262 k rows: 12.7 for 10.4)
+    const int st = wide            ? launch_place<2, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream)
+                   : chunk >= 6000 ? launch_place<16, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream)
+                                   : launch_place<8, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream);
     return st != NRF_OK ? st : nrf_launch_status();
 }

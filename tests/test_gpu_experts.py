@@ -72,6 +72,11 @@ def test_plan(n, E, kind):
         assert (first >= ends[expert]).all() and (first + rows <= ends[expert + 1]).all()
 
 
+@pytest.mark.parametrize("n,E,kind", [(1600009, 4096, "outside"), (2000003, 70, "skew"), (9000011, 300, "skew"), (9000011, 2, "one")])
+def test_plan_of_long_chunks(n, E, kind):
+    test_plan(n, E, kind)
+
+
 @pytest.mark.parametrize("kind", ["one", "none"])
 @pytest.mark.parametrize("n", [130, 20000])
 def test_plan_of_one_or_no_expert(n, kind):
