@@ -421,6 +421,18 @@ __global__ __launch_bounds__(512) void expert_wide_rows_kernel(ExpertArgs g, int
     else wide_rows_tile<T, FORM, 64>(g, smem, a0, b_count, expert, order);
 }
 
+// The expert with the `rank`-th most rows (of at most 64; equal ones by number).  A tile of dW takes as long as its expert has
+// rows, and the longest tiles have to begin first: begun by number, the CUs of 16 uneven experts were busy 67% of the time.
+__device__ __forceinline__ int expert_of_rank(const int* counts, int E, int rank) {
+    const int lane = threadIdx.x & 63, mine = lane < E ? counts[lane] : -1;
+    int above = 0;
+    for (int e = 0; e < E; ++e) {
+        const int other = __builtin_amdgcn_readlane(mine, e);
+        above += other > mine || (other == mine && e < lane);
+    }
+    return __ffsll((long long)__ballot(lane < E && above == rank)) - 1;
+}
+
 // dW: 256 input columns x 128 output columns, k the expert's rows through the list of them in LDS, kListRows at a time.
 constexpr int kListRows = 4096;
 template <class T> struct WideDw {
@@ -448,6 +460,7 @@ __global__ __launch_bounds__(512) void expert_wide_dw_kernel(ExpertArgs g, int a
         expert = (local * 8 + xcd) / tiles, at = (local * 8 + xcd) % tiles;
     }
     if (expert >= g.E) return;
+    if (g.E <= 64) expert = expert_of_rank(g.plan, g.E, expert);
     const int split = at / (a_tiles * b_tiles), tile = at % (a_tiles * b_tiles);
     const int a0 = tile % a_tiles * W::kA, b0 = tile / a_tiles * W::kB;
     const int rows = g.plan[expert], per = ((rows + g.splits - 1) / g.splits + 63) / 64 * 64;
