@@ -13,8 +13,9 @@
 // |A| <= 1.6, |Q| <= 8 for the coefficients the entry points admit) below fp16's 65504.  |G|_F is summed in float64.
 //
 // Two paths, by the shorter side M and the longer side N:
-//   M <= 32, N <= 128   one wavefront per matrix, everything in registers (schulz_small_kernel);
-//   otherwise           the matrices' terms in the workspace, three launches per step (schulz_product_kernel).
+//   M <= 32, N <= 128                       one wavefront per matrix, everything in registers (schulz_small_kernel);
+//   M <= 64, N <= 544 and M <= 128, N <= 160  one workgroup per matrix, everything in LDS (schulz_block_kernel);
+//   otherwise                               the matrices' terms in the workspace, three launches per step (schulz_product_kernel).
 #include "dma_gemm.h"
 #include "split2h.h"
 
@@ -250,6 +251,178 @@ __global__ __launch_bounds__(256, NB == 1 ? 4 : (NB == 2 ? 4 : 3) - __is_same(T,
         } else {
 #pragma unroll
             for (int j = 0; j < NB; ++j) write(j, apply(j, fq));
+        }
+    }
+}
+
+// ---- one workgroup per matrix -------------------------------------------------------------------------------------------
+// X, A and Q stay in LDS as their terms, rows padded by 16 B: X [2][16 MB][Np] and one square [2][16 MB][16 MB], A and then Q.  Only
+// X itself is kept: A = X X^T reads its rows (k along them), X' = Q X its columns, turned on the way by ds_read_b64_tr_b16.  Eight
+// wavefronts; a tile of A and of A^2 is one wavefront's, which so adds up Q from its own sums; a wavefront writes X' over the
+// 16 columns that it alone read.  What bounds one matrix is the chain of a step's four phases on one CU; its 17 launches through
+// the tiles below are worse at every size: 33 x 48 60 -> 16 us, 92 x 112 66 -> 55, 64 x 300 65 -> 40, 64 x 544 74 -> 66; 2000 of
+// 64 x 64 305 -> 95, 1000 of 128 x 160 862 -> 317.
+constexpr int kBlockWaves = 8, kLdsBytes = 160 * 1024;
+struct BlockShape {
+    int Np, pitch, square, bytes;                  // pitch of X's rows, of the square's, LDS in all; in bytes
+    __host__ __device__ BlockShape(int N, int MB) : Np((N + 31) / 32 * 32), pitch(0), square(MB * 32 + 16), bytes(0) {
+        pitch = Np * 2 + 16;
+        bytes = 2 * 16 * MB * (pitch + square);
+    }
+};
+__device__ __forceinline__ u32x4 block_rows(const char* plane, int pitch, int row, int k) {   // lane (c, q): row + c, k + 8 q ..
+    const int c = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
+    return *reinterpret_cast<const u32x4*>(plane + (row + c) * pitch + (k + 8 * q) * 2);
+}
+__device__ __forceinline__ u32x4 block_cols(const char* plane, int pitch, int col, int k) {   // lane (c, q): col + c, k + 8 q ..
+    const int c = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
+    s16x4_g part[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+        part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4_g*)(plane + (k + 8 * q + 4 * u + (c >> 2)) * pitch + col * 2 + (c & 3) * 8));
+    return __builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ f32x4 product16(const u32x4 (&a)[2], const u32x4 (&b)[2], f32x4 c) {
+    c = mfma_dma<false>(a[0], b[1], c);
+    c = mfma_dma<false>(a[1], b[0], c);
+    return mfma_dma<false>(a[0], b[0], c);
+}
+__device__ __forceinline__ void block_store(char* at, int plane, const f32x4& v) {
+    unsigned h0, l0, h1, l1;
+    split_pair_h2(v[0], v[1], h0, l0);
+    split_pair_h2(v[2], v[3], h1, l1);
+    *reinterpret_cast<u32x2*>(at) = (u32x2){h0, h1};
+    *reinterpret_cast<u32x2*>(at + plane) = (u32x2){l0, l1};
+}
+
+template <class T, int MB>
+__global__ __launch_bounds__(512) void schulz_block_kernel(SchulzArgs s, BlockShape L, unsigned by_cols) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr int kI = MB * MB / kBlockWaves, kAhead = 8;      // tiles of A a wavefront sums
+    const int64_t m = blockIdx.x;
+    const int t = int(m / s.per), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
+    const int count = s.rows * s.cols;
+    const int64_t base = (m % s.per) * int64_t(count);
+    const bool tall = s.rows > s.cols;
+    const int M = tall ? s.cols : s.rows, N = tall ? s.rows : s.cols;
+    const int plane_x = 16 * MB * L.pitch, plane_s = 16 * MB * L.square;
+    char *xs = smem, *sq = smem + 2 * plane_x;
+
+    for (int i = threadIdx.x * 16; i < 2 * plane_x; i += 512 * 16) *reinterpret_cast<u32x4*>(xs + i) = (u32x4){0, 0, 0, 0};
+    double sum = 0.0;
+    for (int i0 = threadIdx.x; i0 < count; i0 += 512 * kAhead) {
+        float v[kAhead], mom[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + 512 * u;
+            v[u] = element<T, false>(s, t, base, i < count ? i : count - 1, mom + u);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (i0 + 512 * u < count) {
+                if constexpr (__is_same(T, OutMuon)) (s.mom[t] + base)[unsigned(i0 + 512 * u)] = mom[u];
+                sum = __builtin_fma(double(v[u]), double(v[u]), sum);
+            }
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+    double* s_sum = reinterpret_cast<double*>(sq);
+    if ((threadIdx.x & 63) == 0) s_sum[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < kBlockWaves; ++w) sum += s_sum[w];
+    const float scale = start_scale(sum, s.eps);
+    // a second time (from the L2; a thread's own elements, as it left the momentum)
+    for (int i0 = threadIdx.x; i0 < count; i0 += 512 * kAhead) {
+        float v[kAhead], old[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + 512 * u < count ? i0 + 512 * u : count - 1;
+            v[u] = element<T, true>(s, t, base, i, nullptr) * scale;
+            old[u] = s.steps == 0 ? before<T>(s, t, base, i) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + 512 * u;
+            if (i >= count) continue;
+            const int r = by_cols ? int(__umulhi(i, by_cols)) : i, col = i - r * s.cols;
+            unsigned hi, lo;
+            split_pair_h2(v[u], 0.f, hi, lo);
+            char* at = xs + (tall ? col : r) * L.pitch + (tall ? r : col) * 2;
+            *reinterpret_cast<unsigned short*>(at) = (unsigned short)hi;
+            *reinterpret_cast<unsigned short*>(at + plane_x) = (unsigned short)lo;
+            if (s.steps == 0) emit<T>(s, t, base, i, v[u] * kUnscale, old[u]);
+        }
+    }
+    const int j = wave / (MB / kI), first = wave % (MB / kI) * kI;   // rows 16 j .. of A, columns 16 first ..
+    for (int k = 1; k <= s.steps; ++k) {
+        __syncthreads();
+        f32x4 gram[kI] = {}, v[kI] = {};
+        for (int n = 0; n < L.Np; n += 32) {
+            const u32x4 b[2] = {block_rows(xs, L.pitch, 16 * j, n), block_rows(xs + plane_x, L.pitch, 16 * j, n)};
+#pragma unroll
+            for (int i = 0; i < kI; ++i) {
+                const u32x4 a[2] = {block_rows(xs, L.pitch, 16 * (first + i), n), block_rows(xs + plane_x, L.pitch, 16 * (first + i), n)};
+                gram[i] = product16(a, b, gram[i]);
+            }
+        }
+        char* mine = sq + (16 * j + c) * L.square + (16 * first + 4 * q) * 2;
+#pragma unroll
+        for (int i = 0; i < kI; ++i) {
+            gram[i] = gram[i] * kUnscale;
+            block_store(mine + 32 * i, plane_s, gram[i]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 16 * MB; n += 32) {
+            const u32x4 b[2] = {block_rows(sq, L.square, 16 * j, n), block_rows(sq + plane_s, L.square, 16 * j, n)};
+#pragma unroll
+            for (int i = 0; i < kI; ++i) {
+                const u32x4 a[2] = {block_rows(sq, L.square, 16 * (first + i), n), block_rows(sq + plane_s, L.square, 16 * (first + i), n)};
+                v[i] = product16(a, b, v[i]);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kI; ++i) {                             // Q without the scale, as in schulz_small_kernel
+            f32x4 poly = (s.b * kUnscale) * gram[i] + (s.c * kUnscale * kUnscale) * v[i];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) poly[r] += 16 * (first + i) + 4 * q + r == 16 * j + c ? s.a : 0.f;
+            block_store(mine + 32 * i, plane_s, poly);
+        }
+        __syncthreads();
+        for (int n = 16 * wave; n < N; n += 16 * kBlockWaves) {
+            u32x4 x[MB / 2][2];
+#pragma unroll
+            for (int kk = 0; kk < MB / 2; ++kk)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) x[kk][p] = block_cols(xs + p * plane_x, L.pitch, n, 32 * kk);
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                f32x4 o = {};
+#pragma unroll
+                for (int kk = 0; kk < MB / 2; ++kk) {
+                    const u32x4 b[2] = {block_rows(sq, L.square, 16 * i, 32 * kk), block_rows(sq + plane_s, L.square, 16 * i, 32 * kk)};
+                    o = product16(x[kk], b, o);
+                }
+                const int row = 16 * i + c, col = n + 4 * q;       // X'[row][col ..]
+                if (k < s.steps) {
+                    block_store(xs + row * L.pitch + col * 2, plane_x, o);
+                } else {
+                    unsigned at[4];
+                    float old[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const unsigned y = row < M ? row : M - 1, x = col + r < N ? col + r : N - 1;
+                        at[r] = tall ? x * s.cols + y : y * s.cols + x;
+                        old[r] = before<T>(s, t, base, at[r]);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (row < M && col + r < N) emit<T>(s, t, base, at[r], o[r] * kUnscale, old[r]);
+                }
+            }
         }
     }
 }
@@ -551,6 +724,14 @@ bool small_path(int rows, int cols) {
     return lo <= 32 && hi <= 128;
 }
 
+// the row blocks of the one-workgroup kernel that takes a matrix, 0 for none
+int block_path(int rows, int cols) {
+    const int lo = rows < cols ? rows : cols, hi = rows < cols ? cols : rows;
+    for (int MB = 4; MB <= 8; MB += 4)
+        if (lo <= 16 * MB && hi <= 1024 && BlockShape(hi, MB).bytes <= kLdsBytes) return MB;
+    return 0;
+}
+
 LargeShape large_shape(int rows, int cols) {
     LargeShape L;
     L.M = rows < cols ? rows : cols, L.N = rows < cols ? cols : rows;
@@ -571,6 +752,18 @@ void launch_small(const SchulzArgs& s, hipStream_t stream) {
     if (longer <= 32) schulz_small_kernel<T, 1, TALL><<<grid, 256, 0, stream>>>(s);
     else if (longer <= 64) schulz_small_kernel<T, 2, TALL><<<grid, 256, 0, stream>>>(s);
     else schulz_small_kernel<T, 4, TALL><<<grid, 256, 0, stream>>>(s);
+}
+
+template <class T, int MB>
+int launch_block(const SchulzArgs& s, hipStream_t stream) {
+    const BlockShape L(s.rows < s.cols ? s.cols : s.rows, MB);
+    auto kernel = &schulz_block_kernel<T, MB>;
+    if (L.bytes > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                               kLdsBytes) != hipSuccess)
+        return NRF_ERR_LAUNCH;
+    // i / cols = i * by_cols >> 32 for i < 2^32 / cols (an element's index is below 2^16); 0 for a single column
+    kernel<<<unsigned(s.batch), 512, L.bytes, stream>>>(s, L, s.cols == 1 ? 0u : unsigned((int64_t(1) << 32) / s.cols + 1));
+    return NRF_OK;
 }
 
 template <class T, int WHAT, int TT>
@@ -651,6 +844,10 @@ int run(const SchulzArgs& s, void* workspace, hipStream_t stream) {
         else launch_small<T, false>(s, stream);
         return nrf_launch_status();
     }
+    if (const int MB = block_path(s.rows, s.cols)) {
+        const int st = MB == 4 ? launch_block<T, 4>(s, stream) : launch_block<T, 8>(s, stream);
+        return st != NRF_OK ? st : nrf_launch_status();
+    }
     const LargeShape L = large_shape(s.rows, s.cols);
     double* parts = static_cast<double*>(workspace);
     _Float16* work = reinterpret_cast<_Float16*>(parts + ((s.batch * L.chunks + 31) & ~int64_t(31)));
@@ -661,6 +858,7 @@ int run(const SchulzArgs& s, void* workspace, hipStream_t stream) {
 bool schulz_shape_ok(int64_t batch, int rows, int cols) {
     if (batch < 0 || rows < 1 || cols < 1 || rows > 65536 || cols > 65536) return false;
     if (small_path(rows, cols)) return batch <= int64_t(1) << 24;
+    if (block_path(rows, cols)) return batch <= int64_t(1) << 24;
     const LargeShape L = large_shape(rows, cols);
     return batch <= 65535 && batch * (int64_t(L.Mp / 64) * (L.Np / 64)) <= int64_t(1) << 24;
 }
@@ -682,7 +880,7 @@ bool coefficients_ok(int steps, float a, float b, float c) {
 
 NRF_EXPORT int64_t nrf_newton_schulz_workspace_bytes(int64_t batch, int rows, int cols) {
     if (!schulz_shape_ok(batch, rows, cols)) return -1;
-    if (small_path(rows, cols)) return 0;
+    if (small_path(rows, cols) || block_path(rows, cols)) return 0;
     const LargeShape L = large_shape(rows, cols);
     return ((batch * L.chunks + 31) & ~int64_t(31)) * 8 + batch * L.per_matrix() * 2;
 }

@@ -12,8 +12,9 @@ ABC = (3.4445, -4.7750, 2.0315)
 def test_sizes():
     L = _lib.lib()
     f = L.nrf_newton_schulz_workspace_bytes
-    assert f(4096, 32, 63) == 0 and f(4096, 128, 32) == 0 and f(1, 33, 33) > 0 and f(1, 32, 129) > 0
-    assert f(1, 0, 4) == -1 and f(1, 4, 65537) == -1 and f(-1, 4, 4) == -1 and f(65536, 64, 64) == -1
+    assert f(4096, 32, 63) == 0 and f(4096, 128, 32) == 0 and f(1, 64, 544) == 0 and f(1, 160, 128) == 0     # in registers or LDS
+    assert f(1, 64, 545) > 0 and f(1, 65, 161) > 0 and f(1, 129, 129) > 0
+    assert f(1, 0, 4) == -1 and f(1, 4, 65537) == -1 and f(-1, 4, 4) == -1 and f(65536, 200, 200) == -1 and f((1 << 24) + 1, 64, 64) == -1
     assert f((1 << 24) + 1, 4, 4) == -1
     assert f(16, 65536, 65536) > 0 and f(17, 65536, 65536) == -1         # 2^24 tiles
     # two terms of 16 bits for X, X^T, both twice, and for A and Q: no size that 32 bits would cut
@@ -23,7 +24,7 @@ def test_sizes():
 def test_newton_schulz_refuses_on_the_host():
     L = _lib.lib()
     p, odd = C.c_void_p(64), C.c_void_p(66)          # never read: every call below is refused before a launch
-    call = lambda g=p, out=p, batch=1, rows=40, cols=40, dtype=0, steps=5, abc=ABC, eps=1e-7, work=p, size=1 << 40: \
+    call = lambda g=p, out=p, batch=1, rows=200, cols=200, dtype=0, steps=5, abc=ABC, eps=1e-7, work=p, size=1 << 40: \
         L.nrf_newton_schulz(g, out, batch, rows, cols, dtype, steps, *abc, eps, work, size, None)   # noqa: E731
     assert call(dtype=3) == -2 and call(steps=17) == -2 and call(steps=-1) == -2 and call(eps=0.0) == -2 and call(rows=0) == -2
     assert call(abc=(4.0, 0.0, 0.0)) == -2 and call(abc=(float("nan"), 0.0, 0.0)) == -2
@@ -40,7 +41,7 @@ def test_muon_update_refuses_on_the_host():
     null = (C.c_void_p * 1)(None)
 
     def call(params=arr, grads=arr, mom=arr, n=1, batch=1, clip=40.0, mu=0.9, steps=5, eps=1e-7, work=p, size=1 << 40):
-        return L.nrf_muon_update(params, grads, mom, n, batch, 40, 40, 1.0, clip, mu, 1, 0.02, 0.0, steps, *ABC, eps, work, size, None)
+        return L.nrf_muon_update(params, grads, mom, n, batch, 200, 200, 1.0, clip, mu, 1, 0.02, 0.0, steps, *ABC, eps, work, size, None)
 
     assert call(n=33) == -2 and call(clip=0.0) == -2 and call(mu=1.0) == -2 and call(mu=float("nan")) == -2 and call(steps=20) == -2
     assert call(params=None) == -1 and call(grads=null) == -1 and call(work=None) == -1
