@@ -160,8 +160,8 @@ __device__ __forceinline__ void finish_row(typename Traits<T>::elem* out, f32x4 
     store4<T>(out, v, valid);
 }
 
-// The general tile: TT x TT outputs (64 or 128), k in steps of 32, four wavefronts of a quarter each, the next step's loads in
-// registers while this step is multiplied.  Any size, any alignment.  The larger tile splits fp32 operands half as often per
+// The general tile: TT x TT outputs (64 or 128), k in steps of 32 D, four wavefronts of a quarter each, the next step's loads in
+// registers while this step is multiplied (D = 2 for 16-bit operands, whose 32 k are multiplied sooner than loaded).  Any size, any alignment.  The larger tile splits fp32 operands half as often per
 // product (splitting 32 elements per thread and step takes about half as long as the step's 96 MFMAs; at 64 x 64 as long as its
 // 24); the smaller one fills the chip with small problems.
 constexpr int kK = 32, kPitch = kK + 8;   // LDS row pitch: 80 B, so that 16 rows' 16 B reads spread over the banks
@@ -169,10 +169,11 @@ constexpr int kK = 32, kPitch = kK + 8;   // LDS row pitch: 80 B, so that 16 row
 template <class T, int FORM, int TT>
 __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
     typedef typename Traits<T>::elem elem;
-    constexpr int P = Traits<T>::planes, kTable = TT == 64 ? 1 : 2, N = TT / 64, M = TT / 32;   // octets per thread, 16-row blocks per wave
+    constexpr int P = Traits<T>::planes, D = P == 1 ? 2 : 1, kTable = TT == 64 ? 1 : 2, N = TT / 64, M = TT / 32;   // octets per thread, 16-row blocks per wave
     constexpr bool a_cols = FORM != kForward, b_cols = FORM == kDw;
     typedef DmaSide<kCols, TT, kK, 1, 4> Cols;
-    __shared__ __align__(16) unsigned short s_a[P][TT * (a_cols ? kK : kPitch)], s_b[P][TT * (b_cols ? kK : kPitch)];
+    constexpr int kPlaneA = TT * (a_cols ? kK : kPitch), kPlaneB = TT * (b_cols ? kK : kPitch), kStep = D * kK;
+    __shared__ __align__(16) unsigned short s_a[D][P][kPlaneA], s_b[D][P][kPlaneB];
     __shared__ int s_rows[TT];            // forward / dx: the tile's batch rows
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, q = lane >> 4;
     const int wa = (wave & 1) * (TT / 2), wb = (wave >> 1) * (TT / 2);
@@ -225,34 +226,39 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
     // into the next row, and what lies past the end of k is zeroed on its way into LDS: no load stands under a condition but
     // at the very end of a tensor.
     const elem *w_end = w + int64_t(g.n_out) * g.n_in, *x_end = x + g.n * g.n_in, *dy_end = dy + g.n * g.n_out, *ys_end = ys + g.n * g.n_out;
-    int kr[N], ck[N], cr[N], my_row[N], k_row[N];
+    int kr[N], ck[N], cr[N], my_row[N], k_row[D][N];
     const int kc = (t & 3) * 8;                       // [TT rows][4 octets of k]
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         kr[i] = (t >> 2) + 64 * i;
         ck[i] = (t + 256 * i) / (TT / 8), cr[i] = (t + 256 * i) % (TT / 8) * 8;   // [32 k][TT / 8 octets of rows]
         my_row[i] = FORM == kDw ? 0 : s_rows[kr[i]] < 0 ? s_rows[0] : s_rows[kr[i]];
-        k_row[i] = 0;
+#pragma unroll
+        for (int d = 0; d < D; ++d) k_row[d][i] = 0;
     }
     // dW: the batch rows of a step, looked up a step before its loads
     auto look_up = [&](int k0) {
         if (FORM == kDw)
 #pragma unroll
-            for (int i = 0; i < N; ++i) k_row[i] = order[k0 + ck[i] < k_end ? k0 + ck[i] : k_end - 1];
+            for (int d = 0; d < D; ++d)
+#pragma unroll
+                for (int i = 0; i < N; ++i) k_row[d][i] = order[k0 + d * kK + ck[i] < k_end ? k0 + d * kK + ck[i] : k_end - 1];
     };
-    auto load_a = [&](Oct<T>& v, int i, int k0) {
+    auto load_a = [&](Oct<T>& v, int d, int i, int k0) {
+        k0 += d * kK;
         const int col = a0 + cr[i] < n_a ? a0 + cr[i] : 0;
         if (FORM == kForward) v.load(w + int64_t(a0 + kr[i] < n_a ? a0 + kr[i] : n_a - 1) * g.n_in + (k0 + kc < k_end ? k0 + kc : 0), w_end);
         else if (FORM == kDx) v.load(w + int64_t(k0 + ck[i] < k_end ? k0 + ck[i] : 0) * g.n_in + col, w_end);
-        else v.load(x + int64_t(k_row[i]) * g.n_in + col, x_end);
+        else v.load(x + int64_t(k_row[d][i]) * g.n_in + col, x_end);
     };
-    auto load_b = [&](Oct<T>& v, Oct<T>& s, int i, int k0) {
+    auto load_b = [&](Oct<T>& v, Oct<T>& s, int d, int i, int k0) {
+        k0 += d * kK;
         if (FORM == kForward) {
             v.load(x + int64_t(my_row[i]) * g.n_in + (k0 + kc < k_end ? k0 + kc : 0), x_end);
             return;
         }
         const int64_t at = FORM == kDx ? int64_t(my_row[i]) * g.n_out + (k0 + kc < k_end ? k0 + kc : 0)
-                                       : int64_t(k_row[i]) * g.n_out + (cr[i] < b_count ? b0 + cr[i] : 0);
+                                       : int64_t(k_row[d][i]) * g.n_out + (cr[i] < b_count ? b0 + cr[i] : 0);
         v.load(dy + at, dy_end);
         if (g.relu) s.load(ys + at, ys_end);
     };
@@ -276,42 +282,52 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
     const unsigned one = __is_same(T, Fp16) ? 0x3c003c00u : 0x3f803f80u;
     const u32x4 ones = {one, one, one, one};
     if (!none && k_begin < k_end) {
-        Oct<T> ra[N], rb[N], rs[N];
+        Oct<T> ra[D][N], rb[D][N], rs[D][N];
+        auto load = [&](int k0) {
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+#pragma unroll
+                for (int i = 0; i < N; ++i) load_a(ra[d][i], d, i, k0), load_b(rb[d][i], rs[d][i], d, i, k0);
+        };
         look_up(k_begin);
+        load(k_begin);
+        look_up(k_begin + kStep);
+        for (int k0 = k_begin; k0 < k_end; k0 += kStep) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) load_a(ra[i], i, k_begin), load_b(rb[i], rs[i], i, k_begin);
-        look_up(k_begin + kK);
-        for (int k0 = k_begin; k0 < k_end; k0 += kK) {
+            for (int d = 0; d < D; ++d)
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                stage(s_a[0], sizeof(s_a[0]) / 2, ra[i], i, k0, a_cols);
-                if (FORM != kForward && g.relu) rb[i].keep_positive(rs[i]);
-                stage(s_b[0], sizeof(s_b[0]) / 2, rb[i], i, k0, b_cols);
-            }
+                for (int i = 0; i < N; ++i) {
+                    stage(s_a[d][0], kPlaneA, ra[d][i], i, k0 + d * kK, a_cols);
+                    if (FORM != kForward && g.relu) rb[d][i].keep_positive(rs[d][i]);
+                    stage(s_b[d][0], kPlaneB, rb[d][i], i, k0 + d * kK, b_cols);
+                }
             __syncthreads();
-            if (k0 + kK < k_end) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) load_a(ra[i], i, k0 + kK), load_b(rb[i], rs[i], i, k0 + kK);
-                look_up(k0 + 2 * kK);
+            if (k0 + kStep < k_end) {
+                load(k0 + kStep);
+                look_up(k0 + 2 * kStep);
             }
-            u32x4 fb[M][P];
 #pragma unroll
-            for (int m = 0; m < M; ++m)
+            for (int d = 0; d < D; ++d) {
+                if (d > 0 && k0 + d * kK >= k_end) break;
+                u32x4 fb[M][P];
 #pragma unroll
-                for (int i = 0; i < P; ++i) fb[m][i] = fragment(s_b[i], wb, m, b_cols);
+                for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int ma = 0; ma < M; ++ma) {
-                u32x4 fa[P];
+                    for (int i = 0; i < P; ++i) fb[m][i] = fragment(s_b[d][i], wb, m, b_cols);
 #pragma unroll
-                for (int i = 0; i < P; ++i) fa[i] = fragment(s_a[i], wa, ma, a_cols);
+                for (int ma = 0; ma < M; ++ma) {
+                    u32x4 fa[P];
 #pragma unroll
-                for (int mb = 0; mb < M; ++mb) acc[ma][mb] = mfma_terms<T>(fa, fb[mb], acc[ma][mb]);
+                    for (int i = 0; i < P; ++i) fa[i] = fragment(s_a[d][i], wa, ma, a_cols);
+#pragma unroll
+                    for (int mb = 0; mb < M; ++mb) acc[ma][mb] = mfma_terms<T>(fa, fb[mb], acc[ma][mb]);
+                }
+                if (with_db)
+#pragma unroll
+                    for (int mb = 0; mb < M; ++mb)
+#pragma unroll
+                        for (int i = P - 1; i >= 0; --i) sum[mb] = mfma16<T>(ones, fb[mb][i], sum[mb]);
             }
-            if (with_db)
-#pragma unroll
-                for (int mb = 0; mb < M; ++mb)
-#pragma unroll
-                    for (int i = P - 1; i >= 0; --i) sum[mb] = mfma16<T>(ones, fb[mb][i], sum[mb]);
             __syncthreads();
         }
     }
@@ -545,11 +561,11 @@ int launch_wide_dw(const ExpertArgs& g, hipStream_t stream) {
     return NRF_OK;
 }
 
-// Whether the wide kernels take a product: octets that do not straddle rows, operands under 4 GiB and at least half a tile's
-// columns.  Any number of rows: single tokens through 32 experts of 1024 -> 2048 take 17 us (7.3 TB/s of weights), the general
+// Whether the wide kernels take a product: octets that do not straddle rows (of x and w alone for the forward, which stores its
+// outputs at any alignment), operands under 4 GiB and at least half a tile's columns.  Any number of rows: single tokens through 32 experts of 1024 -> 2048 take 17 us (7.3 TB/s of weights), the general
 // tile 25.
-bool wide(int64_t n, int E, int n_in, int n_out, int dtype) {
-    return dtype != NRF_DTYPE_FP32 && n_in % 8 == 0 && n_out % 8 == 0 && n_in >= 128 && n_out >= 128 &&
+bool wide(int64_t n, int E, int n_in, int n_out, int dtype, bool forward = false) {
+    return dtype != NRF_DTYPE_FP32 && n_in % 8 == 0 && (forward || n_out % 8 == 0) && n_in >= 128 && n_out >= 128 &&
            n * (n_in > n_out ? n_in : n_out) < int64_t(1) << 31 && int64_t(n_out) * n_in < int64_t(1) << 31;
 }
 
@@ -899,7 +915,7 @@ NRF_EXPORT int nrf_expert_linear(const void* x, const void* weight, const void* 
     g.x = x, g.w = weight, g.bias = bias, g.plan = static_cast<const int*>(plan), g.out = y;
     g.n = n_rows, g.E = num_experts, g.n_in = n_in, g.n_out = n_out, g.relu = act == NRF_ACT_RELU, g.splits = 1;
     nrf_launch_begin();
-    if (wide(n_rows, num_experts, n_in, n_out, dtype) && nrf_aligned16(x) && nrf_aligned16(weight)) {
+    if (wide(n_rows, num_experts, n_in, n_out, dtype, true) && nrf_aligned16(x) && nrf_aligned16(weight)) {
         const int st = dtype == NRF_DTYPE_BF16 ? launch_wide_forward<Bf16>(g, static_cast<hipStream_t>(stream))
                                                : launch_wide_forward<Fp16>(g, static_cast<hipStream_t>(stream));
         return st != NRF_OK ? st : nrf_launch_status();

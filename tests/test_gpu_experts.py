@@ -131,7 +131,8 @@ SHAPES = [  # n, E, n_in, n_out, kind
     (33, 2, 63, 32, "uniform"), (300, 5, 32, 32, "outside"), (1000, 64, 63, 32, "skew"), (2000, 3, 319, 256, "uniform"),
     (129, 2, 130, 257, "one"), (64, 3, 16, 8, "none"), (2500, 8, 96, 100, "skew"), (515, 1, 1024, 40, "uniform"),
     (700, 2, 512, 640, "uniform"), (900, 3, 264, 136, "outside"), (1300, 2, 128, 520, "skew"), (5000, 1, 136, 128, "one"),
-    (640, 8, 200, 328, "skew"),
+    (640, 8, 200, 328, "skew"), (700, 3, 256, 131, "outside"), (3000, 2, 136, 517, "skew"), (300, 4, 131, 259, "uniform"),
+    (90, 2, 777, 129, "outside"), (600, 2, 129, 128, "one"),
 ]
 
 
