@@ -75,10 +75,11 @@ __device__ __forceinline__ float before(const SchulzArgs& s, int t, int64_t base
     if constexpr (__is_same(T, OutMuon)) return (static_cast<const float*>(s.out[t]) + base)[i];
     else return 0.f;
 }
-// 4096 / max(norm, eps); a norm that is not a number stays one
+// 4096 / max(norm, eps); NaN for a norm that is not finite
 __device__ __forceinline__ float start_scale(double sum, float eps) {
     double norm = sqrt(sum);
     if (norm < double(eps)) norm = double(eps);
+    if (norm == double(INFINITY)) norm = double(NAN);
     return float(4096.0 / norm);
 }
 

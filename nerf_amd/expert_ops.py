@@ -126,7 +126,8 @@ class _ExpertLinear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, plan, activation):
         y = _forward(x.detach(), weight.detach(), None if bias is None else bias.detach(), plan, activation)
         ctx.plan, ctx.activation = plan, activation
-        ctx.save_for_backward(x, weight, y if activation == "relu" else None)
+        # the plan's buffer among them: autograd then notices a write to the views that the plan hands out
+        ctx.save_for_backward(x, weight, y if activation == "relu" else None, plan.buffer)
         return y
 
     @staticmethod
@@ -134,7 +135,7 @@ class _ExpertLinear(torch.autograd.Function):
     def backward(ctx, grad_y):
         if torch.cuda.is_current_stream_capturing():
             raise NrfError(_CAPTURE)
-        x, weight, y = ctx.saved_tensors
+        x, weight, y, _ = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
         dx, dw, db = expert_linear_backward(grad_y, x, weight, ctx.plan, y=y, activation=ctx.activation, want_x=want_x,
                                             want_weight=want_w or want_b, want_bias=want_b)

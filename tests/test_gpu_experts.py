@@ -309,6 +309,33 @@ def test_autograd_under_capture_is_refused():
     assert float(keep) == 0
 
 
+@pytest.mark.parametrize("n_in,n_out,dtype", [(63, 32, "fp32"), (130, 70, "fp32"), (256, 128, "bf16"), (100, 9, "fp16")])
+@pytest.mark.parametrize("relu", [False, True])
+def test_a_batch_without_rows(n_in, n_out, dtype, relu):
+    x, w = torch.zeros(0, n_in, dtype=DT[dtype], device=DEV), torch.randn(5, n_out, n_in, device=DEV).to(DT[dtype])
+    plan, act = expert_plan(torch.zeros(0, dtype=torch.int32, device=DEV), 5), "relu" if relu else "none"
+    y = expert_linear(x, w, w[:, :, 0], plan, act)
+    dx, dw, db = expert_linear_backward(y, x, w, plan, y=y, activation=act)
+    assert y.shape == (0, n_out) and dx.shape == x.shape and plan.counts.sum() == 0 and not plan.offsets.any()
+    assert dw.shape == w.shape and not dw.any() and db.shape == (5, n_out) and not db.any()
+
+
+def test_index_values_of_any_size():
+    index = torch.tensor([-2 ** 31, 2 ** 31 - 1, 0, 3, 2, -1, 65536, 131074, 2, 16384 * 2 + 1], dtype=torch.int32, device=DEV)
+    plan = expert_plan(index, 3)
+    assert plan.counts.tolist() == [1, 0, 2] and plan.offsets.tolist() == [0, 1, 1, 3]
+    assert plan.order.tolist() == [2, 4, 8, 0, 1, 3, 5, 6, 7, 9]
+
+
+def test_a_plan_written_to_between_forward_and_backward_is_noticed():
+    x = torch.randn(20, 8, device=DEV, requires_grad=True)
+    plan = expert_plan(torch.zeros(20, dtype=torch.int32, device=DEV), 2)
+    y = expert_linear(x, torch.randn(2, 4, 8, device=DEV), None, plan)
+    plan.order.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_refusals():
     x, w, b, dy, index = layer(40, 2, 8, 6, torch.float32, 0)
     plan = expert_plan(index, 2)

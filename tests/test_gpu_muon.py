@@ -112,6 +112,24 @@ def test_zero_low_rank_and_not_finite_matrices(shape):
     assert torch.isnan(newton_schulz(g.to(DEV))[2]).all()
 
 
+@pytest.mark.parametrize("shape", [(3, 20, 24), (3, 100, 31), (3, 60, 70), (3, 100, 140), (3, 150, 90), (3, 200, 130), (3, 64, 2000)], ids=str)
+@pytest.mark.parametrize("steps", [0, 5])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_one_bad_value_is_nan_everywhere_in_its_matrix_alone(shape, steps, bad):
+    g = gradient(*shape).to(DEV)
+    clean = newton_schulz(g, steps=steps)
+    g[1, 7, 11] = bad
+    got = newton_schulz(g, steps=steps)
+    assert got[1].isnan().all() and torch.equal(got[[0, 2]], clean[[0, 2]])
+    p, m = torch.zeros_like(g), torch.zeros_like(g)
+    clipped = newton_schulz(g.clamp(-40, 40), steps=steps)       # an infinite gradient is clipped, NaN stays
+    muon_update(p, g, m, lr=1.0, momentum=0.0, steps=steps)
+    scale = max(1.0, shape[1] / shape[2]) ** 0.5
+    assert bool(p[1].isnan().all()) == (bad != bad)
+    off = (p + scale * clipped)[[0, 2] if bad != bad else [0, 1, 2]].abs()
+    assert float(off.max()) <= 4 * 2.0 ** -24 * scale * float(clipped.nan_to_num().abs().max())     # the rate and the product rounded
+
+
 def test_views_and_in_place():
     g = gradient(3, 48, 80, seed=3).to(DEV)
     want = newton_schulz(g)
