@@ -160,6 +160,48 @@ __device__ __forceinline__ void finish_row(typename Traits<T>::elem* out, f32x4 
     store4<T>(out, v, valid);
 }
 
+// Consecutive workgroups go to different XCDs: each XCD takes a contiguous eighth of the long row runs and of the short
+// ones (an expert's runs share its weights in that XCD's L2).  -> the `local`-th run of this one, -1 past its last.
+__device__ __forceinline__ int xcd_run(const int* runs, int xcd, int local) {
+    const int longs = runs[0], shorts = runs[1] - longs;
+    int begin = int(int64_t(longs) * xcd / 8), end = int(int64_t(longs) * (xcd + 1) / 8);
+    if (local < end - begin) return begin + local;
+    local -= end - begin;
+    begin = int(int64_t(shorts) * xcd / 8), end = int(int64_t(shorts) * (xcd + 1) / 8);
+    return local < end - begin ? longs + begin + local : -1;
+}
+__host__ __device__ constexpr int64_t xcd_blocks(int64_t slots, int a_tiles) { return (slots / 8 + 2) * 8 * a_tiles; }
+
+// The expert with the `rank`-th most rows (of at most 64; equal ones by number).  A tile of dW takes as long as its expert has
+// rows, and the longest tiles have to begin first: begun by number, the CUs of 16 uneven experts were busy 67% of the time.
+__device__ __forceinline__ int expert_of_rank(const int* counts, int E, int rank) {
+    const int lane = threadIdx.x & 63, mine = lane < E ? counts[lane] : -1;
+    int above = 0;
+    for (int e = 0; e < E; ++e) {
+        const int other = __builtin_amdgcn_readlane(mine, e);
+        above += other > mine || (other == mine && e < lane);
+    }
+    return __ffsll((long long)__ballot(lane < E && above == rank)) - 1;
+}
+
+// dW's unit of this workgroup: which expert, which of its `tiles`.  Every XCD takes a contiguous eighth of each expert's tiles
+// (whole experts per XCD leave the XCD of the two most popular of sixteen with twice the average: 172 us where this takes
+// 99); fewer than eight go round.
+__device__ __forceinline__ bool dw_unit(const int* counts, int E, int tiles, int& expert, int& at) {
+    const int local = blockIdx.x / 8, xcd = blockIdx.x % 8;
+    if (tiles >= 8) {
+        const int per = (tiles + 7) / 8;
+        expert = local / per, at = int(int64_t(tiles) * xcd / 8) + local % per;
+        if (at >= int(int64_t(tiles) * (xcd + 1) / 8)) return false;
+    } else {
+        expert = (local * 8 + xcd) / tiles, at = (local * 8 + xcd) % tiles;
+    }
+    if (expert >= E) return false;
+    if (E <= 64) expert = expert_of_rank(counts, E, expert);
+    return true;
+}
+int64_t dw_blocks(int64_t tiles, int E) { return tiles >= 8 ? E * ((tiles + 7) / 8) * 8 : (E * tiles + 7) / 8 * 8; }
+
 // The general tile: TT x TT outputs (64 or 128), k in steps of 32 D, four wavefronts of a quarter each, the next step's loads in
 // registers while this step is multiplied (D = 2 for 16-bit operands, whose 32 k are multiplied sooner than loaded).  Any size, any alignment.  The larger tile splits fp32 operands half as often per
 // product (splitting 32 elements per thread and step takes about half as long as the step's 96 MFMAs; at 64 x 64 as long as its
@@ -167,9 +209,9 @@ __device__ __forceinline__ void finish_row(typename Traits<T>::elem* out, f32x4 
 constexpr int kK = 32, kPitch = kK + 8;   // LDS row pitch: 80 B, so that 16 rows' 16 B reads spread over the banks
 
 template <class T, int FORM, int TT>
-__global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
+__global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g, int a_tiles, int b_tiles) {
     typedef typename Traits<T>::elem elem;
-    constexpr int P = Traits<T>::planes, D = P == 1 ? 2 : 1, kTable = TT == 64 ? 1 : 2, N = TT / 64, M = TT / 32;   // octets per thread, 16-row blocks per wave
+    constexpr int P = Traits<T>::planes, D = P == 1 ? 2 : 1, kSets = TT == 64 ? 2 : 1, kTable = TT == 64 ? 1 : 2, N = TT / 64, M = TT / 32;   // octets per thread, 16-row blocks per wave
     constexpr bool a_cols = FORM != kForward, b_cols = FORM == kDw;
     typedef DmaSide<kCols, TT, kK, 1, 4> Cols;
     constexpr int kPlaneA = TT * (a_cols ? kK : kPitch), kPlaneB = TT * (b_cols ? kK : kPitch), kStep = D * kK;
@@ -177,42 +219,42 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
     __shared__ int s_rows[TT];            // forward / dx: the tile's batch rows
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, q = lane >> 4;
     const int wa = (wave & 1) * (TT / 2), wb = (wave >> 1) * (TT / 2);
-    const int a0 = blockIdx.y * TT;       // first A row = first output column
     const PlanLayout L(g.n, g.E);
     const int* order = g.plan + L.order;
 
-    int expert, b0 = 0, b_count, k_begin = 0, k_end;
+    int expert, a0, b0 = 0, b_count, k_begin = 0, k_end;   // a0: first A row = first output column
     const int n_a = FORM == kForward ? g.n_out : g.n_in;
     int64_t part = 0;                     // dW in parts: which
     bool in_parts = false;
-    if (FORM == kDw) {
-        if (g.splits == 0) {              // a run of at most kPartRows rows
-            const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[kPartTable])[blockIdx.x];   // inside the table's room
-            if (int(blockIdx.x) >= g.plan[L.runs + 2 * kPartTable + 1]) return;
-            expert = tile.y & 0xffff;
+    if (FORM == kDw && g.splits != 0) {
+        int at;
+        if (!dw_unit(g.plan, g.E, a_tiles * b_tiles * g.splits, expert, at)) return;
+        const int split = at / (a_tiles * b_tiles), tile = at % (a_tiles * b_tiles);
+        const int first = g.plan[L.offsets + expert], rows = g.plan[expert];
+        const int per = (((rows + g.splits - 1) / g.splits) + kK - 1) / kK * kK;   // whole k steps
+        k_begin = first + (split * per < rows ? split * per : rows);
+        k_end = first + (split * per + per < rows ? split * per + per : rows);
+        part = int64_t(split) * g.E + expert, in_parts = g.splits > 1;
+        a0 = tile % a_tiles * TT, b0 = tile / a_tiles * TT;
+    } else {                              // a run of rows, all of whose tiles are the same XCD's
+        constexpr int table = FORM == kDw ? kPartTable : kTable;
+        const int tiles = a_tiles * b_tiles, local = blockIdx.x / 8, tile = local % tiles;
+        const int at = xcd_run(g.plan + L.runs + 2 * table, blockIdx.x % 8, local / tiles);
+        if (at < 0) return;
+        const int2 run = reinterpret_cast<const int2*>(g.plan + L.tiles[table])[at];
+        b_count = run.y >> 16, expert = run.y & 0xffff;
+        a0 = tile % a_tiles * TT, b0 = tile / a_tiles * TT;
+        if (FORM == kDw) {
             if (expert == g.E) return;
-            k_begin = tile.x, k_end = tile.x + (tile.y >> 16);
-            part = (tile.x >> 8) + expert, in_parts = g.plan[expert] > kPartRows;
+            k_begin = run.x, k_end = run.x + b_count;
+            part = (run.x >> 8) + expert, in_parts = g.plan[expert] > kPartRows;
         } else {
-            expert = blockIdx.x / g.splits;
-            const int split = blockIdx.x % g.splits;
-            const int first = g.plan[L.offsets + expert], rows = g.plan[expert];
-            const int per = (((rows + g.splits - 1) / g.splits) + kK - 1) / kK * kK;   // whole k steps
-            k_begin = first + (split * per < rows ? split * per : rows);
-            k_end = first + (split * per + per < rows ? split * per + per : rows);
-            part = int64_t(split) * g.E + expert, in_parts = g.splits > 1;
+            if (t < TT) s_rows[t] = t < b_count ? order[run.x + t] : -1;
+            __syncthreads();
+            k_end = FORM == kForward ? g.n_in : g.n_out;
         }
-        b0 = blockIdx.z * TT;
-        b_count = g.n_out - b0 < TT ? g.n_out - b0 : TT;
-    } else {
-        const int2 tile = reinterpret_cast<const int2*>(g.plan + L.tiles[kTable])[blockIdx.x];   // inside the table's room
-        if (int(blockIdx.x) >= g.plan[L.runs + 2 * kTable + 1]) return;
-        b_count = tile.y >> 16;
-        expert = tile.y & 0xffff;
-        if (t < TT) s_rows[t] = t < b_count ? order[tile.x + t] : -1;
-        __syncthreads();
-        k_end = FORM == kForward ? g.n_in : g.n_out;
     }
+    if (FORM == kDw) b_count = g.n_out - b0 < TT ? g.n_out - b0 : TT;
     const bool none = FORM != kDw && expert == g.E;   // rows of no expert: zeros
     const int64_t w_off = int64_t(none ? 0 : expert) * g.n_out * g.n_in;
     const elem* w = static_cast<const elem*>(g.w) + w_off;
@@ -278,33 +320,32 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
 
     f32x4 acc[M][M] = {};
     f32x4 sum[M] = {};                                // dW: db of this wavefront's outputs
-    const bool with_db = FORM == kDw && g.db && blockIdx.y == 0 && wa == 0;
+    const bool with_db = FORM == kDw && g.db && a0 == 0 && wa == 0;
     const unsigned one = __is_same(T, Fp16) ? 0x3c003c00u : 0x3f803f80u;
     const u32x4 ones = {one, one, one, one};
     if (!none && k_begin < k_end) {
-        Oct<T> ra[D][N], rb[D][N], rs[D][N];
-        auto load = [&](int k0) {
+        struct Step {                                 // a step's octets, on their way
+            Oct<T> a[D][N], b[D][N], s[D][N];
+        };
+        auto load = [&](Step& r, int k0) {
 #pragma unroll
             for (int d = 0; d < D; ++d)
 #pragma unroll
-                for (int i = 0; i < N; ++i) load_a(ra[d][i], d, i, k0), load_b(rb[d][i], rs[d][i], d, i, k0);
+                for (int i = 0; i < N; ++i) load_a(r.a[d][i], d, i, k0), load_b(r.b[d][i], r.s[d][i], d, i, k0);
         };
-        look_up(k_begin);
-        load(k_begin);
-        look_up(k_begin + kStep);
-        for (int k0 = k_begin; k0 < k_end; k0 += kStep) {
+        auto walk = [&](Step& r, int k0) {
 #pragma unroll
             for (int d = 0; d < D; ++d)
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    stage(s_a[d][0], kPlaneA, ra[d][i], i, k0 + d * kK, a_cols);
-                    if (FORM != kForward && g.relu) rb[d][i].keep_positive(rs[d][i]);
-                    stage(s_b[d][0], kPlaneB, rb[d][i], i, k0 + d * kK, b_cols);
+                    stage(s_a[d][0], kPlaneA, r.a[d][i], i, k0 + d * kK, a_cols);
+                    if (FORM != kForward && g.relu) r.b[d][i].keep_positive(r.s[d][i]);
+                    stage(s_b[d][0], kPlaneB, r.b[d][i], i, k0 + d * kK, b_cols);
                 }
             __syncthreads();
-            if (k0 + kStep < k_end) {
-                load(k0 + kStep);
-                look_up(k0 + 2 * kStep);
+            if (k0 + kSets * kStep < k_end) {
+                load(r, k0 + kSets * kStep);
+                look_up(k0 + (kSets + 1) * kStep);
             }
 #pragma unroll
             for (int d = 0; d < D; ++d) {
@@ -329,7 +370,18 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
                         for (int i = P - 1; i >= 0; --i) sum[mb] = mfma16<T>(ones, fb[mb][i], sum[mb]);
             }
             __syncthreads();
+        };
+        Step r[kSets];
+        look_up(k_begin);
+#pragma unroll
+        for (int u = 0; u < kSets; ++u) {
+            load(r[u], k_begin + u * kStep);
+            look_up(k_begin + (u + 1) * kStep);
         }
+        for (int k0 = k_begin; k0 < k_end; k0 += kSets * kStep)
+#pragma unroll
+            for (int u = 0; u < kSets; ++u)
+                if (u == 0 || k0 + u * kStep < k_end) walk(r[u], k0 + u * kStep);
     }
 
     // lane (c, q) holds outputs a0 + wa + 16 ma + 4 q .. + 3 of b row wb + 16 mb + c
@@ -359,18 +411,6 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g) {
 }
 
 // ---- bf16 / fp16, wide layers ----------------------------------------------------------------------------------------------
-// Consecutive workgroups go to different XCDs: each XCD takes a contiguous eighth of the long row runs and of the short
-// ones (an expert's runs share its weights in that XCD's L2).  -> the `local`-th run of this one, -1 past its last.
-__device__ __forceinline__ int xcd_run(const int* runs, int xcd, int local) {
-    const int longs = runs[0], shorts = runs[1] - longs;
-    int begin = int(int64_t(longs) * xcd / 8), end = int(int64_t(longs) * (xcd + 1) / 8);
-    if (local < end - begin) return begin + local;
-    local -= end - begin;
-    begin = int(int64_t(shorts) * xcd / 8), end = int(int64_t(shorts) * (xcd + 1) / 8);
-    return local < end - begin ? longs + begin + local : -1;
-}
-__host__ __device__ constexpr int64_t xcd_blocks(int64_t slots, int a_tiles) { return (slots / 8 + 2) * 8 * a_tiles; }
-
 // Forward and dx: 256 output columns by a run of batch rows, eight wavefronts.  Runs of more than 128 rows: 256 x 256, 128 x 64
 // per wavefront (12 KiB of LDS reads to 32 MFMAs), two steps of 64 k in LDS (128 KiB).  Shorter runs wait for data, not for the
 // matrix cores: 256 x 128 with three steps in LDS, 256 x 64 with four, so that more of the weights is on its way (a run of 64
@@ -437,18 +477,6 @@ __global__ __launch_bounds__(512) void expert_wide_rows_kernel(ExpertArgs g, int
     else wide_rows_tile<T, FORM, 64>(g, smem, a0, b_count, expert, order);
 }
 
-// The expert with the `rank`-th most rows (of at most 64; equal ones by number).  A tile of dW takes as long as its expert has
-// rows, and the longest tiles have to begin first: begun by number, the CUs of 16 uneven experts were busy 67% of the time.
-__device__ __forceinline__ int expert_of_rank(const int* counts, int E, int rank) {
-    const int lane = threadIdx.x & 63, mine = lane < E ? counts[lane] : -1;
-    int above = 0;
-    for (int e = 0; e < E; ++e) {
-        const int other = __builtin_amdgcn_readlane(mine, e);
-        above += other > mine || (other == mine && e < lane);
-    }
-    return __ffsll((long long)__ballot(lane < E && above == rank)) - 1;
-}
-
 // dW: 256 input columns x 128 output columns, k the expert's rows through the list of them in LDS, kListRows at a time.
 constexpr int kListRows = 4096;
 template <class T> struct WideDw {
@@ -464,19 +492,8 @@ __global__ __launch_bounds__(512) void expert_wide_dw_kernel(ExpertArgs g, int a
     extern __shared__ __align__(16) char smem[];
     int* s_list = reinterpret_cast<int*>(smem + Gemm::kLds);
     const PlanLayout L(g.n, g.E);
-    // Every XCD takes a contiguous eighth of each expert's tiles (whole experts per XCD leave the XCD of the two most popular
-    // of sixteen with twice the average: 172 us where this takes 99); fewer than eight go round.
-    const int tiles = a_tiles * b_tiles * g.splits, local = blockIdx.x / 8, xcd = blockIdx.x % 8;
     int expert, at;
-    if (tiles >= 8) {
-        const int per = (tiles + 7) / 8;
-        expert = local / per, at = tiles * xcd / 8 + local % per;
-        if (at >= tiles * (xcd + 1) / 8) return;
-    } else {
-        expert = (local * 8 + xcd) / tiles, at = (local * 8 + xcd) % tiles;
-    }
-    if (expert >= g.E) return;
-    if (g.E <= 64) expert = expert_of_rank(g.plan, g.E, expert);
+    if (!dw_unit(g.plan, g.E, a_tiles * b_tiles * g.splits, expert, at)) return;
     const int split = at / (a_tiles * b_tiles), tile = at % (a_tiles * b_tiles);
     const int a0 = tile % a_tiles * W::kA, b0 = tile / a_tiles * W::kB;
     const int rows = g.plan[expert], per = ((rows + g.splits - 1) / g.splits + 63) / 64 * 64;
@@ -556,7 +573,7 @@ int launch_wide_dw(const ExpertArgs& g, hipStream_t stream) {
     auto kernel = &expert_wide_dw_kernel<T>;
     const int st = allow_lds(reinterpret_cast<const void*>(kernel), W::kLds);
     if (st != NRF_OK) return st;
-    const int64_t tiles = int64_t(a_tiles) * b_tiles * g.splits, blocks = tiles >= 8 ? g.E * ((tiles + 7) / 8) * 8 : (g.E * tiles + 7) / 8 * 8;
+    const int64_t blocks = dw_blocks(int64_t(a_tiles) * b_tiles * g.splits, g.E);
     kernel<<<dim3(unsigned(blocks)), 512, W::kLds, stream>>>(g, a_tiles, b_tiles);
     return NRF_OK;
 }
@@ -872,13 +889,14 @@ int64_t part_bytes(int64_t n, int E, int n_in, int n_out, int splits) {
 
 template <int FORM, int TT>
 void launch_tile(int dtype, const ExpertArgs& g, hipStream_t stream) {
-    const unsigned in = (g.n_in + TT - 1) / TT, out = (g.n_out + TT - 1) / TT, slots = unsigned(PlanLayout::slots(g.n, g.E, TT == 64 ? 1 : 2));
-    const dim3 grid = FORM == kForward ? dim3(slots, out) : FORM == kDx ? dim3(slots, in) 
-                      : g.splits == 0 ? dim3(unsigned(PlanLayout::slots(g.n, g.E, kPartTable)), in, out)
-                                      : dim3(unsigned(g.E) * unsigned(g.splits), in, out);
-    if (dtype == NRF_DTYPE_FP32) expert_tile_kernel<Fp32, FORM, TT><<<grid, 256, 0, stream>>>(g);
-    else if (dtype == NRF_DTYPE_BF16) expert_tile_kernel<Bf16, FORM, TT><<<grid, 256, 0, stream>>>(g);
-    else expert_tile_kernel<Fp16, FORM, TT><<<grid, 256, 0, stream>>>(g);
+    const int a_tiles = ((FORM == kForward ? g.n_out : g.n_in) + TT - 1) / TT, b_tiles = FORM == kDw ? (g.n_out + TT - 1) / TT : 1;
+    const int table = FORM == kDw ? kPartTable : TT == 64 ? 1 : 2;
+    const int64_t blocks = FORM == kDw && g.splits != 0 ? dw_blocks(int64_t(g.splits) * a_tiles * b_tiles, g.E)
+                                                        : xcd_blocks(PlanLayout::slots(g.n, g.E, table), a_tiles * b_tiles);
+    const dim3 grid{unsigned(blocks)};
+    if (dtype == NRF_DTYPE_FP32) expert_tile_kernel<Fp32, FORM, TT><<<grid, 256, 0, stream>>>(g, a_tiles, b_tiles);
+    else if (dtype == NRF_DTYPE_BF16) expert_tile_kernel<Bf16, FORM, TT><<<grid, 256, 0, stream>>>(g, a_tiles, b_tiles);
+    else expert_tile_kernel<Fp16, FORM, TT><<<grid, 256, 0, stream>>>(g, a_tiles, b_tiles);
 }
 template <int FORM>
 void launch_tile(int dtype, const ExpertArgs& g, hipStream_t stream) {
