@@ -211,7 +211,7 @@ constexpr int kK = 32, kPitch = kK + 8;   // LDS row pitch: 80 B, so that 16 row
 template <class T, int FORM, int TT>
 __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g, int a_tiles, int b_tiles) {
     typedef typename Traits<T>::elem elem;
-    constexpr int P = Traits<T>::planes, D = P == 1 ? 2 : 1, kSets = TT == 64 ? 2 : 1, kTable = TT == 64 ? 1 : 2, N = TT / 64, M = TT / 32;   // octets per thread, 16-row blocks per wave
+    constexpr int P = Traits<T>::planes, D = P == 1 ? 2 : 1, kSets = TT == 64 ? 2 : 1, kTable = TT == 64 ? 1 : 2, M = TT / 32;   // 16-row blocks per wave
     constexpr bool a_cols = FORM != kForward, b_cols = FORM == kDw;
     typedef DmaSide<kCols, TT, kK, 1, 4> Cols;
     constexpr int kPlaneA = TT * (a_cols ? kK : kPitch), kPlaneB = TT * (b_cols ? kK : kPitch), kStep = D * kK;
@@ -263,55 +263,52 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g, int a_ti
     const elem* ys = static_cast<const elem*>(g.y);
     const SplitSel sel = SplitSel::make();
 
-    // This thread's eight elements of a step, N times: along k for an operand whose k is contiguous, along the tile's rows
-    // otherwise.  Rows past the operand's last one read a row that is there (their outputs are not stored), octets may run on
-    // into the next row, and what lies past the end of k is zeroed on its way into LDS: no load stands under a condition but
-    // at the very end of a tensor.
+    // This thread's eight elements of a step and operand, kOcts times: along k for an operand whose k is contiguous, along the
+    // tile's rows otherwise.  (16-bit: 64 k, eight lanes and 128 B of one row; rows that are 4 B aligned move 118 B/ns per CU so,
+    // 67 with four lanes of 64 B.)  Rows past the operand's last one read a row that is there (their outputs are not stored),
+    // octets may run on into the next row, and what lies past the end of k is zeroed on its way into LDS: no load stands under
+    // a condition but at the very end of a tensor.
     const elem *w_end = w + int64_t(g.n_out) * g.n_in, *x_end = x + g.n * g.n_in, *dy_end = dy + g.n * g.n_out, *ys_end = ys + g.n * g.n_out;
-    int kr[N], ck[N], cr[N], my_row[N], k_row[D][N];
-    const int kc = (t & 3) * 8;                       // [TT rows][4 octets of k]
+    constexpr int kLanes = kStep / 8, kOcts = TT * kLanes / 256, kDown = 256 / kLanes, kAlong = TT / 8, kNext = 256 / kAlong;
+    int my_row[kOcts], k_row[kOcts];
+    const int kr = t / kLanes, kc = t % kLanes * 8;   // [TT rows][kLanes octets of k]: rows kr + kDown j
+    const int ck = t / kAlong, cr = t % kAlong * 8;   // [kStep k][kAlong octets of rows]: k = ck + kNext j
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        kr[i] = (t >> 2) + 64 * i;
-        ck[i] = (t + 256 * i) / (TT / 8), cr[i] = (t + 256 * i) % (TT / 8) * 8;   // [32 k][TT / 8 octets of rows]
-        my_row[i] = FORM == kDw ? 0 : s_rows[kr[i]] < 0 ? s_rows[0] : s_rows[kr[i]];
-#pragma unroll
-        for (int d = 0; d < D; ++d) k_row[d][i] = 0;
+    for (int j = 0; j < kOcts; ++j) {
+        my_row[j] = FORM == kDw ? 0 : s_rows[kr + kDown * j] < 0 ? s_rows[0] : s_rows[kr + kDown * j];
+        k_row[j] = 0;
     }
     // dW: the batch rows of a step, looked up a step before its loads
     auto look_up = [&](int k0) {
         if (FORM == kDw)
 #pragma unroll
-            for (int d = 0; d < D; ++d)
-#pragma unroll
-                for (int i = 0; i < N; ++i) k_row[d][i] = order[k0 + d * kK + ck[i] < k_end ? k0 + d * kK + ck[i] : k_end - 1];
+            for (int j = 0; j < kOcts; ++j) k_row[j] = order[k0 + ck + kNext * j < k_end ? k0 + ck + kNext * j : k_end - 1];
     };
-    auto load_a = [&](Oct<T>& v, int d, int i, int k0) {
-        k0 += d * kK;
-        const int col = a0 + cr[i] < n_a ? a0 + cr[i] : 0;
-        if (FORM == kForward) v.load(w + int64_t(a0 + kr[i] < n_a ? a0 + kr[i] : n_a - 1) * g.n_in + (k0 + kc < k_end ? k0 + kc : 0), w_end);
-        else if (FORM == kDx) v.load(w + int64_t(k0 + ck[i] < k_end ? k0 + ck[i] : 0) * g.n_in + col, w_end);
-        else v.load(x + int64_t(k_row[d][i]) * g.n_in + col, x_end);
+    auto load_a = [&](Oct<T>& v, int j, int k0) {
+        const int row = a0 + kr + kDown * j, k = k0 + ck + kNext * j, col = a0 + cr < n_a ? a0 + cr : 0;
+        if (FORM == kForward) v.load(w + int64_t(row < n_a ? row : n_a - 1) * g.n_in + (k0 + kc < k_end ? k0 + kc : 0), w_end);
+        else if (FORM == kDx) v.load(w + int64_t(k < k_end ? k : 0) * g.n_in + col, w_end);
+        else v.load(x + int64_t(k_row[j]) * g.n_in + col, x_end);
     };
-    auto load_b = [&](Oct<T>& v, Oct<T>& s, int d, int i, int k0) {
-        k0 += d * kK;
+    auto load_b = [&](Oct<T>& v, Oct<T>& s, int j, int k0) {
         if (FORM == kForward) {
-            v.load(x + int64_t(my_row[i]) * g.n_in + (k0 + kc < k_end ? k0 + kc : 0), x_end);
+            v.load(x + int64_t(my_row[j]) * g.n_in + (k0 + kc < k_end ? k0 + kc : 0), x_end);
             return;
         }
-        const int64_t at = FORM == kDx ? int64_t(my_row[i]) * g.n_out + (k0 + kc < k_end ? k0 + kc : 0)
-                                       : int64_t(k_row[d][i]) * g.n_out + (cr[i] < b_count ? b0 + cr[i] : 0);
+        const int64_t at = FORM == kDx ? int64_t(my_row[j]) * g.n_out + (k0 + kc < k_end ? k0 + kc : 0)
+                                       : int64_t(k_row[j]) * g.n_out + (cr < b_count ? b0 + cr : 0);
         v.load(dy + at, dy_end);
         if (g.relu) s.load(ys + at, ys_end);
     };
-    // LDS holds [row][k] (pitch kPitch) of an operand whose k is contiguous, [k][row] of the others, read back transposed
-    auto stage = [&](unsigned short* s, int plane, Oct<T> v, int i, int k0, bool cols) {
-        if (k0 + kK > k_end) v.limit(cols ? (k0 + ck[i] < k_end ? 8 : 0) : k_end - k0 - kc);
+    // LDS holds, per 32 k, [row][k] (pitch kPitch) of an operand whose k is contiguous, [k][row] of the others, read back transposed
+    auto stage = [&](unsigned short* s, int plane, Oct<T> v, int j, int k0, bool cols) {
+        const int k = cols ? ck + kNext * j : kc, row = cols ? cr : kr + kDown * j;
+        if (k0 + kStep > k_end) v.limit(cols ? (k0 + k < k_end ? 8 : 0) : k_end - k0 - k);
         u32x4 p[P];
         v.terms(sel, p);
+        unsigned short* to = s + k / kK * (P * plane) + (cols ? k % kK * TT + ((row / 8) ^ Cols::swizzle(k % kK)) * 8 : row * kPitch + k % kK);
 #pragma unroll
-        for (int j = 0; j < P; ++j)
-            *reinterpret_cast<u32x4*>(s + j * plane + (cols ? ck[i] * TT + ((cr[i] / 8) ^ Cols::swizzle(ck[i])) * 8 : kr[i] * kPitch + kc)) = p[j];
+        for (int i = 0; i < P; ++i) *reinterpret_cast<u32x4*>(to + i * plane) = p[i];
     };
     auto fragment = [&](const unsigned short* s, int first, int m, bool cols) {
         return cols ? __builtin_bit_cast(u32x4, Cols::frag(reinterpret_cast<const char*>(s), first, m, 0, c, q))
@@ -325,23 +322,19 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g, int a_ti
     const u32x4 ones = {one, one, one, one};
     if (!none && k_begin < k_end) {
         struct Step {                                 // a step's octets, on their way
-            Oct<T> a[D][N], b[D][N], s[D][N];
+            Oct<T> a[kOcts], b[kOcts], s[kOcts];
         };
         auto load = [&](Step& r, int k0) {
 #pragma unroll
-            for (int d = 0; d < D; ++d)
-#pragma unroll
-                for (int i = 0; i < N; ++i) load_a(r.a[d][i], d, i, k0), load_b(r.b[d][i], r.s[d][i], d, i, k0);
+            for (int j = 0; j < kOcts; ++j) load_a(r.a[j], j, k0), load_b(r.b[j], r.s[j], j, k0);
         };
         auto walk = [&](Step& r, int k0) {
 #pragma unroll
-            for (int d = 0; d < D; ++d)
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    stage(s_a[d][0], kPlaneA, r.a[d][i], i, k0 + d * kK, a_cols);
-                    if (FORM != kForward && g.relu) r.b[d][i].keep_positive(r.s[d][i]);
-                    stage(s_b[d][0], kPlaneB, r.b[d][i], i, k0 + d * kK, b_cols);
-                }
+            for (int j = 0; j < kOcts; ++j) {
+                stage(s_a[0][0], kPlaneA, r.a[j], j, k0, a_cols);
+                if (FORM != kForward && g.relu) r.b[j].keep_positive(r.s[j]);
+                stage(s_b[0][0], kPlaneB, r.b[j], j, k0, b_cols);
+            }
             __syncthreads();
             if (k0 + kSets * kStep < k_end) {
                 load(r, k0 + kSets * kStep);
