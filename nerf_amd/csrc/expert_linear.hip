@@ -854,8 +854,14 @@ int64_t tile_count(int form, int64_t n, int E, int n_in, int n_out, int tile) {
     const int64_t in = (n_in + tile - 1) / tile, out = (n_out + tile - 1) / tile, rows = n / tile + (E < n ? E : n) / 2;
     return form == kForward ? rows * out : form == kDx ? rows * in : in * out * E;
 }
+// Two tiles of 128 fit a CU: they are taken where they fill one round (20 k rows, 319 -> 256 fp32: 495 tiles, backward 80 us, with
+// tiles of 64 89) or several, and dW's shares of uneven experts only in several (16 k rows, 1001 -> 1001 fp16: 512 tiles,
+// backward 306 us, with tiles of 64 256; 16 k rows, 500 -> 500 fp32: 540 tiles, forward 100 us, 90; 1032 of 1001 -> 1001: 94, 112).
 int tile_size(int form, int64_t n, int E, int n_in, int n_out, int splits) {
-    return n / E > 64 && n_in > 64 && n_out > 64 && tile_count(form, n, E, n_in, n_out, 128) * splits >= 384 ? 128 : 64;
+    if (n / E <= 64 || n_in <= 64 || n_out <= 64) return 64;
+    const bool by_runs = form == kDw && splits == 0;
+    const int64_t tiles = tile_count(form, n, E, n_in, n_out, 128) * (by_runs ? n / E / kPartRows : splits);
+    return (tiles >= 384 && tiles <= 512 && (form != kDw || by_runs)) || tiles >= 960 ? 128 : 64;
 }
 // How dW's sum over an expert's rows is cut (see ExpertArgs): not at all where the outputs alone give 512 workgroups; else by
 // runs, which balances uneven experts, while the parts stay under 1 GiB; else into equal shares.  Wide kernels: equal shares of
@@ -893,7 +899,7 @@ void launch_tile(int dtype, const ExpertArgs& g, hipStream_t stream) {
 }
 template <int FORM>
 void launch_tile(int dtype, const ExpertArgs& g, hipStream_t stream) {
-    if (tile_size(FORM, g.n, g.E, g.n_in, g.n_out, g.splits == 0 ? int(g.n / g.E / kPartRows) : g.splits) == 128) launch_tile<FORM, 128>(dtype, g, stream);
+    if (tile_size(FORM, g.n, g.E, g.n_in, g.n_out, g.splits) == 128) launch_tile<FORM, 128>(dtype, g, stream);
     else launch_tile<FORM, 64>(dtype, g, stream);
 }
 
