@@ -75,6 +75,18 @@ __device__ __forceinline__ float before(const SchulzArgs& s, int t, int64_t base
     if constexpr (__is_same(T, OutMuon)) return (static_cast<const float*>(s.out[t]) + base)[i];
     else return 0.f;
 }
+// four consecutive elements, all of them there; rows may start anywhere
+template <class T>
+__device__ __forceinline__ void emit4(const SchulzArgs& s, int t, int64_t base, unsigned i, const f32x4& v) {
+    typedef typename Elem<T>::type elem;
+    typedef elem vec __attribute__((ext_vector_type(4), aligned(sizeof(elem))));
+    vec* to = reinterpret_cast<vec*>(static_cast<elem*>(s.out[t]) + base + i);
+    vec o;
+    if constexpr (__is_same(T, OutMuon)) o = *to;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = __is_same(T, OutMuon) ? (elem)__fmaf_rn(-s.rate, v[r], s.decay * float(o[r])) : (elem)v[r];
+    *to = o;
+}
 // 4096 / max(norm, eps); NaN for a norm that is not finite
 __device__ __forceinline__ float start_scale(double sum, float eps) {
     double norm = sqrt(sum);
@@ -410,6 +422,8 @@ __global__ __launch_bounds__(512) void schulz_block_kernel(SchulzArgs s, BlockSh
                 const int row = 16 * i + c, col = n + 4 * q;       // X'[row][col ..]
                 if (k < s.steps) {
                     block_store(xs + row * L.pitch + col * 2, plane_x, o);
+                } else if (!tall && row < M && col + 3 < N) {
+                    emit4<T>(s, t, base, unsigned(row) * s.cols + col, o * kUnscale);   // (four stores of 4 B take 10 us more at 64 x 544)
                 } else {
                     unsigned at[4];
                     float old[4];
