@@ -272,9 +272,9 @@ __global__ __launch_bounds__(256, NB == 1 ? 4 : (NB == 2 ? 4 : 3) - __is_same(T,
 // X, A and Q stay in LDS as their terms, rows padded by 16 B: X [2][16 MB][Np] and one square [2][16 MB][16 MB], A and then Q.  Only
 // X itself is kept: A = X X^T reads its rows (k along them), X' = Q X its columns, turned on the way by ds_read_b64_tr_b16.  Eight
 // wavefronts; a tile of A and of A^2 is one wavefront's, which so adds up Q from its own sums; a wavefront writes X' over the
-// 16 columns that it alone read.  What bounds one matrix is the chain of a step's four phases on one CU; its 17 launches through
-// the tiles below are worse at every size: 33 x 48 60 -> 16 us, 92 x 112 66 -> 55, 64 x 300 65 -> 40, 64 x 544 74 -> 66; 2000 of
-// 64 x 64 305 -> 95, 1000 of 128 x 160 862 -> 317.
+// 16 columns that it alone read.  The LDS bounds a step (64 x 544: 1.5 MB of fragment reads, 5.3 of 7.4 us); 17 launches through the
+// tiles below are worse at every size: 33 x 48 60 -> 16 us, 92 x 112 66 -> 47, 64 x 300 65 -> 35, 64 x 544 74 -> 53; 2000 of
+// 64 x 64 305 -> 83, 1000 of 128 x 160 862 -> 245.
 constexpr int kBlockWaves = 8, kLdsBytes = 160 * 1024;
 struct BlockShape {
     int Np, pitch, square, bytes;                  // pitch of X's rows, of the square's, LDS in all; in bytes
@@ -312,7 +312,7 @@ __device__ __forceinline__ void block_store(char* at, int plane, const f32x4& v)
 template <class T, int MB>
 __global__ __launch_bounds__(512) void schulz_block_kernel(SchulzArgs s, BlockShape L, unsigned by_cols) {
     extern __shared__ __align__(16) char smem[];
-    constexpr int kI = MB * MB / kBlockWaves, kAhead = 8;      // tiles of A a wavefront sums
+    constexpr int kJ = MB / 4, kI = MB * MB / kBlockWaves / kJ, kAhead = 8;   // kI x kJ tiles of A are a wavefront's (kI columns)
     const int64_t m = blockIdx.x;
     const int t = int(m / s.per), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
     const int count = s.rows * s.cols;
@@ -368,42 +368,46 @@ __global__ __launch_bounds__(512) void schulz_block_kernel(SchulzArgs s, BlockSh
             if (s.steps == 0) emit<T>(s, t, base, i, v[u] * kUnscale, old[u]);
         }
     }
-    const int j = wave / (MB / kI), first = wave % (MB / kI) * kI;   // rows 16 j .. of A, columns 16 first ..
-    for (int k = 1; k <= s.steps; ++k) {
-        __syncthreads();
-        f32x4 gram[kI] = {}, v[kI] = {};
-        for (int n = 0; n < L.Np; n += 32) {
-            const u32x4 b[2] = {block_rows(xs, L.pitch, 16 * j, n), block_rows(xs + plane_x, L.pitch, 16 * j, n)};
+    const int j0 = wave / (MB / kI) * kJ, i0 = wave % (MB / kI) * kI;   // rows 16 j0 .. of A, columns 16 i0 ..
+    // sums over 32 k of the wavefront's tiles of V V^T, V's rows at `from`
+    auto square = [&](f32x4 (&sum)[kJ][kI], const char* from, int plane, int pitch, int n) {
+        u32x4 b[kJ][2];
 #pragma unroll
-            for (int i = 0; i < kI; ++i) {
-                const u32x4 a[2] = {block_rows(xs, L.pitch, 16 * (first + i), n), block_rows(xs + plane_x, L.pitch, 16 * (first + i), n)};
-                gram[i] = product16(a, b, gram[i]);
-            }
-        }
-        char* mine = sq + (16 * j + c) * L.square + (16 * first + 4 * q) * 2;
+        for (int j = 0; j < kJ; ++j)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) b[j][p] = block_rows(from + p * plane, pitch, 16 * (j0 + j), n);
 #pragma unroll
         for (int i = 0; i < kI; ++i) {
-            gram[i] = gram[i] * kUnscale;
-            block_store(mine + 32 * i, plane_s, gram[i]);
-        }
-        __syncthreads();
+            const u32x4 a[2] = {block_rows(from, pitch, 16 * (i0 + i), n), block_rows(from + plane, pitch, 16 * (i0 + i), n)};
 #pragma unroll
-        for (int n = 0; n < 16 * MB; n += 32) {
-            const u32x4 b[2] = {block_rows(sq, L.square, 16 * j, n), block_rows(sq + plane_s, L.square, 16 * j, n)};
+            for (int j = 0; j < kJ; ++j) sum[j][i] = product16(a, b[j], sum[j][i]);
+        }
+    };
+    char* mine = sq + (16 * j0 + c) * L.square + (16 * i0 + 4 * q) * 2;
+    for (int k = 1; k <= s.steps; ++k) {
+        __syncthreads();
+        f32x4 gram[kJ][kI] = {}, v[kJ][kI] = {};
+        for (int n = 0; n < L.Np; n += 32) square(gram, xs, plane_x, L.pitch, n);
+#pragma unroll
+        for (int j = 0; j < kJ; ++j)
 #pragma unroll
             for (int i = 0; i < kI; ++i) {
-                const u32x4 a[2] = {block_rows(sq, L.square, 16 * (first + i), n), block_rows(sq + plane_s, L.square, 16 * (first + i), n)};
-                v[i] = product16(a, b, v[i]);
+                gram[j][i] = gram[j][i] * kUnscale;
+                block_store(mine + 16 * j * L.square + 32 * i, plane_s, gram[j][i]);
             }
-        }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kI; ++i) {                             // Q without the scale, as in schulz_small_kernel
-            f32x4 poly = (s.b * kUnscale) * gram[i] + (s.c * kUnscale * kUnscale) * v[i];
+        for (int n = 0; n < 16 * MB; n += 32) square(v, sq, plane_s, L.square, n);
+        __syncthreads();
 #pragma unroll
-            for (int r = 0; r < 4; ++r) poly[r] += 16 * (first + i) + 4 * q + r == 16 * j + c ? s.a : 0.f;
-            block_store(mine + 32 * i, plane_s, poly);
-        }
+        for (int j = 0; j < kJ; ++j)
+#pragma unroll
+            for (int i = 0; i < kI; ++i) {                         // Q without the scale, as in schulz_small_kernel
+                f32x4 poly = (s.b * kUnscale) * gram[j][i] + (s.c * kUnscale * kUnscale) * v[j][i];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) poly[r] += 16 * (i0 + i) + 4 * q + r == 16 * (j0 + j) + c ? s.a : 0.f;
+                block_store(mine + 16 * j * L.square + 32 * i, plane_s, poly);
+            }
         __syncthreads();
         for (int n = 16 * wave; n < N; n += 16 * kBlockWaves) {
             u32x4 x[MB / 2][2];
