@@ -15,7 +15,8 @@
 // Two paths, by the shorter side M and the longer side N:
 //   M <= 32, N <= 128                       one wavefront per matrix, everything in registers (schulz_small_kernel);
 //   M <= 64, N <= 544 and M <= 128, N <= 160  one workgroup per matrix, everything in LDS (schulz_block_kernel);
-//   otherwise                               the matrices' terms in the workspace, three launches per step (schulz_product_kernel).
+//   otherwise                               the matrices' terms in the workspace: a launch per step up to 64 x 640 and 128 x 320
+//                                           (schulz_step_kernel), else three (schulz_product_kernel).
 #include "dma_gemm.h"
 #include "split2h.h"
 
@@ -268,6 +269,20 @@ __global__ __launch_bounds__(256, NB == 1 ? 4 : (NB == 2 ? 4 : 3) - __is_same(T,
     }
 }
 
+// The workspace of a matrix, in fp16 elements, M and N padded with zeros (which every product keeps) to the tile: X [2 terms]
+// [M][N] and X^T [2][N][M], both twice (a step reads one and writes the other), A and Q [2][M][M].
+struct LargeShape {
+    int M, N, Mp, Np, tile, chunks, chunk;   // chunks: of the norm's sum, `chunk` elements each
+    __host__ __device__ int64_t x_size() const { return int64_t(2) * Mp * Np; }
+    __host__ __device__ int64_t s_size() const { return int64_t(2) * Mp * Mp; }
+    __host__ __device__ int64_t per_matrix() const { return 4 * x_size() + 2 * s_size(); }
+    __host__ __device__ int64_t x_at(int which) const { return which * 2 * x_size(); }
+    __host__ __device__ int64_t xt_at(int which) const { return which * 2 * x_size() + x_size(); }
+    __host__ __device__ int64_t gram_at() const { return 4 * x_size(); }
+    __device__ float* parts(_Float16* w, int which) const { return reinterpret_cast<float*>(w + x_at(which ^ 1)); }
+    __host__ __device__ int64_t poly_at() const { return 4 * x_size() + s_size(); }
+};
+
 // ---- one workgroup per matrix -------------------------------------------------------------------------------------------
 // X, A and Q stay in LDS as their terms, rows padded by 16 B: X [2][16 MB][Np] and one square [2][16 MB][16 MB], A and then Q.  Only
 // X itself is kept: A = X X^T reads its rows (k along them), X' = Q X its columns, turned on the way by ds_read_b64_tr_b16.  Eight
@@ -301,12 +316,32 @@ __device__ __forceinline__ f32x4 product16(const u32x4 (&a)[2], const u32x4 (&b)
     c = mfma_dma<false>(a[1], b[0], c);
     return mfma_dma<false>(a[0], b[0], c);
 }
-__device__ __forceinline__ void block_store(char* at, int plane, const f32x4& v) {
+__device__ __forceinline__ void block_store(char* at, int64_t plane, const f32x4& v) {
     unsigned h0, l0, h1, l1;
     split_pair_h2(v[0], v[1], h0, l0);
     split_pair_h2(v[2], v[3], h1, l1);
     *reinterpret_cast<u32x2*>(at) = (u32x2){h0, h1};
     *reinterpret_cast<u32x2*>(at + plane) = (u32x2){l0, l1};
+}
+
+// X'[row][col ..] to the output, what of it is there
+template <class T>
+__device__ __forceinline__ void block_emit(const SchulzArgs& s, int t, int64_t base, bool tall, int M, int N, int row, int col, const f32x4& v) {
+    if (!tall && row < M && col + 3 < N) {
+        emit4<T>(s, t, base, unsigned(row) * s.cols + col, v);       // (four stores of 4 B take 10 us more at 64 x 544)
+        return;
+    }
+    unsigned at[4];
+    float old[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const unsigned y = row < M ? row : M - 1, x = col + r < N ? col + r : N - 1;
+        at[r] = tall ? x * s.cols + y : y * s.cols + x;
+        old[r] = before<T>(s, t, base, at[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (row < M && col + r < N) emit<T>(s, t, base, at[r], v[r], old[r]);
 }
 
 template <class T, int MB>
@@ -426,40 +461,148 @@ __global__ __launch_bounds__(512) void schulz_block_kernel(SchulzArgs s, BlockSh
                 const int row = 16 * i + c, col = n + 4 * q;       // X'[row][col ..]
                 if (k < s.steps) {
                     block_store(xs + row * L.pitch + col * 2, plane_x, o);
-                } else if (!tall && row < M && col + 3 < N) {
-                    emit4<T>(s, t, base, unsigned(row) * s.cols + col, o * kUnscale);   // (four stores of 4 B take 10 us more at 64 x 544)
                 } else {
-                    unsigned at[4];
-                    float old[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const unsigned y = row < M ? row : M - 1, x = col + r < N ? col + r : N - 1;
-                        at[r] = tall ? x * s.cols + y : y * s.cols + x;
-                        old[r] = before<T>(s, t, base, at[r]);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (row < M && col + r < N) emit<T>(s, t, base, at[r], o[r] * kUnscale, old[r]);
+                    block_emit<T>(s, t, base, tall, M, N, row, col, o * kUnscale);
                 }
             }
         }
     }
 }
 
-// ---- larger matrices ----------------------------------------------------------------------------------------------------
-// The workspace of a matrix, in fp16 elements, M and N padded with zeros (which every product keeps) to the tile: X [2 terms]
-// [M][N] and X^T [2][N][M], both twice (a step reads one and writes the other), A and Q [2][M][M].
-struct LargeShape {
-    int M, N, Mp, Np, tile, chunks, chunk;   // chunks: of the norm's sum, `chunk` elements each
-    __host__ __device__ int64_t x_size() const { return int64_t(2) * Mp * Np; }
-    __host__ __device__ int64_t s_size() const { return int64_t(2) * Mp * Mp; }
-    __host__ __device__ int64_t per_matrix() const { return 4 * x_size() + 2 * s_size(); }
-    __host__ __device__ int64_t x_at(int which) const { return which * 2 * x_size(); }
-    __host__ __device__ int64_t xt_at(int which) const { return which * 2 * x_size() + x_size(); }
-    __host__ __device__ int64_t gram_at() const { return 4 * x_size(); }
-    __device__ float* parts(_Float16* w, int which) const { return reinterpret_cast<float*>(w + x_at(which ^ 1)); }
-    __host__ __device__ int64_t poly_at() const { return 4 * x_size() + s_size(); }
+// A whole step in one launch, for matrices of up to 128 rows that the kernel above has no LDS for: a workgroup per 64 columns of X.
+// Each sums all of A = X X^T itself (X's 64-column pieces pass through a ring in LDS, its own piece stays), squares it, and
+// multiplies its own columns: one launch per step for three, at the price of A's sums once per workgroup (0.7 us per piece at 128
+// rows).  One round of workgroups, up to 10 pieces at 64 rows and 5 at 128: 64 x 600 80 -> 45 us, 128 x 200 73 -> 64, 2 of 128 x 283
+// 75 -> 70, 50 of 128 x 300 106 -> 91; past that the tiles below win (128 x 640 85 us, 96 this way).
+template <int MB> struct StepShape {
+    typedef DmaSide<kRows, 16 * MB, 64, 2, kBlockWaves> Side;
+    static constexpr int kSquare = MB * 32 + 16, kSquareBytes = 2 * 16 * MB * kSquare;
+    static constexpr int kLds = Side::kBytes + (2 * Side::kBytes > kSquareBytes ? 2 * Side::kBytes : kSquareBytes);   // own piece; ring, then the square
 };
+template <class T, int MB, bool LAST>
+__global__ __launch_bounds__(512) void schulz_step_kernel(SchulzArgs s, LargeShape L, _Float16* __restrict__ work, int which, int share) {
+    typedef StepShape<MB> Shape;
+    typedef typename Shape::Side Side;
+    extern __shared__ __align__(16) char smem[];
+    constexpr int kJ = MB / 4, kI = MB * MB / kBlockWaves / kJ, kSquare = Shape::kSquare, kPlaneS = 16 * MB * kSquare;
+    const int pieces = L.Np / 64, unit = int(blockIdx.x & 7) * share + int(blockIdx.x >> 3);
+    if (unit >= int(s.batch) * pieces) return;
+    const int64_t m = unit / pieces;
+    const int own = unit % pieces;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+    _Float16* w = work + m * L.per_matrix();
+    const int64_t plane_x = int64_t(L.Mp) * L.Np;
+    char *ring = smem + Side::kBytes, *sq = ring;
+    const unsigned lds = lds_addr(smem) + wave * (Side::kPieces * 1024);
+    Side side;
+    side.start_rows(wave, lane, w + L.x_at(which), plane_x * 2, [&](int row) { return unsigned(row * L.Np) * 2u; });
+    // piece i of the walk: its own first, then the others in their order through the two slots of the ring
+    auto issue = [&](int i) {
+        const int piece = i == 0 ? own : i <= own ? i - 1 : i;
+        const unsigned to = lds + (i == 0 ? 0 : Side::kBytes * (1 + ((i - 1) & 1)));
+#pragma unroll
+        for (int j = 0; j < Side::kPieces; ++j) side.issue(j, wave, lane, to, 64, int64_t(piece) * 128, nullptr, 0u);
+    };
+    for (int i = 0; i < 3 && i < pieces; ++i) issue(i);
+    const int j0 = wave / (MB / kI) * kJ, i0 = wave % (MB / kI) * kI;   // rows 16 j0 .. of A, columns 16 i0 ..
+    f32x4 gram[kJ][kI] = {}, v[kJ][kI] = {};
+    for (int i = 0; i < pieces; ++i) {
+        // piece i has landed: one more may be in flight, two behind the first
+        if (i == 0 && pieces >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Side::kPieces) : "memory");
+        else if (i + 1 < pieces) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Side::kPieces) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        const char* from = i == 0 ? smem : ring + ((i - 1) & 1) * Side::kBytes;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            u32x4 b[kJ][2];
+#pragma unroll
+            for (int j = 0; j < kJ; ++j)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) b[j][p] = Side::frag(from + p * Side::kPlane, 16 * j0, j, kk, c, q);
+#pragma unroll
+            for (int a_i = 0; a_i < kI; ++a_i) {
+                const u32x4 a[2] = {Side::frag(from, 16 * i0, a_i, kk, c, q), Side::frag(from + Side::kPlane, 16 * i0, a_i, kk, c, q)};
+#pragma unroll
+                for (int j = 0; j < kJ; ++j) gram[j][a_i] = product16(a, b[j], gram[j][a_i]);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();                                   // every wavefront holds what it read of this slot
+        if (i >= 1 && i + 2 < pieces) issue(i + 2);
+    }
+    char* mine = sq + (16 * j0 + c) * kSquare + (16 * i0 + 4 * q) * 2;
+#pragma unroll
+    for (int j = 0; j < kJ; ++j)
+#pragma unroll
+        for (int i = 0; i < kI; ++i) {
+            gram[j][i] = gram[j][i] * kUnscale;
+            block_store(mine + 16 * j * kSquare + 32 * i, kPlaneS, gram[j][i]);
+        }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 16 * MB; n += 32) {
+        u32x4 b[kJ][2];
+#pragma unroll
+        for (int j = 0; j < kJ; ++j)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) b[j][p] = block_rows(sq + p * kPlaneS, kSquare, 16 * (j0 + j), n);
+#pragma unroll
+        for (int i = 0; i < kI; ++i) {
+            const u32x4 a[2] = {block_rows(sq, kSquare, 16 * (i0 + i), n), block_rows(sq + kPlaneS, kSquare, 16 * (i0 + i), n)};
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) v[j][i] = product16(a, b[j], v[j][i]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kJ; ++j)
+#pragma unroll
+        for (int i = 0; i < kI; ++i) {                                  // Q without the scale, as in schulz_small_kernel
+            f32x4 poly = (s.b * kUnscale) * gram[j][i] + (s.c * kUnscale * kUnscale) * v[j][i];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) poly[r] += 16 * (i0 + i) + 4 * q + r == 16 * (j0 + j) + c ? s.a : 0.f;
+            block_store(mine + 16 * j * kSquare + 32 * i, kPlaneS, poly);
+        }
+    __syncthreads();
+    // 16 columns and half of the rows per wavefront
+    const int n = wave % 4 * 16, first = wave / 4 * (MB / 2);
+    u32x4 x[MB / 2][2];
+#pragma unroll
+    for (int kk = 0; kk < MB / 2; ++kk)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            s16x4_g part[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int row = 32 * kk + 8 * q + 4 * u + (c >> 2), octet = (n / 8 + ((c & 3) >> 1)) ^ Side::swizzle(row);
+                part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4_g*)(smem + p * Side::kPlane + row * 128 + octet * 16 + (c & 1) * 8));
+            }
+            x[kk][p] = __builtin_bit_cast(u32x4, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    const int t = int(m / s.per), col = own * 64 + n + 4 * q;
+    const int64_t base = (m % s.per) * int64_t(s.rows) * s.cols;
+    const bool tall = s.rows > s.cols;
+#pragma unroll
+    for (int i = 0; i < MB / 2; ++i) {
+        f32x4 o = {};
+#pragma unroll
+        for (int kk = 0; kk < MB / 2; ++kk) {
+            const u32x4 b[2] = {block_rows(sq, kSquare, 16 * (first + i), 32 * kk), block_rows(sq + kPlaneS, kSquare, 16 * (first + i), 32 * kk)};
+            o = product16(x[kk], b, o);
+        }
+        const int row = 16 * (first + i) + c;                           // X'[row][col ..]
+        if constexpr (!LAST) {
+            block_store(reinterpret_cast<char*>(w + L.x_at(which ^ 1) + int64_t(row) * L.Np + col), plane_x * 2, o);
+        } else {
+            block_emit<T>(s, t, base, tall, L.M, L.N, row, col, o * kUnscale);
+        }
+    }
+}
+
+// ---- larger matrices ----------------------------------------------------------------------------------------------------
 constexpr int kNormBatch = 8;       // elements of a thread at a time, all loaded before the first is used
 
 // |G|_F^2 in L.chunks parts; Muon: the momentum's update
@@ -835,6 +978,28 @@ int launch_gram(const SchulzArgs& s, const LargeShape& L, _Float16* work, int wh
                                                              : launch_tiles<Out32, kGram, 64>(s, L, work, which, stream);
 }
 
+bool step_path(const SchulzArgs& s, const LargeShape& L) {
+    return L.Mp <= 128 && L.Np <= (L.Mp == 64 ? 640 : 320) && s.batch * (L.Np / 64) <= 256;
+}
+template <class T, int MB, bool LAST>
+int launch_step(const SchulzArgs& s, const LargeShape& L, _Float16* work, int which, hipStream_t stream) {
+    auto kernel = &schulz_step_kernel<T, MB, LAST>;
+    constexpr int lds = StepShape<MB>::kLds;
+    if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+        return NRF_ERR_LAUNCH;
+    const int pieces = L.Np / 64, whole = int((s.batch + 7) / 8) * pieces;   // whole matrices per XCD while they fit its CUs
+    const int share = whole <= 32 ? whole : (int(s.batch) * pieces + 7) / 8;
+    kernel<<<8 * share, 512, lds, stream>>>(s, L, work, which, share);
+    return NRF_OK;
+}
+template <class T, int MB>
+int run_steps(const SchulzArgs& s, const LargeShape& L, _Float16* work, hipStream_t stream) {
+    for (int k = 0; k < s.steps; ++k) {
+        const int st = k + 1 < s.steps ? launch_step<Out32, MB, false>(s, L, work, k & 1, stream) : launch_step<T, MB, true>(s, L, work, k & 1, stream);
+        if (st != NRF_OK) return st;
+    }
+    return NRF_OK;
+}
 template <class T>
 int run_large(const SchulzArgs& s, const LargeShape& L, double* parts, _Float16* work, hipStream_t stream) {
     const dim3 cover(unsigned((s.rows > s.cols ? L.Mp : L.Np) / 64), unsigned((s.rows > s.cols ? L.Np : L.Mp) / 64), unsigned(s.batch));
@@ -844,6 +1009,7 @@ int run_large(const SchulzArgs& s, const LargeShape& L, double* parts, _Float16*
         return NRF_OK;
     }
     schulz_start_kernel<T><<<cover, 256, 0, stream>>>(s, L, parts, work);
+    if (step_path(s, L)) return L.Mp == 64 ? run_steps<T, 4>(s, L, work, stream) : run_steps<T, 8>(s, L, work, stream);
     for (int k = 0; k < s.steps; ++k) {
         int st = launch_gram(s, L, work, k & 1, stream);   // the output's type matters to kLast alone
         if (st == NRF_OK) st = launch_product<Out32, kPoly>(s, L, work, k & 1, stream);

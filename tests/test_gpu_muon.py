@@ -61,7 +61,8 @@ def gradient(batch, m, n, seed=0, dtype=torch.float32, scale=1e-3):
 
 SHAPES = [(1, 1, 1), (3, 1, 7), (2, 7, 1), (5, 2, 2), (4, 31, 33), (9, 32, 32), (7, 32, 63), (6, 63, 32), (5, 32, 64), (3, 20, 128),
           (3, 128, 32), (2, 17, 100), (1, 32, 129), (2, 33, 33), (2, 40, 7), (2, 64, 64), (2, 65, 130), (1, 130, 65), (3, 64, 544), (2, 545, 64), (1, 544, 33), (2, 33, 48), (3, 128, 160), (2, 160, 127), (1, 161, 128), (2, 97, 97), (1, 1, 544),
-          (2, 500, 1), (1, 129, 129), (2, 96, 112), (2, 128, 283),
+          (2, 500, 1), (1, 129, 129), (2, 96, 112), (3, 100, 640), (2, 640, 101), (1, 64, 576), (5, 33, 601), (2, 641, 70), (1, 128, 192),
+          (40, 128, 165), (90, 120, 190), (17, 10, 600), (2, 128, 283),
           (1, 283, 128), (3, 256, 256), (1, 513, 600), (1, 600, 514), (1, 5, 700), (300, 16, 16)]
 
 
@@ -162,7 +163,7 @@ def muon64(p, g, m, lr, mu, nesterov, wd, clip, scale, dtype=torch.float64):
     return (1 - lr * wd) * p.to(dtype) - lr * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5 * o, m, o
 
 
-@pytest.mark.parametrize("shape", [(5, 32, 63), (3, 63, 32), (2, 128, 283), (2, 283, 128), (1, 256, 256), (4, 3, 128), (2, 600, 520), (3, 64, 300), (2, 150, 110)], ids=str)
+@pytest.mark.parametrize("shape", [(5, 32, 63), (3, 63, 32), (2, 128, 283), (2, 283, 128), (1, 256, 256), (4, 3, 128), (2, 600, 520), (3, 64, 300), (2, 150, 110), (3, 62, 620), (4, 333, 99)], ids=str)
 @pytest.mark.parametrize("nesterov", [True, False])
 def test_muon_update(shape, nesterov):
     gen = torch.Generator().manual_seed(7)
