@@ -42,10 +42,10 @@ struct DmaSide {
     static constexpr int kPlane = R * KS * 2, kBytes = P * kPlane, kPieces = kBytes / 1024 / WAVES;
     static constexpr int kSlots = MODE == kRows ? KS / 8 : R / 8;        // octets of an LDS row
     static_assert(kBytes % (1024 * WAVES) == 0 && kPlane % 1024 == 0, "whole pieces per wavefront");
-    static_assert(64 % kSlots == 0 && (MODE == kRows || P == 1), "layout");
+    static_assert(64 % kSlots == 0 && (MODE == kRows ? KS == 64 : P == 1), "layout");
 
     static __device__ __forceinline__ int swizzle(int row) {
-        if (MODE == kRows) return KS == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+        if (MODE == kRows) return (row >> 1) & 7;
         if (R == 64) return ((row >> 1) & 1) * 2 + ((row >> 3) & 1) * 4;
         return (row & 3) * 2 + ((row >> 3) & 1) * 8;
     }
@@ -120,14 +120,13 @@ __device__ __forceinline__ f32x4 mfma_dma(const u32x4_g& a, const u32x4_g& b, co
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_g, a), __builtin_bit_cast(f16x8_g, b), c, 0, 0, 0);
 }
 
-template <bool BF16, int MODE_A, int MODE_B, int TA, int TB, int WA, int WB, int P, int KS, int STA, int STB, bool SUM_B = false>
+template <bool BF16, int MODE_A, int MODE_B, int TA, int TB, int WA, int WB, int P, int ST, bool SUM_B = false>
 struct DmaGemm {
-    static constexpr int kWaves = WA * WB, kThreads = 64 * kWaves;
+    static constexpr int KS = 64, kWaves = WA * WB, kThreads = 64 * kWaves;
     static constexpr int kMA = TA / WA / 16, kMB = TB / WB / 16;             // 16 x 16 accumulators of a wavefront
     typedef DmaSide<MODE_A, TA, KS, P, kWaves> A;
     typedef DmaSide<MODE_B, TB, KS, P, kWaves> B;
-    static constexpr int kLds = STA * A::kBytes + STB * B::kBytes, kPieces = A::kPieces + B::kPieces;
-    static_assert(STA <= STB && KS == 64, "B's ring is the longer one; two halves");
+    static constexpr int kStage = A::kBytes + B::kBytes, kLds = ST * kStage, kPieces = A::kPieces + B::kPieces;
 
     A a;
     B b;
@@ -142,30 +141,26 @@ struct DmaGemm {
     __device__ __forceinline__ int wave_a() const { return (wave % WA) * (TA / WA); }
     __device__ __forceinline__ int wave_b() const { return (wave / WA) * (TB / WB); }
 
-    // piece j of step k, to `slot` of the operand's ring: A's STA steps at the start of LDS, B's STB steps behind them
-    __device__ __forceinline__ void issue_a(int j, unsigned lds, int slot, int k, int k_count, const int* list) const {
-        a.issue(j, wave, lane, lds + slot * A::kBytes + wave * (A::kPieces * 1024), k_count - k * KS, k * step_a, list + k * KS, pitch_a);
-    }
-    __device__ __forceinline__ void issue_b(int j, unsigned lds, int slot, int k, int k_count, const int* list) const {
-        b.issue(j, wave, lane, lds + STA * A::kBytes + slot * B::kBytes + wave * (B::kPieces * 1024), k_count - k * KS, k * step_b, list + k * KS, pitch_b);
+    // piece j of step k, to the slot at lds
+    __device__ __forceinline__ void issue(int j, unsigned lds, int k, int k_count, const int* list) const {
+        if (j < A::kPieces)
+            a.issue(j, wave, lane, lds + wave * (A::kPieces * 1024), k_count - k * KS, k * step_a, list + k * KS, pitch_a);
+        else
+            b.issue(j - A::kPieces, wave, lane, lds + A::kBytes + wave * (B::kPieces * 1024), k_count - k * KS, k * step_b, list + k * KS, pitch_b);
     }
 
     struct Frags {
         u32x4_g a[kMA][P], b[kMB][P];
     };
     static constexpr int kReads = P * (kMA + kMB);
-    struct Slots {
-        int a, b;
-        __device__ __forceinline__ Slots next() const { return {a + 1 == STA ? 0 : a + 1, b + 1 == STB ? 0 : b + 1}; }
-    };
-    __device__ __forceinline__ void read(int i, Frags& f, const char* smem, Slots s, int kk) const {   // fragment i of the 32 k
+    __device__ __forceinline__ void read(int i, Frags& f, const char* stage, int kk) const {   // fragment i of the 32 k
         const int c = lane & 15, q = lane >> 4, p = i / (kMA + kMB), m = i % (kMA + kMB);
-        if (m < kMB) f.b[m][p] = B::frag(smem + STA * A::kBytes + s.b * B::kBytes + p * B::kPlane, wave_b(), m, kk, c, q);
-        else f.a[m - kMB][p] = A::frag(smem + s.a * A::kBytes + p * A::kPlane, wave_a(), m - kMB, kk, c, q);
+        if (m < kMB) f.b[m][p] = B::frag(stage + A::kBytes + p * B::kPlane, wave_b(), m, kk, c, q);
+        else f.a[m - kMB][p] = A::frag(stage + p * A::kPlane, wave_a(), m - kMB, kk, c, q);
     }
-    __device__ __forceinline__ void read(Frags& f, const char* smem, Slots s, int kk) const {
+    __device__ __forceinline__ void read(Frags& f, const char* stage, int kk) const {
 #pragma unroll
-        for (int i = 0; i < kReads; ++i) read(i, f, smem, s, kk);
+        for (int i = 0; i < kReads; ++i) read(i, f, stage, kk);
     }
     // the k of a last, partial step that lie past the end
     __device__ __forceinline__ void mask(Frags& f, int left) const {
@@ -202,9 +197,9 @@ struct DmaGemm {
 
     // `list`: the rows of k for kGather sides (in LDS, complete before the call).  with_sum: sum[mb][0] += sum over k of B.
     // A step is two halves of 32 k.  The second half's fragments are read while the first half is multiplied; once every
-    // wavefront holds them (first barrier) the step's slots are refilled with A's step k + STA and B's step k + STB, the DMA
-    // issued between the rest of the first half's MFMAs.  Once the next step has landed (counted vmcnt, second barrier) its
-    // first half is read between the second half's MFMAs.  A's DMA so has STA - 3/4 steps of time to arrive, B's STB - 3/4.
+    // wavefront holds them (first barrier) the step's slot is refilled with step k + ST, the DMA issued between the rest of the
+    // first half's MFMAs.  Once the next step has landed (counted vmcnt, second barrier) its first half is read between the
+    // second half's MFMAs.
     __device__ __forceinline__ void run(const char* smem, int k_count, f32x4 (&acc)[kMA][kMB], const int* list = nullptr,
                                         f32x4 (*sum)[kMB] = nullptr, bool with_sum = false) {
         if (__builtin_amdgcn_readfirstlane(idle)) walk<false>(smem, k_count, acc, list, sum, false);
@@ -217,41 +212,34 @@ struct DmaGemm {
         const int k_steps = (k_count + KS - 1) / KS;
         if (k_steps == 0) return;
 #pragma unroll
-        for (int s = 0; s < STB; ++s)
-            if (s < k_steps) {
-                if (s < STA)
+        for (int s = 0; s < ST; ++s)
+            if (s < k_steps)
 #pragma unroll
-                    for (int j = 0; j < A::kPieces; ++j) issue_a(j, lds, s, s, k_count, list);
-#pragma unroll
-                for (int j = 0; j < B::kPieces; ++j) issue_b(j, lds, s, s, k_count, list);
-            }
-        if (k_steps >= STB) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(A::kPieces * (STA - 1) + B::kPieces * (STB - 1)) : "memory");
+                for (int j = 0; j < kPieces; ++j) issue(j, lds + s * kStage, s, k_count, list);
+        if (k_steps >= ST) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kPieces * (ST - 1)) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         Frags f0, f1;
-        Slots at{0, 0};
-        if (WORK) read(f0, smem, at, 0);
-        int k = 0;
-        // steps that refill both rings; A's only; none; the last
-        for (; k + STB < k_steps; ++k) step<WORK, true, true, true>(smem, lds, k, k_count, at, f0, f1, acc, list, sum, with_sum);
-        if constexpr (STA < STB)
-            for (; k + STA < k_steps; ++k) step<WORK, true, false, true>(smem, lds, k, k_count, at, f0, f1, acc, list, sum, with_sum);
-        for (; k + 1 < k_steps; ++k) step<WORK, false, false, true>(smem, lds, k, k_count, at, f0, f1, acc, list, sum, with_sum);
-        step<WORK, false, false, false>(smem, lds, k, k_count, at, f0, f1, acc, list, sum, with_sum);
+        if (WORK) read(f0, smem, 0);
+        int slot = 0, k = 0;
+        // steps that refill their slot; steps without a step ST on; the last
+        for (; k + ST < k_steps; ++k) step<WORK, true, true>(smem, lds, k, k_count, slot, f0, f1, acc, list, sum, with_sum);
+        for (; k + 1 < k_steps; ++k) step<WORK, false, true>(smem, lds, k, k_count, slot, f0, f1, acc, list, sum, with_sum);
+        step<WORK, false, false>(smem, lds, k, k_count, slot, f0, f1, acc, list, sum, with_sum);
     }
-    template <bool WORK, bool FILL_A, bool FILL_B, bool NEXT>
-    __device__ __forceinline__ void step(const char* smem, unsigned lds, int k, int k_count, Slots& at, Frags& f0, Frags& f1,
+    template <bool WORK, bool FILL, bool NEXT>
+    __device__ __forceinline__ void step(const char* smem, unsigned lds, int k, int k_count, int& slot, Frags& f0, Frags& f1,
                                          f32x4 (&acc)[kMA][kMB], const int* list, f32x4 (*sum)[kMB], bool with_sum) const {
-        const Slots next = at.next();
+        const int next = slot + 1 == ST ? 0 : slot + 1;
         constexpr int kHalf = kMA / 2, D = (kPieces + kMA - kHalf - 1) / (kMA - kHalf), R = (kReads + kMA - 1) / kMA;
         if (WORK) {
-            read(f1, smem, at, 1);
+            read(f1, smem + slot * kStage, 1);
             __builtin_amdgcn_sched_barrier(0);
             if (!NEXT && k_count - k * KS < KS) mask(f0, k_count - k * KS), mask(f1, k_count - k * KS - 32);
 #pragma unroll
             for (int ma = 0; ma < kHalf; ++ma) multiply(ma, f0, acc);
         }
-        if (FILL_A) {   // every wavefront holds all of this step
+        if (FILL) {     // every wavefront holds all of this step
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
@@ -261,16 +249,12 @@ struct DmaGemm {
             if (WORK) multiply(ma, f0, acc);
 #pragma unroll
             for (int j = 0; j < kPieces; ++j)
-                if (FILL_A && j / D == ma - kHalf) {
-                    if (j < A::kPieces) issue_a(j, lds, at.a, k + STA, k_count, list);
-                    else if (FILL_B) issue_b(j - A::kPieces, lds, at.b, k + STB, k_count, list);
-                }
+                if (FILL && j / D == ma - kHalf) issue(j, lds + slot * kStage, k + ST, k_count, list);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (WORK) sum_up(f0, sum, with_sum);
-        if (NEXT) {     // the next step has landed
-            if (FILL_B) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(A::kPieces * (STA - 1) + B::kPieces * (STB - 1)) : "memory");
-            else if (FILL_A) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(A::kPieces * (STA - 1)) : "memory");
+        if (NEXT) {     // the next step has landed; near the end fewer are in flight, and all are waited for
+            if (FILL) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kPieces * (ST - 1)) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
         }
@@ -279,11 +263,11 @@ struct DmaGemm {
             if (WORK) multiply(ma, f1, acc);
 #pragma unroll
             for (int i = 0; i < kReads; ++i)
-                if (WORK && NEXT && i / R == ma) read(i, f0, smem, next, 0);
+                if (WORK && NEXT && i / R == ma) read(i, f0, smem + next * kStage, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (WORK) sum_up(f1, sum, with_sum);
-        at = next;
+        slot = next;
     }
 };
 

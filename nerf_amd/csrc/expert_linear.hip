@@ -414,7 +414,7 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g, int a_ti
 constexpr int kWideA = 256;
 template <class T, int FORM, int ROWS> struct WideRows {
     static constexpr int kWA = ROWS == 256 ? 2 : 4, kST = ROWS == 256 ? 2 : ROWS == 128 ? 3 : 4;
-    typedef DmaGemm<__is_same(T, Bf16), FORM == kForward ? kRows : kCols, kRows, kWideA, ROWS, kWA, 8 / kWA, 1, 64, kST, kST> Gemm;
+    typedef DmaGemm<__is_same(T, Bf16), FORM == kForward ? kRows : kCols, kRows, kWideA, ROWS, kWA, 8 / kWA, 1, kST> Gemm;
 };
 constexpr int kWideLds = 4 * (256 + 64) * 128;   // of the 256 x 64 form, the largest
 
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(512) void expert_wide_rows_kernel(ExpertArgs g, int
 constexpr int kListRows = 4096;
 template <class T> struct WideDw {
     static constexpr int kA = 256, kB = 128;
-    typedef DmaGemm<__is_same(T, Bf16), kGather, kGather, kA, kB, 4, 2, 1, 64, 2, 2, true> Gemm;
+    typedef DmaGemm<__is_same(T, Bf16), kGather, kGather, kA, kB, 4, 2, 1, 2, true> Gemm;
     static constexpr int kLds = Gemm::kLds + kListRows * 4;
 };
 template <class T>

@@ -697,7 +697,7 @@ __global__ __launch_bounds__(256) void schulz_start_kernel(SchulzArgs s, LargeSh
 enum Product { kGram, kPoly, kApply, kLast, kGramPart };
 
 // 64 x 64 or 128 x 128 outputs by four wavefronts
-template <int TT> using SchulzGemm = DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 64, 2, 2>;
+template <int TT> using SchulzGemm = DmaGemm<false, kRows, kRows, TT, TT, 2, 2, 2, 2>;
 
 // words[i] = {hi, lo} of eight consecutive elements -> 16 B of each plane
 __device__ __forceinline__ void store_octet(_Float16* dst, int64_t plane, const unsigned (&w)[8]) {
