@@ -126,8 +126,9 @@ class _ExpertLinear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, plan, activation):
         y = _forward(x.detach(), weight.detach(), None if bias is None else bias.detach(), plan, activation)
         ctx.plan, ctx.activation = plan, activation
-        # the plan's buffer among them: autograd then notices a write to the views that the plan hands out
-        ctx.save_for_backward(x, weight, y if activation == "relu" else None, plan.buffer)
+        # the plan's buffer among them: autograd then notices a write to the views that the plan hands out (a buffer made in
+        # inference mode counts no writes and cannot be saved)
+        ctx.save_for_backward(x, weight, y if activation == "relu" else None, None if plan.buffer.is_inference() else plan.buffer)
         return y
 
     @staticmethod

@@ -89,4 +89,5 @@ def muon_update(params, grads, momentum_buffers, lr: float = 0.02, momentum: flo
                   "nrf_muon_update")
     bump = torch.autograd.graph.increment_version    # the kernel writes behind torch's back
     for t in list(params) + list(momentum_buffers):
-        bump(t)
+        if not t.is_inference():                     # (those count no versions)
+            bump(t)

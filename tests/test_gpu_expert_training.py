@@ -159,3 +159,23 @@ def test_autograd_and_the_update():
         muon_update(p, p.grad, m, lr=0.05, momentum=0.9, clip_value=1e4)
     net.step()
     assert all(torch.equal(p, q) for p, q in zip(net.w, other.w))
+
+
+def test_inference_mode():
+    """a plan made there serves a training step; an update of tensors made there works"""
+    net = Net(300, 4, (63, 32, 4), torch.float32, 8)
+    with torch.inference_mode():
+        plan = expert_plan(net.index, net.E)
+        serving = expert_linear(net.x, net.w[0], net.b[0], plan, "relu")
+        p, g, m = (torch.ones(40, 40, device=DEV) * v for v in (1.0, 0.5, 0.0))
+        muon_update(p, g, m)
+        assert bool((p != 1).any())
+    w = net.w[0].clone().requires_grad_()
+    y = expert_linear(net.x, w, net.b[0], plan, "relu")
+    assert torch.equal(y, serving)
+    y.sum().backward()
+    _, dw, _ = expert_linear_backward(torch.ones_like(y), net.x, net.w[0], plan, y=y.detach(), activation="relu")
+    assert torch.equal(w.grad, dw)
+    with torch.inference_mode():
+        muon_update(net.w[0], dw, net.m[0])
+    assert not torch.equal(net.w[0], w.detach())
