@@ -15,6 +15,13 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # steep at 0 (weak directions catch u
 MAX_TENSORS = 32                           # of one nrf_muon_update call
 
 
+def _written(tensors) -> None:
+    """the kernels write behind torch's back: autograd's version counters (tensors of inference mode have none)"""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _workspace(batch: int, rows: int, cols: int, device):
     need = lib().nrf_newton_schulz_workspace_bytes(batch, rows, cols)
     if need < 0:
@@ -45,6 +52,7 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, ep
     with _on(g.device):
         check(lib().nrf_newton_schulz(_ptr(g), _ptr(out), batch, rows, cols, DTYPES[g.dtype], int(steps), a, b, c, eps,
                                       _ptr(work), need, _stream(g)), "nrf_newton_schulz")
+    _written([out])
     return out
 
 
@@ -87,7 +95,4 @@ def muon_update(params, grads, momentum_buffers, lr: float = 0.02, momentum: flo
             check(lib().nrf_muon_update(*arrays, n, batch, rows, cols, grad_scale, clip_value, momentum, int(nesterov), lr,
                                         weight_decay, int(steps), a, b, c, eps, _ptr(work), need, _stream(params[0])),
                   "nrf_muon_update")
-    bump = torch.autograd.graph.increment_version    # the kernel writes behind torch's back
-    for t in list(params) + list(momentum_buffers):
-        if not t.is_inference():                     # (those count no versions)
-            bump(t)
+    _written((*params, *momentum_buffers))

@@ -10,7 +10,7 @@ import torch
 
 from nerf_amd.expert_ops import expert_linear, expert_linear_backward, expert_plan
 from nerf_amd.muon_ops import COEFFICIENTS as ABC
-from nerf_amd.muon_ops import muon_update
+from nerf_amd.muon_ops import muon_update, newton_schulz
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -179,3 +179,16 @@ def test_inference_mode():
     with torch.inference_mode():
         muon_update(net.w[0], dw, net.m[0])
     assert not torch.equal(net.w[0], w.detach())
+
+
+@pytest.mark.parametrize("how", ["update", "in place"])
+def test_weights_written_between_forward_and_backward_are_noticed(how):
+    net = Net(300, 4, (63, 32, 4), torch.float32, 9)
+    x = net.x.clone().requires_grad_()
+    y = expert_linear(x, net.w[0], net.b[0], expert_plan(net.index, net.E))
+    if how == "update":
+        muon_update(net.w[0], torch.ones_like(net.w[0]), net.m[0])
+    else:
+        newton_schulz(net.w[0], out=net.w[0])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
