@@ -354,7 +354,12 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g, int a_ti
 #pragma unroll
                     for (int i = 0; i < P; ++i) fa[i] = fragment(s_a[d][i], wa, ma, a_cols);
 #pragma unroll
-                    for (int mb = 0; mb < M; ++mb) acc[ma][mb] = mfma_terms<T>(fa, fb[mb], acc[ma][mb]);
+                    for (int mb = 0; mb < M; ++mb) {
+                        // fp32: a step's six products among themselves, then one rounding at the size of the whole sum, not six
+                        // (200 rows of 1000 -> 300: 1.2e-7 off float64 for 4.8e-7; dW's tile of 128 has no registers left for it)
+                        if constexpr (P == 3 && (FORM != kDw || TT == 64)) acc[ma][mb] = acc[ma][mb] + mfma_terms<T>(fa, fb[mb], (f32x4){});
+                        else acc[ma][mb] = mfma_terms<T>(fa, fb[mb], acc[ma][mb]);
+                    }
                 }
                 if (with_db)
 #pragma unroll
