@@ -132,7 +132,8 @@ SHAPES = [  # n, E, n_in, n_out, kind
     (129, 2, 130, 257, "one"), (64, 3, 16, 8, "none"), (2500, 8, 96, 100, "skew"), (515, 1, 1024, 40, "uniform"),
     (700, 2, 512, 640, "uniform"), (900, 3, 264, 136, "outside"), (1300, 2, 128, 520, "skew"), (5000, 1, 136, 128, "one"),
     (640, 8, 200, 328, "skew"), (700, 3, 256, 131, "outside"), (3000, 2, 136, 517, "skew"), (300, 4, 131, 259, "uniform"),
-    (90, 2, 777, 129, "outside"), (600, 2, 129, 128, "one"),
+    (90, 2, 777, 129, "outside"), (600, 2, 129, 128, "one"), (1500, 70, 136, 128, "skew"), (2000, 90, 100, 70, "outside"),
+    (3000, 1000, 63, 32, "skew"), (300, 100, 130, 257, "skew"),
 ]
 
 
@@ -307,6 +308,34 @@ def test_autograd_under_capture_is_refused():
     graph.replay()
     torch.cuda.synchronize()
     assert float(keep) == 0
+
+
+@pytest.mark.parametrize("n,n_in,n_out,dtype", [(4200003, 520, 72, "bf16"), (4200003, 520, 136, "fp16"), (34000001, 64, 5, "fp32")])
+def test_offsets_past_32_bits(n, n_in, n_out, dtype):
+    """x of more than 2^31 elements; rows sampled, dW over all of them in 64 bits"""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    x = torch.randn(n, n_in, device=DEV, generator=g, dtype=DT[dtype])
+    w = torch.randn(3, n_out, n_in, device=DEV, generator=g).to(DT[dtype])
+    index = torch.randint(-1, 3, (n,), device=DEV, generator=g, dtype=torch.int32)
+    plan = expert_plan(index, 3)
+    y = expert_linear(x, w, None, plan)
+    dy = torch.randn(n, n_out, device=DEV, generator=g, dtype=DT[dtype])
+    dx, dw, _ = expert_linear_backward(dy, x, w, plan)
+    at = torch.cat([torch.arange(64), torch.randint(0, n, (500,)), torch.arange(n - 64, n)]).to(DEV)
+    want, mag = linear64(x[at], w, None, index[at], False)
+    assert ((y[at].double().cpu() - want).abs() <= tolerance(n_in, mag, want, DT[dtype])).all()
+    (want, _, _), (mag, _, _), _ = backward64(dy[at], x[at], w, None, index[at], False)
+    assert ((dx[at].double().cpu() - want).abs() <= tolerance(n_out, mag, want, DT[dtype])).all()
+    for e in range(3):
+        want, mag = (torch.zeros(n_out, n_in, dtype=torch.float64, device=DEV) for _ in range(2))
+        for r in range(0, n, 1 << 20):
+            part = dy[r:r + (1 << 20)].double() * (index[r:r + (1 << 20)] == e)[:, None]
+            rows = x[r:r + (1 << 20)].double()
+            want += part.T.contiguous() @ rows
+            mag += part.T.abs().contiguous() @ rows.abs()
+        off = (dw[e].double() - want).abs()
+        assert (off <= tolerance(n, mag, want, DT[dtype])).all()
+        assert float(off.norm() / want.norm()) <= 2.0 ** -8     # far under what the bound over so many rows allows
 
 
 @pytest.mark.parametrize("n_in,n_out,dtype", [(63, 32, "fp32"), (130, 70, "fp32"), (256, 128, "bf16"), (100, 9, "fp16")])

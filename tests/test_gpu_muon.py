@@ -244,6 +244,17 @@ def test_long_sums_are_split(shape):
     assert torch.equal(got, newton_schulz(g.to(DEV)))
 
 
+@pytest.mark.parametrize("batch,m,n", [(100003, 3, 5), (70001, 34, 33), (66000, 20, 60)])
+def test_many_matrices(batch, m, n):
+    g = torch.randn(batch, m, n, generator=torch.Generator(device=DEV).manual_seed(batch), device=DEV)
+    got = newton_schulz(g)
+    for at in (0, 65535, 65536, batch - 1):
+        assert torch.equal(got[at], newton_schulz(g[at]))
+    pick = torch.tensor([1, 65534, 65537, batch - 2])
+    want = definition(g[pick.to(DEV)])
+    assert (norm(got[pick.to(DEV)].double().cpu() - want) <= bound(g[pick.to(DEV)], want, torch.float32)).all()
+
+
 def test_planes_of_more_than_2_gib():
     """One non-zero per row, in columns of their own: every singular value goes its own way, x -> a x + b x^3 + c x^5.  A plane of
     X takes 2.2 GiB, both 4.3: offsets past 32 bits.  Off by the output's rounding and the floor of the terms (no sums: each
