@@ -310,9 +310,9 @@ def test_autograd_under_capture_is_refused():
     assert float(keep) == 0
 
 
-@pytest.mark.parametrize("n,n_in,n_out,dtype", [(4200003, 520, 72, "bf16"), (4200003, 520, 136, "fp16"), (34000001, 64, 5, "fp32")])
+@pytest.mark.parametrize("n,n_in,n_out,dtype", [(4194300, 512, 128, "bf16"), (4200003, 520, 136, "fp16"), (34000001, 64, 5, "fp32")])
 def test_offsets_past_32_bits(n, n_in, n_out, dtype):
-    """x of more than 2^31 elements; rows sampled, dW over all of them in 64 bits"""
+    """x of 2^31 elements and more (the wide kernels up to there, the general tile beyond); rows sampled, dW over all of them in 64 bits"""
     g = torch.Generator(device=DEV).manual_seed(n)
     x = torch.randn(n, n_in, device=DEV, generator=g, dtype=DT[dtype])
     w = torch.randn(3, n_out, n_in, device=DEV, generator=g).to(DT[dtype])
