@@ -10,6 +10,7 @@ import contextlib
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import NrfError, check, lib
 from .ops import _ptr
@@ -33,6 +34,16 @@ def _on(device: torch.device):
 def _stream(t: torch.Tensor):
     """the current stream of the tensor's device, without building a Stream object (2 us)"""
     return C.c_void_p(torch._C._cuda_getCurrentRawStream(t.device.index))
+
+
+def _refuse_unseen(name: str, *tensors) -> None:
+    """What torch cannot see pass through the library: a trace would record the empty output alone, a tangent of forward-mode
+    differentiation would be dropped, which torch takes for zero."""
+    if torch._C._is_tracing():
+        raise NrfError(f"{name}: torch.jit.trace does not see the library's kernels (the traced graph would return memory that "
+                       "nothing wrote)")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NrfError(f"{name}: forward-mode derivatives (dual tensors) are not supported")
 
 
 def _up4(v: int) -> int:
@@ -66,6 +77,7 @@ class ExpertPlan:
 def expert_plan(index: torch.Tensor, num_experts: int) -> ExpertPlan:
     """Group the rows of a batch by expert (nrf_expert_plan).  ``index`` (n,) int32 on the GPU: the expert of each row; a
     value outside [0, num_experts) means the row has none.  Nothing is read back, the result is the same on every run."""
+    _refuse_unseen("expert_plan")
     if not index.is_cuda:
         raise NrfError("index: expected a cuda tensor (there is no CPU fallback)")
     if index.dtype != torch.int32 or index.ndim != 1:
@@ -151,7 +163,9 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
                   activation: str = "none") -> torch.Tensor:
     """``y[i] = act(weight[index[i]] @ x[i] + bias[index[i]])`` for the rows of ``plan``, zeros for rows of no expert
     (nrf_expert_linear).  x (n, n_in), weight (E, n_out, n_in), bias (E, n_out) or None, all float32, bfloat16 or float16
-    alike; ``activation`` "none" or "relu".  Differentiable in x, weight and bias."""
+    alike; ``activation`` "none" or "relu".  Differentiable in x, weight and bias: once, in reverse mode; forward mode and
+    ``torch.jit.trace`` are refused."""
+    _refuse_unseen("expert_linear", x, weight, bias)
     _check_layer(x, weight, bias, plan, activation)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         if torch.cuda.is_current_stream_capturing():
@@ -166,7 +180,8 @@ def expert_linear_backward(grad_y: torch.Tensor, x: torch.Tensor, weight: torch.
                            want_weight: bool = True, want_bias: bool = True):
     """Gradients of ``expert_linear`` -> (grad_x, grad_weight, grad_bias), None for those not wanted
     (nrf_expert_linear_backward).  ``y``: the forward's outputs, needed with "relu".  grad_bias is summed with grad_weight,
-    so it needs ``want_weight``.  The same bits on every run."""
+    so it needs ``want_weight``.  The same bits on every run.  Not differentiable itself."""
+    _refuse_unseen("expert_linear_backward", grad_y, x, weight)
     _check_layer(x, weight, None, plan, activation)
     shape = (x.shape[0], weight.shape[1])
     if activation == "relu" and y is None:

@@ -8,7 +8,7 @@ import ctypes as C
 import torch
 
 from ._lib import NrfError, check, lib
-from .expert_ops import DTYPES, _on, _stream
+from .expert_ops import DTYPES, _on, _refuse_unseen, _stream
 from .ops import _ptr
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # steep at 0 (weak directions catch up in five steps), within 0.7 .. 1.2 near 1
@@ -36,6 +36,7 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, ep
     """Orthogonalise matrices (nrf_newton_schulz): ``X = g / max(|g|_F, eps)``, then ``steps`` times
     ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``.  g (rows, cols) or (batch, rows, cols), float32, bfloat16 or float16;
     fp32-class arithmetic for every type, one rounding at the end.  ``out`` may be ``g``.  Not differentiable."""
+    _refuse_unseen("newton_schulz", g)
     if not g.is_cuda:
         raise NrfError("g: expected a cuda tensor (there is no CPU fallback)")
     if g.dtype not in DTYPES or g.ndim not in (2, 3):
@@ -66,6 +67,7 @@ def muon_update(params, grads, momentum_buffers, lr: float = 0.02, momentum: flo
     ``p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) newton_schulz(u)``."""
     if isinstance(params, torch.Tensor):
         params, grads, momentum_buffers = [params], [grads], [momentum_buffers]
+    _refuse_unseen("muon_update", *params, *grads, *momentum_buffers)
     if not (len(params) == len(grads) == len(momentum_buffers)):
         raise NrfError(f"muon_update: {len(params)} parameters, {len(grads)} gradients, {len(momentum_buffers)} momentum buffers")
     if not params:
