@@ -13,6 +13,7 @@
 // an output is rounded to its type once, after bias and relu.
 #include "dma_gemm.h"
 #include "experts.h"
+#include "grid.h"
 #include "split3.h"
 
 namespace {
@@ -170,7 +171,7 @@ __device__ __forceinline__ int xcd_run(const int* runs, int xcd, int local) {
     begin = int(int64_t(shorts) * xcd / 8), end = int(int64_t(shorts) * (xcd + 1) / 8);
     return local < end - begin ? longs + begin + local : -1;
 }
-__host__ __device__ constexpr int64_t xcd_blocks(int64_t slots, int a_tiles) { return (slots / 8 + 2) * 8 * a_tiles; }
+constexpr int64_t xcd_blocks(int64_t runs, int a_tiles) { return (runs / 8 + 2) * 8 * a_tiles; }
 
 // The expert with the `rank`-th most rows (of at most 64; equal ones by number).  A tile of dW takes as long as its expert has
 // rows, and the longest tiles have to begin first: begun by number, the CUs of 16 uneven experts were busy 67% of the time.
@@ -187,8 +188,8 @@ __device__ __forceinline__ int expert_of_rank(const int* counts, int E, int rank
 // dW's unit of this workgroup: which expert, which of its `tiles`.  Every XCD takes a contiguous eighth of each expert's tiles
 // (whole experts per XCD leave the XCD of the two most popular of sixteen with twice the average: 172 us where this takes
 // 99); fewer than eight go round.
-__device__ __forceinline__ bool dw_unit(const int* counts, int E, int tiles, int& expert, int& at) {
-    const int local = blockIdx.x / 8, xcd = blockIdx.x % 8;
+__device__ __forceinline__ bool dw_unit(const int* counts, int E, int tiles, int block, int& expert, int& at) {
+    const int local = block / 8, xcd = block % 8;
     if (tiles >= 8) {
         const int per = (tiles + 7) / 8;
         expert = local / per, at = int(int64_t(tiles) * xcd / 8) + local % per;
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g, int a_ti
     bool in_parts = false;
     if (FORM == kDw && g.splits != 0) {
         int at;
-        if (!dw_unit(g.plan, g.E, a_tiles * b_tiles * g.splits, expert, at)) return;
+        if (!dw_unit(g.plan, g.E, a_tiles * b_tiles * g.splits, nrf::grid_block(), expert, at)) return;
         const int split = at / (a_tiles * b_tiles), tile = at % (a_tiles * b_tiles);
         const int first = g.plan[L.offsets + expert], rows = g.plan[expert];
         const int per = (((rows + g.splits - 1) / g.splits) + kK - 1) / kK * kK;   // whole k steps
@@ -238,8 +239,8 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g, int a_ti
         a0 = tile % a_tiles * TT, b0 = tile / a_tiles * TT;
     } else {                              // a run of rows, all of whose tiles are the same XCD's
         constexpr int table = FORM == kDw ? kPartTable : kTable;
-        const int tiles = a_tiles * b_tiles, local = blockIdx.x / 8, tile = local % tiles;
-        const int at = xcd_run(g.plan + L.runs + 2 * table, blockIdx.x % 8, local / tiles);
+        const int tiles = a_tiles * b_tiles, block = nrf::grid_block(), local = block / 8, tile = local % tiles;
+        const int at = xcd_run(g.plan + L.runs + 2 * table, block % 8, local / tiles);
         if (at < 0) return;
         const int2 run = reinterpret_cast<const int2*>(g.plan + L.tiles[table])[at];
         b_count = run.y >> 16, expert = run.y & 0xffff;
@@ -491,7 +492,7 @@ __global__ __launch_bounds__(512) void expert_wide_dw_kernel(ExpertArgs g, int a
     int* s_list = reinterpret_cast<int*>(smem + Gemm::kLds);
     const PlanLayout L(g.n, g.E);
     int expert, at;
-    if (!dw_unit(g.plan, g.E, a_tiles * b_tiles * g.splits, expert, at)) return;
+    if (!dw_unit(g.plan, g.E, a_tiles * b_tiles * g.splits, blockIdx.x, expert, at)) return;
     const int split = at / (a_tiles * b_tiles), tile = at % (a_tiles * b_tiles);
     const int a0 = tile % a_tiles * W::kA, b0 = tile / a_tiles * W::kB;
     const int rows = g.plan[expert], per = ((rows + g.splits - 1) / g.splits + 63) / 64 * 64;
@@ -556,7 +557,7 @@ int launch_wide_rows(const ExpertArgs& g, hipStream_t stream) {
     auto kernel = &expert_wide_rows_kernel<T, FORM, ROWS>;
     const int st = allow_lds(reinterpret_cast<const void*>(kernel), kWideLds);
     if (st != NRF_OK) return st;
-    const int64_t blocks = xcd_blocks(PlanLayout::slots(g.n, g.E, ROWS == 256 ? 3 : 2), a_tiles);
+    const int64_t blocks = xcd_blocks(PlanLayout::most_runs(g.n, g.E, ROWS == 256 ? 3 : 2), a_tiles);   // under 2^23 (wide)
     kernel<<<dim3(unsigned(blocks)), 512, kWideLds, stream>>>(g, a_tiles);
     return NRF_OK;
 }
@@ -578,8 +579,9 @@ int launch_wide_dw(const ExpertArgs& g, hipStream_t stream) {
 }
 
 // Whether the wide kernels take a product: octets that do not straddle rows (of x and w alone for the forward, which stores its
-// outputs at any alignment), operands under 4 GiB and at least half a tile's columns.  Any number of rows: single tokens through 32 experts of 1024 -> 2048 take 17 us (7.3 TB/s of weights), the general
-// tile 25.
+// outputs at any alignment), operands under 4 GiB and at least half a tile's columns.  Any number of rows: single tokens through 32 experts of 1024 -> 2048
+// take 17 us (7.3 TB/s of weights), the general tile 25.  A launch of 512 threads stays under 2^23 workgroups: rows times columns
+// under 2^31 leave 2^18 whole tiles, 16384 experts 2^22 short runs' tiles, and dW's tiles hold 2^14 weights each (2^37 fill the memory).
 bool wide(int64_t n, int E, int n_in, int n_out, int dtype, bool forward = false) {
     return dtype != NRF_DTYPE_FP32 && n_in % 8 == 0 && (forward || n_out % 8 == 0) && n_in >= 128 && n_out >= 128 &&
            n * (n_in > n_out ? n_in : n_out) < int64_t(1) << 31 && int64_t(n_out) * n_in < int64_t(1) << 31;
@@ -815,7 +817,7 @@ __global__ __launch_bounds__(256) void expert_cell_backward_kernel(ExpertArgs g,
 }
 int launch_cell_forward(const ExpertArgs& g, hipStream_t stream) {
     const bool i2 = g.n_in > 32, o2 = g.n_out > 32;
-    const dim3 grid(unsigned(PlanLayout::slots(g.n, g.E, kCellRowsTable)));
+    const dim3 grid(unsigned(PlanLayout::most_runs(g.n, g.E, kCellRowsTable)));
     if (i2 && o2) expert_cell_forward_kernel<2, 2><<<grid, 256, 0, stream>>>(g);
     else if (i2) expert_cell_forward_kernel<2, 1><<<grid, 256, 0, stream>>>(g);
     else if (o2) expert_cell_forward_kernel<1, 2><<<grid, 256, 0, stream>>>(g);
@@ -824,7 +826,7 @@ int launch_cell_forward(const ExpertArgs& g, hipStream_t stream) {
 }
 template <int NI, int NO>
 int launch_cell_backward(const ExpertArgs& g, float* dx, hipStream_t stream) {
-    expert_cell_backward_kernel<NI, NO><<<dim3(unsigned(PlanLayout::slots(g.n, g.E, kPartTable))), 256, 0, stream>>>(g, dx);
+    expert_cell_backward_kernel<NI, NO><<<dim3(unsigned(PlanLayout::most_runs(g.n, g.E, kPartTable))), 256, 0, stream>>>(g, dx);
     return NRF_OK;
 }
 int launch_cell_backward(const ExpertArgs& g, float* dx, hipStream_t stream) {
@@ -898,8 +900,8 @@ void launch_tile(int dtype, const ExpertArgs& g, hipStream_t stream) {
     const int a_tiles = ((FORM == kForward ? g.n_out : g.n_in) + TT - 1) / TT, b_tiles = FORM == kDw ? (g.n_out + TT - 1) / TT : 1;
     const int table = FORM == kDw ? kPartTable : TT == 64 ? 1 : 2;
     const int64_t blocks = FORM == kDw && g.splits != 0 ? dw_blocks(int64_t(g.splits) * a_tiles * b_tiles, g.E)
-                                                        : xcd_blocks(PlanLayout::slots(g.n, g.E, table), a_tiles * b_tiles);
-    const dim3 grid{unsigned(blocks)};
+                                                        : xcd_blocks(PlanLayout::most_runs(g.n, g.E, table), a_tiles * b_tiles);
+    const dim3 grid = nrf::grid_rows(blocks);
     if (dtype == NRF_DTYPE_FP32) expert_tile_kernel<Fp32, FORM, TT><<<grid, 256, 0, stream>>>(g, a_tiles, b_tiles);
     else if (dtype == NRF_DTYPE_BF16) expert_tile_kernel<Bf16, FORM, TT><<<grid, 256, 0, stream>>>(g, a_tiles, b_tiles);
     else expert_tile_kernel<Fp16, FORM, TT><<<grid, 256, 0, stream>>>(g, a_tiles, b_tiles);

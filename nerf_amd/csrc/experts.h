@@ -10,8 +10,8 @@
 //            the length and less: as costly as whole ones, next to the runs that share their weights), then the short rests
 //            (a product's last workgroups are then its shortest; 32 k rows, 32 experts of 2048 x 2048: 297 - 311 us, with
 //            every rest at the end 317 - 376, with none there 302 - 323)
-// A table of runs of 2^s rows has at most (n >> s) + E + 1 entries: the host sizes the products' grids with that and never
-// reads a count back; workgroups past the table's count leave at once.
+// A table of runs of 2^s rows has at most (n >> s) + E + 1 entries, and no more than rows: the host sizes the products' grids
+// with that and never reads a count back; workgroups past the table's count leave at once.
 #pragma once
 #include "nrf_common.h"
 
@@ -25,6 +25,7 @@ struct PlanLayout {
     int64_t offsets, order, runs, tiles[kTileTables], total;   // in int32 words; counts at 0
     __host__ __device__ static constexpr int64_t up4(int64_t v) { return (v + 3) & ~int64_t(3); }
     __host__ __device__ static constexpr int64_t slots(int64_t n, int E, int table) { return (n >> (kTileShift0 + table)) + E + 1; }
+    static constexpr int64_t most_runs(int64_t n, int E, int table) { return slots(n, E, table) < n ? slots(n, E, table) : n; }
     __host__ __device__ constexpr PlanLayout(int64_t n, int E) : offsets(up4(E)), order(0), runs(0), tiles{0, 0, 0, 0}, total(0) {
         order = offsets + up4(E + 1);
         runs = order + up4(n);
