@@ -546,8 +546,9 @@ int nrf_expert_linear_backward(const void* grad_y, const void* x, const void* we
  * (two fp16 terms per operand, 22 significand bits, fp32 sums; the norm in float64), one rounding at the end.  A matrix with
  * a value that is not finite gives NaN, the others of the batch are untouched by it; a zero matrix gives zeros.
  * eps >= 1e-30, steps <= 16; the iteration over the singular values in [0, 1] must stay within 1.5 (checked on the host).
- * Sides up to 65536; batch up to 2^24 where the shorter side is <= 32 and the longer <= 128, else 65535 and 2^24 / (the
- * matrix's tiles of 64 x 64, its sides rounded up to 128 each).  Apart from out = g nothing may overlap.  The reference has no counterpart: its optimisers are
+ * Sides up to 65536; batch up to 2^24 where no workspace is asked for (a shorter side <= 32 with a longer <= 128, <= 64 with
+ * <= 544, <= 128 with <= 160), else 65535 and 2^24 / (the matrix's tiles of 64 x 64; sides rounded up to whole tiles, of 128
+ * where the shorter side is over 512).  Apart from out = g nothing may overlap.  The reference has no counterpart: its optimisers are
  * torch.optim's (src/train/optimizer.py:9-29). */
 int64_t nrf_newton_schulz_workspace_bytes(int64_t batch, int rows, int cols);
 int nrf_newton_schulz(const void* g, void* out, int64_t batch, int rows, int cols, int dtype, int steps, float a, float b, float c,

@@ -18,6 +18,7 @@
 //   otherwise                               the matrices' terms in the workspace: a launch per step up to 64 x 640 and 128 x 320
 //                                           (schulz_step_kernel), else three (schulz_product_kernel).
 #include "dma_gemm.h"
+#include "grid.h"
 #include "split2h.h"
 
 namespace {
@@ -350,7 +351,8 @@ template <class T, int MB>
 __global__ __launch_bounds__(512) void schulz_block_kernel(SchulzArgs s, BlockShape L, unsigned by_cols) {
     extern __shared__ __align__(16) char smem[];
     constexpr int kJ = MB / 4, kI = MB * MB / kBlockWaves / kJ, kAhead = 8;   // kI x kJ tiles of A are a wavefront's (kI columns)
-    const int64_t m = blockIdx.x;
+    const int64_t m = nrf::grid_block();
+    if (m >= s.batch) return;
     const int t = int(m / s.per), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
     const int count = s.rows * s.cols;
     const int64_t base = (m % s.per) * int64_t(count);
@@ -928,7 +930,7 @@ int launch_block(const SchulzArgs& s, hipStream_t stream) {
                                                kLdsBytes) != hipSuccess)
         return NRF_ERR_LAUNCH;
     // i / cols = i * by_cols >> 32 for i < 2^32 / cols (an element's index is below 2^16); 0 for a single column
-    kernel<<<unsigned(s.batch), 512, L.bytes, stream>>>(s, L, s.cols == 1 ? 0u : unsigned((int64_t(1) << 32) / s.cols + 1));
+    kernel<<<nrf::grid_rows(s.batch), 512, L.bytes, stream>>>(s, L, s.cols == 1 ? 0u : unsigned((int64_t(1) << 32) / s.cols + 1));
     return NRF_OK;
 }
 
@@ -1046,8 +1048,7 @@ int run(const SchulzArgs& s, void* workspace, hipStream_t stream) {
 
 bool schulz_shape_ok(int64_t batch, int rows, int cols) {
     if (batch < 0 || rows < 1 || cols < 1 || rows > 65536 || cols > 65536) return false;
-    if (small_path(rows, cols)) return batch <= int64_t(1) << 24;
-    if (block_path(rows, cols)) return batch <= int64_t(1) << 24;
+    if (small_path(rows, cols) || block_path(rows, cols)) return batch <= int64_t(1) << 24;
     const LargeShape L = large_shape(rows, cols);
     return batch <= 65535 && batch * (int64_t(L.Mp / 64) * (L.Np / 64)) <= int64_t(1) << 24;
 }

@@ -26,7 +26,7 @@ def _workspace(batch: int, rows: int, cols: int, device):
     need = lib().nrf_newton_schulz_workspace_bytes(batch, rows, cols)
     if need < 0:
         raise NrfError(f"{batch} matrices of {rows} x {cols}: sides of 1 to 65536 and up to 65535 matrices are supported "
-                       "(2^24 up to 32 x 128), 2^24 tiles of 64 x 64 in all")
+                       "(2^24 up to 32 x 128, 64 x 544 and 128 x 160), 2^24 tiles of 64 x 64 in all")
     return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
 
 
