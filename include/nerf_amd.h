@@ -504,8 +504,8 @@ int nrf_kilo_clip_adam(float* const* params, float* const* grads, float* const* 
 /* The general form of what nrf_kilo_forward does for its fixed tiny networks: row i of a batch goes through the weights of
  * expert index[i].  Any number of experts up to 16384, layer sizes up to 65536, up to 2^28 rows, three types.  (The reference
  * has no counterpart beyond BatchedKiloNeRF's bmm over padded cells, src/models/kilonerf/network.py:123-167.)  Pointers are
- * contiguous tensors of `dtype`, aligned to one element; the plan and workspaces to 16 bytes.  Every entry point may be
- * captured into a graph; nothing is read back. */
+ * contiguous tensors of `dtype`, aligned to one element; the plan and workspaces to 16 bytes.  An output overlaps neither an
+ * operand nor another output (NRF_ERR_SHAPE).  Every entry point may be captured into a graph; nothing is read back. */
 enum { NRF_DTYPE_FP32 = 0, NRF_DTYPE_BF16 = 1, NRF_DTYPE_FP16 = 2 };
 enum { NRF_ACT_NONE = 0, NRF_ACT_RELU = 1 };
 
@@ -548,8 +548,8 @@ int nrf_expert_linear_backward(const void* grad_y, const void* x, const void* we
  * eps >= 1e-30, steps <= 16; the iteration over the singular values in [0, 1] must stay within 1.5 (checked on the host).
  * Sides up to 65536; batch up to 2^24 where no workspace is asked for (a shorter side <= 32 with a longer <= 128, <= 64 with
  * <= 544, <= 128 with <= 160), else 65535 and 2^24 / (the matrix's tiles of 64 x 64; sides rounded up to whole tiles, of 128
- * where the shorter side is over 512).  Apart from out = g nothing may overlap.  The reference has no counterpart: its optimisers are
- * torch.optim's (src/train/optimizer.py:9-29). */
+ * where the shorter side is over 512).  Apart from out = g nothing may overlap (NRF_ERR_SHAPE).  The reference has no counterpart:
+ * its optimisers are torch.optim's (src/train/optimizer.py:9-29). */
 int64_t nrf_newton_schulz_workspace_bytes(int64_t batch, int rows, int cols);
 int nrf_newton_schulz(const void* g, void* out, int64_t batch, int rows, int cols, int dtype, int steps, float a, float b, float c,
                       float eps, void* workspace, int64_t workspace_bytes, nrf_stream_t stream);
@@ -558,7 +558,7 @@ int nrf_newton_schulz(const void* g, void* out, int64_t batch, int rows, int col
  * u = nesterov ? g + mu momentum : momentum; O = the Newton-Schulz products of u (nrf_newton_schulz);
  * p = (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) O.  params / grads / momentum: HOST arrays of n_tensors <= 32
  * DEVICE pointers, each a contiguous fp32 (batch, rows, cols); params and momentum are updated in place: none of them may
- * overlap another or a gradient (equal pointers give NRF_ERR_SHAPE).  workspace: nrf_newton_schulz_workspace_bytes(n_tensors * batch, rows, cols). */
+ * overlap another or a gradient (NRF_ERR_SHAPE).  workspace: nrf_newton_schulz_workspace_bytes(n_tensors * batch, rows, cols). */
 int nrf_muon_update(float* const* params, const float* const* grads, float* const* momentum, int n_tensors, int64_t batch, int rows,
                     int cols, float grad_scale, float clip_value, float mu, int nesterov, float lr, float weight_decay, int steps,
                     float a, float b, float c, float eps, void* workspace, int64_t workspace_bytes, nrf_stream_t stream);

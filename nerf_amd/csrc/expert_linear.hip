@@ -13,7 +13,7 @@
 // an output is rounded to its type once, after bias and relu.
 #include "dma_gemm.h"
 #include "experts.h"
-#include "grid.h"
+#include "launch.h"
 #include "split3.h"
 
 namespace {
@@ -925,7 +925,8 @@ bool shapes_ok(int64_t n, int E, int n_in, int n_out, int dtype, int act) {
            n_out <= 65536 && dtype >= NRF_DTYPE_FP32 && dtype <= NRF_DTYPE_FP16 && (act == NRF_ACT_NONE || act == NRF_ACT_RELU);
 }
 
-bool elem_aligned(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == NRF_DTYPE_FP32 ? 3u : 1u)) == 0; }
+int elem_bytes(int dtype) { return dtype == NRF_DTYPE_FP32 ? 4 : 2; }
+bool elem_aligned(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & unsigned(elem_bytes(dtype) - 1)) == 0; }
 
 }  // namespace
 
@@ -937,6 +938,10 @@ NRF_EXPORT int nrf_expert_linear(const void* x, const void* weight, const void* 
     if (!elem_aligned(x, dtype) || !elem_aligned(weight, dtype) || !elem_aligned(bias, dtype) || !elem_aligned(y, dtype) ||
         !nrf_aligned16(plan))
         return NRF_ERR_ALIGN;
+    const int64_t size = elem_bytes(dtype), y_bytes = n_rows * n_out * size;
+    if (nrf::overlap(y, y_bytes, x, n_rows * n_in * size) || nrf::overlap(y, y_bytes, weight, int64_t(num_experts) * n_out * n_in * size) ||
+        nrf::overlap(y, y_bytes, bias, int64_t(num_experts) * n_out * size))
+        return NRF_ERR_SHAPE;
     ExpertArgs g{};
     g.x = x, g.w = weight, g.bias = bias, g.plan = static_cast<const int*>(plan), g.out = y;
     g.n = n_rows, g.E = num_experts, g.n_in = n_in, g.n_out = n_out, g.relu = act == NRF_ACT_RELU, g.splits = 1;
@@ -990,6 +995,13 @@ NRF_EXPORT int nrf_expert_linear_backward(const void* grad_y, const void* x, con
     if (!nrf_aligned16(plan) || !nrf_aligned16(workspace)) return NRF_ERR_ALIGN;
     const BackwardWork work(n_rows, num_experts, n_in, n_out, dtype);
     if (work.dz + work.partial > 0 && (!workspace || workspace_bytes < work.dz + work.partial)) return NRF_ERR_WORKSPACE;
+    const int64_t size = elem_bytes(dtype), x_bytes = n_rows * n_in * size, y_bytes = n_rows * n_out * size,
+                  w_bytes = int64_t(num_experts) * n_out * n_in * size, b_bytes = int64_t(num_experts) * n_out * size;
+    const struct { const void* p; int64_t bytes; } parts[] = {{grad_x, x_bytes}, {grad_weight, w_bytes}, {grad_bias, b_bytes},
+                                                              {grad_y, y_bytes}, {x, x_bytes}, {weight, w_bytes}, {act == NRF_ACT_RELU ? y : nullptr, y_bytes}};
+    for (int i = 0; i < 3; ++i)              // an output with another, or with an operand that is read again after it was written
+        for (int j = i + 1; j < 7; ++j)
+            if (nrf::overlap(parts[i].p, parts[i].bytes, parts[j].p, parts[j].bytes)) return NRF_ERR_SHAPE;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     ExpertArgs g{};
     g.x = x, g.w = weight, g.y = y, g.g = grad_y, g.plan = static_cast<const int*>(plan);

@@ -18,7 +18,7 @@
 //   otherwise                               the matrices' terms in the workspace: a launch per step up to 64 x 640 and 128 x 320
 //                                           (schulz_step_kernel), else three (schulz_product_kernel).
 #include "dma_gemm.h"
-#include "grid.h"
+#include "launch.h"
 #include "split2h.h"
 
 namespace {
@@ -1086,6 +1086,8 @@ NRF_EXPORT int nrf_newton_schulz(const void* g, void* out, int64_t batch, int ro
     const uintptr_t low = dtype == NRF_DTYPE_FP32 ? 3 : 1;
     if ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(out)) & low || (need > 0 && !nrf_aligned16(workspace)))
         return NRF_ERR_ALIGN;
+    const int64_t bytes = batch * rows * cols * (dtype == NRF_DTYPE_FP32 ? 4 : 2);
+    if (g != out && nrf::overlap(g, bytes, out, bytes)) return NRF_ERR_SHAPE;   // one matrix' result over another's input
     SchulzArgs s{};
     s.g[0] = g, s.out[0] = out, s.batch = batch, s.per = int(batch), s.rows = rows, s.cols = cols, s.steps = steps;
     s.a = a, s.b = b, s.c = c, s.eps = eps;
@@ -1113,10 +1115,12 @@ NRF_EXPORT int nrf_muon_update(float* const* params, const float* const* grads, 
             return NRF_ERR_ALIGN;
         s.g[i] = grads[i], s.out[i] = params[i], s.mom[i] = momentum[i];
     }
-    for (int i = 0; i < n_tensors; ++i)      // the same tensor twice, or as gradient and momentum: read while it is written
+    const int64_t bytes = batch * rows * cols * 4;
+    const auto shared = [bytes](const float* x, const float* y) { return nrf::overlap(x, bytes, y, bytes); };
+    for (int i = 0; i < n_tensors; ++i)      // a tensor twice, or as gradient and momentum, or in parts: read while it is written
         for (int j = 0; j < n_tensors; ++j)
-            if (params[i] == momentum[j] || params[i] == grads[j] || momentum[i] == grads[j] ||
-                (i != j && (params[i] == params[j] || momentum[i] == momentum[j])))
+            if (shared(params[i], momentum[j]) || shared(params[i], grads[j]) || shared(momentum[i], grads[j]) ||
+                (i != j && (shared(params[i], params[j]) || shared(momentum[i], momentum[j]))))
                 return NRF_ERR_SHAPE;
     s.batch = batch * n_tensors, s.per = int(batch), s.rows = rows, s.cols = cols, s.steps = steps, s.nesterov = nesterov != 0;
     s.a = a, s.b = b, s.c = c, s.eps = eps, s.grad_scale = grad_scale, s.clip = clip_value, s.mu = mu;

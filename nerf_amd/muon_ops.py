@@ -22,6 +22,16 @@ def _written(tensors) -> None:
             torch.autograd.graph.increment_version(t)
 
 
+def _shared(written, read, size: int) -> bool:
+    """whether one of the tensors at ``written``, all of ``size`` bytes, shares memory with another or with one at ``read``"""
+    ends = {True: 0, False: 0}     # of what was passed in the order of the addresses: the written, the read
+    for at, in_place in sorted([(p, True) for p in written] + [(p, False) for p in read]):
+        if at < ends[True] or (in_place and at < ends[False]):
+            return True
+        ends[in_place] = at + size
+    return False
+
+
 def _workspace(batch: int, rows: int, cols: int, device):
     need = lib().nrf_newton_schulz_workspace_bytes(batch, rows, cols)
     if need < 0:
@@ -35,7 +45,8 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, ep
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """Orthogonalise matrices (nrf_newton_schulz): ``X = g / max(|g|_F, eps)``, then ``steps`` times
     ``X <- a X + (b A + c A^2) X`` with ``A = X X^T``.  g (rows, cols) or (batch, rows, cols), float32, bfloat16 or float16;
-    fp32-class arithmetic for every type, one rounding at the end.  ``out`` may be ``g``.  Not differentiable."""
+    fp32-class arithmetic for every type, one rounding at the end.  ``out`` may be ``g``, but share no other memory with it.  Not
+    differentiable."""
     _refuse_unseen("newton_schulz", g)
     if not g.is_cuda:
         raise NrfError("g: expected a cuda tensor (there is no CPU fallback)")
@@ -49,6 +60,8 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, ep
         raise NrfError(f"out: expected a contiguous {g.dtype} {tuple(g.shape)} on {g.device}")
     work, need = _workspace(batch, rows, cols, g.device)
     g = g.contiguous()
+    if 0 < abs(out.data_ptr() - g.data_ptr()) < g.numel() * g.element_size():
+        raise NrfError("out: overlaps g without being g (matrices would be read after others were written over them)")
     a, b, c = coefficients
     with _on(g.device):
         check(lib().nrf_newton_schulz(_ptr(g), _ptr(out), batch, rows, cols, DTYPES[g.dtype], int(steps), a, b, c, eps,
@@ -64,7 +77,8 @@ def muon_update(params, grads, momentum_buffers, lr: float = 0.02, momentum: flo
     """One Muon step in place (nrf_muon_update) on a float32 tensor (rows, cols) or (batch, rows, cols), or on a list of such
     tensors of one shape (more than 32 go in several calls).  ``momentum_buffers`` like ``params``, zero at the first step:
     ``g = clamp(grad * grad_scale, +-clip_value)``, ``m <- momentum m + g``, ``u = g + momentum m`` (nesterov) or ``m``,
-    ``p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) newton_schulz(u)``."""
+    ``p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) newton_schulz(u)``.  A parameter or momentum buffer shares no
+    memory with another tensor of the call; gradients may with each other."""
     if isinstance(params, torch.Tensor):
         params, grads, momentum_buffers = [params], [grads], [momentum_buffers]
     _refuse_unseen("muon_update", *params, *grads, *momentum_buffers)
@@ -81,10 +95,9 @@ def muon_update(params, grads, momentum_buffers, lr: float = 0.02, momentum: flo
                 raise NrfError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}, want float32 {tuple(shape)} on {dev}")
             if name != "grad" and not t.is_contiguous():
                 raise NrfError(f"{name}: expected a contiguous tensor (it is updated in place)")
-    written = [t.data_ptr() for t in (*params, *momentum_buffers)]
-    if shape.numel() and len({*written, *(g.data_ptr() for g in grads)}) < len(written) + len({g.data_ptr() for g in grads}):
-        raise NrfError("muon_update: a tensor is given twice (each parameter and momentum buffer is updated in place)")
     grads = [g.contiguous() for g in grads]
+    if _shared([t.data_ptr() for t in (*params, *momentum_buffers)], [g.data_ptr() for g in grads], 4 * shape.numel()):
+        raise NrfError("muon_update: tensors overlap (each parameter and momentum buffer is updated in place)")
     rows, cols = shape[-2:]
     batch = shape[0] if len(shape) == 3 else 1
     a, b, c = coefficients

@@ -44,3 +44,29 @@ def test_an_update_of_more_matrices_than_a_grid_row():
     for at, (p1, g1, m1) in zip(AT, singly):
         muon_update(p1, g1, m1)
         assert torch.equal(p[at], p1) and torch.equal(m[at], m1) and torch.equal(g[at], g1)
+
+
+def test_overlapping_tensors_are_refused_and_neighbours_are_not():
+    flat = torch.randn(3 * 600, device=DEV, generator=torch.Generator(device=DEV).manual_seed(3))
+    first, second, third = flat.view(3, 2, 15, 20)
+    want = newton_schulz(first)
+    with pytest.raises(muon_ops.NrfError, match="overlaps"):
+        newton_schulz(first, out=flat[300:900].view(2, 15, 20))
+    assert torch.equal(newton_schulz(first, out=second), want) and torch.equal(second, want)
+    start, grad = flat[300:900].clone().view(2, 15, 20), third.clone()
+    for args in ((first, third, flat[300:900].view(2, 15, 20)), (flat[300:900].view(2, 15, 20), first, third),
+                 ([first, flat[1:601].view(2, 15, 20)], [third, third], [torch.zeros_like(first), torch.zeros_like(first)])):
+        with pytest.raises(muon_ops.NrfError, match="overlap"):
+            muon_update(*args)
+    assert torch.equal(flat[300:900].view(2, 15, 20), start) and torch.equal(third, grad)
+    p, m = first.clone(), second.clone()
+    muon_update(p, third, m)
+    muon_update(first, third, second)                        # neighbours of one buffer
+    assert torch.equal(first, p) and torch.equal(second, m) and torch.equal(third, grad)
+    # a transposed gradient is laid out anew before the call
+    square = torch.randn(8, 8, device=DEV)
+    p, m = square.clone(), torch.zeros_like(square)
+    muon_update(p, square.t().contiguous(), m)
+    q = square.clone()
+    muon_update(q, q.t(), torch.zeros_like(q))
+    assert torch.equal(p, q)
