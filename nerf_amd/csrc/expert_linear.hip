@@ -850,9 +850,10 @@ __global__ __launch_bounds__(256) void expert_sum_kernel(ExpertArgs g) {
     const int parts = by_runs ? (rows + kPartRows - 1) / kPartRows : g.splits;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < size; i += int64_t(gridDim.x) * 256) {
         const float* p = g.partial + first * size + i;
-        float v = 0.f;
+        double sum = 0.0;          // 2^26 rows are 2^18 parts: a running sum of 32 bits no longer takes in a part's last bits (0.4 % off)
 #pragma unroll 4
-        for (int r = 0; r < parts; ++r) v += p[r * step * size];
+        for (int r = 0; r < parts; ++r) sum += double(p[r * step * size]);
+        const float v = float(sum);
         if (i < weights) static_cast<elem*>(g.out)[expert * weights + i] = from_float(v, T{});
         else if (g.db) static_cast<elem*>(g.db)[int64_t(expert) * g.n_out + i - weights] = from_float(v, T{});
     }
