@@ -880,11 +880,11 @@ __global__ __launch_bounds__(256) void schulz_copy_kernel(SchulzArgs s, LargeSha
     const int64_t m = blockIdx.y, count = int64_t(s.rows) * s.cols;
     double sum = 0.0;
     for (int i = 0; i < L.chunks; ++i) sum += parts[m * L.chunks + i];
-    const float scale = start_scale(sum, s.eps) * kUnscale;
+    const float scale = start_scale(sum, s.eps);     // 1 / norm itself would be subnormal from norms of 8.5e37 on
     const int t = int(m / s.per);
     const int64_t base = (m % s.per) * count;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count; i += int64_t(gridDim.x) * 256)
-        emit<T>(s, t, base + i, 0, element<T, true>(s, t, base + i, 0, nullptr) * scale, before<T>(s, t, base + i, 0));
+        emit<T>(s, t, base + i, 0, element<T, true>(s, t, base + i, 0, nullptr) * scale * kUnscale, before<T>(s, t, base + i, 0));
 }
 
 bool small_path(int rows, int cols) {
