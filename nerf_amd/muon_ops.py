@@ -75,7 +75,7 @@ def muon_update(params, grads, momentum_buffers, lr: float = 0.02, momentum: flo
                 weight_decay: float = 0.0, clip_value: float = 40.0, grad_scale: float = 1.0, steps: int = 5,
                 coefficients=COEFFICIENTS, eps: float = 1e-7) -> None:
     """One Muon step in place (nrf_muon_update) on a float32 tensor (rows, cols) or (batch, rows, cols), or on a list of such
-    tensors of one shape (more than 32 go in several calls).  ``momentum_buffers`` like ``params``, zero at the first step:
+    tensors of one shape (more than 32, or than one call's matrices, go in several calls).  ``momentum_buffers`` like ``params``, zero at the first step:
     ``g = clamp(grad * grad_scale, +-clip_value)``, ``m <- momentum m + g``, ``u = g + momentum m`` (nesterov) or ``m``,
     ``p <- (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) newton_schulz(u)``.  A parameter or momentum buffer shares no
     memory with another tensor of the call; gradients may with each other."""
@@ -101,8 +101,11 @@ def muon_update(params, grads, momentum_buffers, lr: float = 0.02, momentum: flo
     rows, cols = shape[-2:]
     batch = shape[0] if len(shape) == 3 else 1
     a, b, c = coefficients
-    for i in range(0, len(params), MAX_TENSORS):
-        part = [ts[i:i + MAX_TENSORS] for ts in (params, grads, momentum_buffers)]
+    per = min(len(params), MAX_TENSORS)
+    while per > 1 and lib().nrf_newton_schulz_workspace_bytes(batch * per, rows, cols) < 0:
+        per //= 2
+    for i in range(0, len(params), per):
+        part = [ts[i:i + per] for ts in (params, grads, momentum_buffers)]
         n = len(part[0])
         work, need = _workspace(batch * n, rows, cols, dev)
         arrays = [(C.c_void_p * n)(*[t.data_ptr() for t in ts]) for ts in part]

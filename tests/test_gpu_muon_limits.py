@@ -70,3 +70,16 @@ def test_overlapping_tensors_are_refused_and_neighbours_are_not():
     q = square.clone()
     muon_update(q, q.t(), torch.zeros_like(q))
     assert torch.equal(p, q)
+
+
+def test_a_list_of_more_matrices_than_one_call_takes():
+    """3 x 22000 matrices of 1 x 545, of which a call takes 65535: each tensor alone would be taken"""
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    p, g, m = ([torch.randn(22000, 1, 545, device=DEV, generator=gen) for _ in range(3)] for _ in range(3))
+    singly = [[t.clone() for t in ts] for ts in zip(p, g, m)]
+    muon_update(p, g, m)
+    for i, (p1, g1, m1) in enumerate(singly):     # (whole tensors: a few matrices alone take the launch-per-step kernel)
+        muon_update(p1, g1, m1)
+        assert torch.equal(p[i], p1) and torch.equal(m[i], m1)
+    with pytest.raises(muon_ops.NrfError, match="up to 65535"):
+        muon_update(*([torch.zeros(65536, 1, 545, device=DEV) for _ in range(2)] for _ in range(3)))
