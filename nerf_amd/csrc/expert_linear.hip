@@ -8,9 +8,9 @@
 //   forward   a = output feature (W rows)             b = batch row (x rows, gathered)       k = input
 //   dx        a = input feature (W columns)           b = batch row (dz rows, gathered)      k = output
 //   dW        a = input feature (x columns, gathered) b = output feature (dz columns)        k = the expert's batch rows
-// bf16 / fp16 operands go to the matrix cores as they are.  fp32 operands are split into three bf16 terms on their way into
-// LDS (split3.h: 24 significand bits, six products, fp32 sums): an operand that is not finite gives NaN.  Sums are fp32;
-// an output is rounded to its type once, after bias and relu.
+// bf16 / fp16 operands go to the matrix cores as they are, so do those of fp32 layers up to 64 x 64.  Other fp32 operands are split
+// into three bf16 terms on their way into LDS (split3.h: 24 significand bits, six products, fp32 sums): one that is not finite
+// gives NaN.  Sums are fp32; an output is rounded to its type once, after bias and relu.
 #include "dma_gemm.h"
 #include "experts.h"
 #include "launch.h"
@@ -54,13 +54,15 @@ template <> struct Oct<Fp32> {
 #pragma unroll
         for (int j = 0; j < 4; ++j) lo[j] = y.lo[j] > 0.f ? lo[j] : 0.f, hi[j] = y.hi[j] > 0.f ? hi[j] : 0.f;
     }
-    // -> the eight elements of each bf16 term
-    __device__ __forceinline__ void terms(const SplitSel& sel, u32x4 (&out)[3]) const {
+    // -> the eight elements of each bf16 term.  Elements that belong to different outputs (`apart`) are split each for itself, four more
+    // instructions per pair: dot2 multiplies the pair's other element by zero, and one that is not finite would make NaN of both
+    __device__ __forceinline__ void terms(const SplitSel& sel, bool apart, u32x4 (&out)[3]) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float a = j < 2 ? lo[2 * j] : hi[2 * j - 4], b = j < 2 ? lo[2 * j + 1] : hi[2 * j - 3];
             unsigned p0, p1, p2;
-            split_pair_dot2(sel, a, b, p0, p1, p2);
+            if (apart) split_pair(a, b, p0, p1, p2);
+            else split_pair_dot2(sel, a, b, p0, p1, p2);
             out[0][j] = p0, out[1][j] = p1, out[2][j] = p2;
         }
     }
@@ -87,7 +89,7 @@ template <class T, unsigned INF> struct Oct16 {
             v[j] &= (lo - 1u < INF ? 0xffffu : 0u) | (hi - 1u < INF ? 0xffff0000u : 0u);
         }
     }
-    __device__ __forceinline__ void terms(const SplitSel&, u32x4 (&out)[1]) const { out[0] = v; }
+    __device__ __forceinline__ void terms(const SplitSel&, bool, u32x4 (&out)[1]) const { out[0] = v; }
 };
 template <> struct Oct<Bf16> : Oct16<Bf16, 0x7f80u> {};
 template <> struct Oct<Fp16> : Oct16<Fp16, 0x7c00u> {};
@@ -306,7 +308,7 @@ __global__ __launch_bounds__(256) void expert_tile_kernel(ExpertArgs g, int a_ti
         const int k = cols ? ck + kNext * j : kc, row = cols ? cr : kr + kDown * j;
         if (k0 + kStep > k_end) v.limit(cols ? (k0 + k < k_end ? 8 : 0) : k_end - k0 - k);
         u32x4 p[P];
-        v.terms(sel, p);
+        v.terms(sel, cols, p);
         unsigned short* to = s + k / kK * (P * plane) + (cols ? k % kK * TT + ((row / 8) ^ Cols::swizzle(k % kK)) * 8 : row * kPitch + k % kK);
 #pragma unroll
         for (int i = 0; i < P; ++i) *reinterpret_cast<u32x4*>(to + i * plane) = p[i];
