@@ -522,9 +522,11 @@ int nrf_expert_plan(const int32_t* index, int64_t n_rows, int num_experts, void*
 
 /* y[i] = act(weight[index[i]] x[i] + bias[index[i]]); rows of no expert give zeros.  x (n_rows, n_in), weight
  * (num_experts, n_out, n_in), bias (num_experts, n_out) or NULL, y (n_rows, n_out), all of `dtype`; `plan` from
- * nrf_expert_plan with these n_rows and num_experts.  Sums are fp32, y is rounded once.  NRF_DTYPE_FP32 multiplies three
- * bf16 terms per operand (24 significand bits, the rule of nrf_mlp_forward_rays_bf16x3); there an operand that is not
- * finite gives NaN in every output it reaches. */
+ * nrf_expert_plan with these n_rows and num_experts.  Sums are fp32, y is rounded once.  NRF_DTYPE_FP32 has two forms.  Layers with
+ * n_in and n_out up to 64 multiply fp32 as it is.  Others multiply three bf16 terms per operand (24 significand bits, the rule of
+ * nrf_mlp_forward_rays_bf16x3; fewer under 2^-110, whose last terms are under bf16's smallest, and 3.3962e38 and more count
+ * as infinite).  A product of an operand that is not finite is not finite: NaN of three terms, infinite or NaN of fp32 and of the
+ * 16-bit types.  It reaches the outputs whose sums it is in, no others. */
 int nrf_expert_linear(const void* x, const void* weight, const void* bias, const void* plan, int64_t n_rows, int num_experts,
                       int n_in, int n_out, int dtype, int act, void* y, nrf_stream_t stream);
 
