@@ -838,14 +838,15 @@ int launch_cell_backward(const ExpertArgs& g, float* dx, hipStream_t stream) {
 }
 bool cells(int n_in, int n_out, int dtype) { return dtype == NRF_DTYPE_FP32 && n_in <= 64 && n_out <= 64; }
 
-// An expert's parts, added in their order; zeros for an expert without rows.  Many parts (an expert of thousands of rows) are dealt to
-// the four wavefronts, 64 outputs at a time, their sums joined in order; else 256 outputs at a time.  8.6 us for 4096 cells of 32 x 32
-// and 131 k rows, 8 us for 8 experts of 319 x 256 and 20 k rows: launch and one chain of loads.
+// An expert's parts, added in their order; zeros for an expert without rows.  256 outputs at a time; where there are FEW experts, an
+// expert's many parts are dealt to the four wavefronts, 64 outputs at a time, and their sums joined in order (for every number of
+// experts in one kernel: 13 us for 4096 cells of 32 x 32 and 131 k rows, this way 9).  8 us for 8 experts of 319 x 256 and 20 k rows: launch
+// and one chain of loads.
 constexpr int kManyParts = 32;
-template <class T>
+template <class T, bool FEW>
 __global__ __launch_bounds__(256) void expert_sum_kernel(ExpertArgs g) {
     typedef typename Traits<T>::elem elem;
-    __shared__ double s_sum[4][64];
+    __shared__ double s_sum[FEW ? 4 : 1][64];
     const PlanLayout L(g.n, g.E);
     const int expert = blockIdx.y, rows = g.plan[expert], wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const bool by_runs = g.splits == 0;
@@ -853,7 +854,7 @@ __global__ __launch_bounds__(256) void expert_sum_kernel(ExpertArgs g) {
     const int64_t size = part_size(g.n_in, g.n_out), weights = int64_t(g.n_out) * g.n_in;
     const int64_t first = by_runs ? (g.plan[L.offsets + expert] >> 8) + expert : expert, step = by_runs ? 1 : g.E;
     const int parts = by_runs ? (rows + kPartRows - 1) / kPartRows : g.splits;
-    const bool dealt = parts >= kManyParts;
+    const bool dealt = FEW && parts >= kManyParts;
     const int wide = dealt ? 64 : 256, begin = dealt ? int(int64_t(parts) * wave / 4) : 0, end = dealt ? int(int64_t(parts) * (wave + 1) / 4) : parts;
     for (int64_t base = int64_t(blockIdx.x) * wide; base < size; base += int64_t(gridDim.x) * wide) {
         const int64_t i = base + (dealt ? lane : int(threadIdx.x));
@@ -937,10 +938,11 @@ void launch_sum(int dtype, const ExpertArgs& g, hipStream_t stream) {
     // expert 645 -> 235 us, 8 experts 261 -> 209, 2 M rows of one expert 6.6 -> 2.1 ms; 4096 cells of 32 x 32 keep one each)
     const int64_t size = part_size(g.n_in, g.n_out), least = size > 8192 ? (size + 255) / 256 : (size + 2047) / 2048, most = (size + 63) / 64;
     const int64_t want = (1024 + g.E - 1) / g.E, blocks = want < least ? least : want < most ? want : most;
+    const bool few = want > least;
     const dim3 grid(unsigned(blocks < 1024 ? blocks : 1024), unsigned(g.E));
-    if (dtype == NRF_DTYPE_FP32) expert_sum_kernel<Fp32><<<grid, 256, 0, stream>>>(g);
-    else if (dtype == NRF_DTYPE_BF16) expert_sum_kernel<Bf16><<<grid, 256, 0, stream>>>(g);
-    else expert_sum_kernel<Fp16><<<grid, 256, 0, stream>>>(g);
+    if (dtype == NRF_DTYPE_FP32) few ? expert_sum_kernel<Fp32, true><<<grid, 256, 0, stream>>>(g) : expert_sum_kernel<Fp32, false><<<grid, 256, 0, stream>>>(g);
+    else if (dtype == NRF_DTYPE_BF16) few ? expert_sum_kernel<Bf16, true><<<grid, 256, 0, stream>>>(g) : expert_sum_kernel<Bf16, false><<<grid, 256, 0, stream>>>(g);
+    else few ? expert_sum_kernel<Fp16, true><<<grid, 256, 0, stream>>>(g) : expert_sum_kernel<Fp16, false><<<grid, 256, 0, stream>>>(g);
 }
 
 bool shapes_ok(int64_t n, int E, int n_in, int n_out, int dtype, int act) {
