@@ -895,7 +895,8 @@ int tile_size(int form, int64_t n, int E, int n_in, int n_out, int splits) {
 }
 // How dW's sum over an expert's rows is cut (see ExpertArgs): not at all where the outputs alone give 512 workgroups; else by
 // runs, which balances uneven experts, while the parts stay under 1 GiB; else into equal shares.  Wide kernels: equal shares of
-// at least 512 rows of the average expert, enough for a workgroup per CU.
+// at least 512 rows of the average expert, enough for a workgroup per CU.  (The tiny fp32 layers' kernel always cuts by runs: its parts,
+// (n_in + 1) n_out words per 256 rows and per expert, are at most a quarter of what x, dy and the weights hold.)
 int dw_splits(int64_t n, int E, int n_in, int n_out, bool is_wide) {
     int64_t want, most;
     if (is_wide) {

@@ -156,8 +156,8 @@ __global__ __launch_bounds__(1024) void plan_chunks_kernel(int* __restrict__ his
     }
 }
 
-// The walk of 2 M rows over 4096 experts takes 21 us: 3 launch, 3.5 counting again, 3 sums and places, 10 ranks (13 ballots per 64
-// rows, a chain through the counters), the rest scattered 4 B stores; the tables beside it 5.  2048 rows in one workgroup: 5 us.
+// The walk of 2 M rows over 4096 experts takes 21 us: 3 launch, 3.5 counting again, 3 sums and places, 10 ranks (15 ballots per 64
+// rows, 8 up to 255 experts, a chain through the counters), the rest scattered 4 B stores; the tables beside it 5.  2048 rows in one workgroup: 5 us.
 // Workgroups 0 .. kTableBlocks - 1: the run tables, kTableShares for each table; table 0's also write counts and offsets.  Those
 // behind them: the walk.  SINGLE: one workgroup does it all.
 constexpr int kTableShares = 2, kTableBlocks = nrf::kTileTables * kTableShares;
@@ -351,8 +351,9 @@ NRF_EXPORT int nrf_expert_plan(const int32_t* index, int64_t n_rows, int num_exp
         return NRF_ERR_LAUNCH;
     plan_hist_kernel<<<dim3(unsigned(chunks)), 512, hist_lds, stream>>>(index, n_rows, E, chunk, hist);
     plan_chunks_kernel<<<dim3(unsigned(E / 64 + 1)), 1024, 0, stream>>>(hist, int(chunks), E, totals);
-    // sixteen wavefronts hide more of a long chunk's latency than their counters cost (2 M rows, 4096 experts: 22.7 us for 24.5;
-    // 262 k rows: 12.7 for 10.4)
+    // sixteen wavefronts hide more of a long chunk's latency than their counters cost (2 M rows in runs of one expert, 4096 of them:
+    // 22.7 us for 24.5; 262 k rows: 12.7 for 10.4).  Rows of any order: the whole call takes 35 us for 44 with 1024 experts, 55 for 52
+    // with 4096 and 61 for 56 with 64; between the two lengths neither wins everywhere
     const int st = wide            ? launch_place<2, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream)
                    : chunk >= 6000 ? launch_place<16, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream)
                                    : launch_place<8, false>(index, n_rows, E, chunk, chunks, hist, totals, out, stream);

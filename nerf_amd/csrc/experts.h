@@ -8,8 +8,8 @@
 //   tiles    for 32, 64, 128 and 256 rows: {first grouped place, rows << 16 | expert} of the runs of at most that many rows of
 //            one expert ("expert" E: the rows of no expert): first, in grouped order, the long runs (all but those of half
 //            the length and less: as costly as whole ones, next to the runs that share their weights), then the short rests
-//            (a product's last workgroups are then its shortest; 32 k rows, 32 experts of 2048 x 2048: 297 - 311 us, with
-//            every rest at the end 317 - 376, with none there 302 - 323)
+//            (a product's last workgroups are then its shortest; 32 k rows, 32 experts of 2048 x 2048, five routings: 375 -
+//            398 us, with every rest at the end 397 - 406, with none there 381 - 396)
 // A table of runs of 2^s rows has at most (n >> s) + E + 1 entries, and no more than rows: the host sizes the products' grids
 // with that and never reads a count back; workgroups past the table's count leave at once.
 #pragma once

@@ -268,7 +268,7 @@ __global__ __launch_bounds__(256) void kilo_dir_table_kernel(const float* __rest
     }
 }
 
-// heads: dot products over the 16 registers of a block, two terms per v_pk_fma_f32
+// heads: dot products over the 16 registers of a block, two running sums (fp32 FMAs: the build keeps packed ones off)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float dot16(const f32x16& w, const f32x16& x) {
     f32x2 acc = {0.f, 0.f};

@@ -199,7 +199,7 @@ __device__ __forceinline__ void fold_slice(f32x16& y, const f32x16& base, const 
     for (int t = 0; t < 16; ++t)
         if (t >= t0 && t < t1) v[t] = fmaf(yl[t], kLoUnscale, base[t]);
 #else
-    // two elements per instruction (v_pk_fma_f32); every slice is a whole number of even-aligned pairs
+    // written two elements at a time (two v_fma_f32: the build keeps packed fp32 off); every slice is a whole number of even-aligned pairs
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     const f32x2 c = {kLoUnscale, kLoUnscale};
 #pragma unroll

@@ -12,11 +12,12 @@
 // The scale keeps lo a normal fp16 number for every entry above 2^-15 and the largest entry possible (|X| <= 1.3,
 // |A| <= 1.6, |Q| <= 8 for the coefficients the entry points admit) below fp16's 65504.  |G|_F is summed in float64.
 //
-// Two paths, by the shorter side M and the longer side N:
+// Four paths, by the shorter side M and the longer side N:
 //   M <= 32, N <= 128                       one wavefront per matrix, everything in registers (schulz_small_kernel);
 //   M <= 64, N <= 544 and M <= 128, N <= 160  one workgroup per matrix, everything in LDS (schulz_block_kernel);
-//   otherwise                               the matrices' terms in the workspace: a launch per step up to 64 x 640 and 128 x 320
-//                                           (schulz_step_kernel), else three (schulz_product_kernel).
+//   M <= 64, N <= 640 and M <= 128, N <= 320  the matrices' terms in the workspace, a launch per step (schulz_step_kernel), up to
+//                                           256 pieces of 64 columns in all;
+//   otherwise                               the same, three launches per step (schulz_product_kernel).
 #include "dma_gemm.h"
 #include "launch.h"
 #include "split2h.h"
@@ -97,9 +98,11 @@ __device__ __forceinline__ float start_scale(double sum, float eps) {
     return float(4096.0 / norm);
 }
 
-// a, b -> the packed pairs of their terms hi and lo (a, b already scaled; results of vector arithmetic, not of an MFMA).  The
-// residual is taken from the packed word itself: written as a - float((_Float16)a), the compiler converts twice, once with
-// the scaling folded in, and where the two round a tie apart lo belongs to another hi (2^-11 off, one entry in some thousands).
+// a, b -> the packed pairs of their terms hi and lo (a, b already scaled).  The residual is taken from the packed word itself:
+// written as a - float((_Float16)a), the compiler converts twice, once with the scaling folded in, and where the two round a tie
+// apart lo belongs to another hi (2^-11 off, one entry in some thousands).  The residuals' asm may read an MFMA's result, for
+// which the compiler adds no wait inside asm: it needs `hi`, and the conversion that makes it, the compiler's own, reads a and b
+// first and waits.  So no asm in here may read a or b without `hi`.
 __device__ __forceinline__ void split_pair_h2(float a, float b, unsigned& hi, unsigned& lo) {
     hi = pk_f16(a, b);
     lo = pk_f16(f16_residual_lo(a, hi), f16_residual_hi(b, hi));
@@ -477,7 +480,9 @@ __global__ __launch_bounds__(512) void schulz_block_kernel(SchulzArgs s, BlockSh
 // Each sums all of A = X X^T itself (X's 64-column pieces pass through a ring in LDS, its own piece stays), squares it, and
 // multiplies its own columns: one launch per step for three, at the price of A's sums once per workgroup (0.7 us per piece at 128
 // rows).  One round of workgroups, up to 10 pieces at 64 rows and 5 at 128: 64 x 600 80 -> 45 us, 128 x 200 73 -> 64, 2 of 128 x 283
-// 75 -> 70, 50 of 128 x 300 106 -> 91; past that the tiles below win (128 x 640 85 us, 96 this way).
+// 75 -> 70, 50 of 128 x 300 106 -> 91.  At 128 rows one or two matrices are even with the tiles below at 384 columns (75 us both) and
+// slower from 448 on (80 for 78; 640: 96 for 85), twenty are faster up to 640 (107 for 110); at 64 rows this way would win up to 1024
+// columns where the pieces are one round (58 us for 90), even where they are two.
 template <int MB> struct StepShape {
     typedef DmaSide<kRows, 16 * MB, 64, 2, kBlockWaves> Side;
     static constexpr int kSquare = MB * 32 + 16, kSquareBytes = 2 * 16 * MB * kSquare;

@@ -25,8 +25,8 @@ __device__ __forceinline__ void split_pair(float a, float b, unsigned& p0, unsig
     p1 = pk_bf16(ra, rb);
     p2 = pk_bf16(__fsub_rn(ra, bf_lo(p1)), __fsub_rn(rb, bf_hi(p1)));
 }
-// the same split with the two residual subtractions as one v_pk_add_f32 each (9 instead of 11 instructions per pair; same
-// bits: the packed op is two IEEE fp32 subtractions) -- for the kernels whose splits are not hand-sliced into MFMA gaps
+// the same split, the same bits, with the two residual subtractions written as one of pairs -- for the kernels whose splits are not
+// hand-sliced into MFMA gaps.  The build keeps packed fp32 instructions off, so each is two v_sub_f32
 typedef float f32x2_s3 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split_pair_pk(float a, float b, unsigned& p0, unsigned& p1, unsigned& p2) {
     p0 = pk_bf16(a, b);
