@@ -840,7 +840,7 @@ bool cells(int n_in, int n_out, int dtype) { return dtype == NRF_DTYPE_FP32 && n
 
 // An expert's parts, added in their order; zeros for an expert without rows.  256 outputs at a time; where there are FEW experts, an
 // expert's many parts are dealt to the four wavefronts, 64 outputs at a time, and their sums joined in order (for every number of
-// experts in one kernel: 13 us for 4096 cells of 32 x 32 and 131 k rows, this way 9).  8 us for 8 experts of 319 x 256 and 20 k rows: launch
+// experts in one kernel: 13 us for 4096 cells of 32 x 32 and 131 k rows, this way 7 - 9).  7 us for 8 experts of 319 x 256 and 20 k rows: launch
 // and one chain of loads.
 constexpr int kManyParts = 32;
 template <class T, bool FEW>
