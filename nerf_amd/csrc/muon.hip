@@ -1054,7 +1054,7 @@ int run(const SchulzArgs& s, void* workspace, hipStream_t stream) {
 bool schulz_shape_ok(int64_t batch, int rows, int cols) {
     if (batch < 0 || rows < 1 || cols < 1 || rows > 65536 || cols > 65536) return false;
     if (small_path(rows, cols) || block_path(rows, cols)) return batch <= int64_t(1) << 24;
-    const LargeShape L = large_shape(rows, cols);
+    const LargeShape L = large_shape(rows, cols);       // (2^24 tiles are 1 TB of workspace: no launch comes near 2^32 work-items)
     return batch <= 65535 && batch * (int64_t(L.Mp / 64) * (L.Np / 64)) <= int64_t(1) << 24;
 }
 // the iteration on the singular values, which start in [0, 1]: entries of X, A and Q must stay inside fp16 at scale 2^12
